@@ -47,6 +47,8 @@ class BlockParams(ctypes.Structure):
 
 DTYPE_F32, DTYPE_F64, DTYPE_I32, DTYPE_BOOL, DTYPE_I64 = 0, 1, 2, 3, 4
 DTYPE_BF16, DTYPE_F16 = 5, 6
+FORMAT_E4M3, FORMAT_E5M2 = 0, 1
+BLOCKS_ROWS, BLOCKS_TILES = 0, 1
 GEMM_3XTF32, GEMM_EXACT_TREE = 0, 1
 DGEMM_AUTO, DGEMM_DMMA, DGEMM_FFMA = 0, 1, 2
 ROWS_EXACT, ROWS_FAST = 0, 1
@@ -167,6 +169,17 @@ SIGNATURES = {
     "chelis_cuda_gelu_adjoint_f32": (c_int, [c_vp, c_vp, c_vp, c_i64]),
     "chelis_cuda_layer_norm_bwd_f32": (c_int, [c_vp, c_vp, c_f32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "chelis_cuda_cross_entropy_f32": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
+    "chelis_cuda_expert_route": (c_int, [c_i32, c_vp, c_i64, c_i32, c_i32, c_int, c_vp, c_vp]),
+    "chelis_cuda_expert_route_bwd": (c_int, [c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_int, c_vp]),
+    "chelis_cuda_expert_sort": (c_int, [c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "chelis_cuda_expert_spread": (c_int, [c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i64, c_vp]),
+    "chelis_cuda_expert_combine": (c_int, [c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i64, c_vp]),
+    "chelis_cuda_expert_combine_bwd": (c_int, [c_i32] + [c_vp] * 5 + [c_i64, c_i32, c_i64, c_vp, c_vp]),
+    "chelis_cuda_quantize8": (c_int, [c_i32, c_i32, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "chelis_cuda_quantize8_places": (c_i64, [c_i64, c_i32]),
+    "chelis_cuda_quantize8_transposed": (c_int, [c_i32, c_i32, c_vp, c_vp, c_i32, c_i64, c_i64, c_vp, c_vp]),
+    "chelis_cuda_matmul8": (c_int, [c_i32, c_i32, c_int, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_i32, c_vp]),
+    "chelis_cuda_matmul8_wgrad": (c_int, [c_i32, c_i32, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_i32, c_vp]),
     "chelis_cuda_dp_shard": (c_int, [c_i64, c_i32, c_i32, ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "chelis_cuda_dp_unique_id": (c_int, [c_vp]),
     "chelis_cuda_dp_init": (c_int, [c_i32, c_i32, c_vp]),

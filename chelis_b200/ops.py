@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -518,3 +519,271 @@ def cross_entropy(logits, labels, want_grad: bool = True):
     L.call("chelis_cuda_cross_entropy_f32", logits.data_ptr(), labels.data_ptr(), rows, classes,
            loss.data_ptr(), _ptr(dz))
     return loss, dz
+
+
+# ---------------------------------------------------------------- routed feed-forward
+
+_ACT = {torch.float32: L.DTYPE_F32, torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
+_FLOAT8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+_FORMAT = {torch.float8_e4m3fn: L.FORMAT_E4M3, torch.float8_e5m2: L.FORMAT_E5M2}
+
+
+class ExpertOrder(NamedTuple):
+    """The (token, slot) pairs sorted by expert (expert_sort), all int32."""
+    offsets: torch.Tensor   # [experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1]
+    position: torch.Tensor  # [tokens, k]: each pair's row, -1 for a pair with none
+    source: torch.Tensor    # [tokens * k]: each row's pair, -1 for a row that no pair takes
+
+
+class Blocks8(NamedTuple):
+    """A matrix in 8-bit floating point with a scale for each block of 128.
+    Its numbers are data times the scale of their block."""
+    data: torch.Tensor    # float8_e4m3fn or float8_e5m2, [..., rows, cols rounded up to 16]
+    scales: torch.Tensor  # f32; rows: [ceil(cols / 128), rows]; tiles: [..., ceil(rows / 128), ceil(cols / 128)]
+    cols: int             # numbers in a row; the bytes past them are zero
+    blocks: str           # "rows" (1 x 128) or "tiles" (128 x 128)
+
+
+def _act(name: str, t: torch.Tensor) -> int:
+    if t.dtype not in _ACT:
+        raise ValueError(f"{name} takes f32, bf16 or f16 tensors")
+    return _ACT[t.dtype]
+
+
+def _check(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _check_i32(name: str, *tensors: torch.Tensor) -> None:
+    _check(all(t.dtype == torch.int32 for t in tensors), f"{name} takes int32 indices")
+
+
+def _check_order(name: str, order: ExpertOrder) -> None:
+    _check_i32(name, *order)
+    _check(order.position.dim() == 2 and order.offsets.dim() == 1 and order.offsets.numel() >= 2
+           and order.source.shape == (order.position.numel(),), f"{name} takes expert_sort's order")
+
+
+def _routed(order: ExpertOrder) -> int:
+    """The device address of the number of rows that a pair takes."""
+    return order.offsets.data_ptr() + 4 * (order.offsets.numel() - 1)
+
+
+def expert_route(logits: torch.Tensor, k: int, renormalize: bool = True):
+    """The router: (weights f32 [tokens, k], experts int32 [tokens, k]), the k
+    largest of the softmax of logits [tokens, experts], with renormalize over
+    the chosen alone.  Ties go to the lowest index; an expert at -inf is never
+    chosen (id -1, weight 0 where fewer than k are left)."""
+    dt = _act("expert_route", logits)
+    _check(logits.dim() == 2, "expert_route takes logits [tokens, experts]")
+    _prepare(logits)
+    tokens, experts = logits.shape
+    weights = torch.empty((tokens, max(k, 0)), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((tokens, max(k, 0)), dtype=torch.int32, device=logits.device)
+    L.call("chelis_cuda_expert_route", dt, logits.data_ptr(), tokens, experts, k, int(renormalize),
+           weights.data_ptr(), ids.data_ptr())
+    return weights, ids
+
+
+def expert_route_bwd(logits: torch.Tensor, experts: torch.Tensor, dweights: torch.Tensor,
+                     renormalize: bool = True) -> torch.Tensor:
+    """dlogits of expert_route, given the experts that it chose."""
+    dt = _act("expert_route_bwd", logits)
+    _check_i32("expert_route_bwd", experts)
+    _check(logits.dim() == 2 and experts.dim() == 2 and experts.shape == dweights.shape
+           and experts.shape[0] == logits.shape[0] and dweights.dtype == torch.float32,
+           "expert_route_bwd takes logits [tokens, experts] and experts, f32 dweights [tokens, k]")
+    _prepare(logits, experts, dweights)
+    dlogits = torch.empty_like(logits)
+    L.call("chelis_cuda_expert_route_bwd", dt, logits.data_ptr(), experts.data_ptr(),
+           dweights.data_ptr(), logits.shape[0], logits.shape[1], experts.shape[1],
+           int(renormalize), dlogits.data_ptr())
+    return dlogits
+
+
+def expert_sort(experts: torch.Tensor, n_experts: int) -> ExpertOrder:
+    """The stable order by expert of the (token, slot) pairs of experts
+    [tokens, k]; an id of -1 is a pair that goes nowhere.  Other ids outside
+    [0, n_experts) count as -1 and raise at the next device_status()."""
+    _check_i32("expert_sort", experts)
+    _check(experts.dim() == 2, "expert_sort takes experts [tokens, k]")
+    _prepare(experts)
+    dev = experts.device
+    order = ExpertOrder(torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev),
+                        torch.empty_like(experts),
+                        torch.empty(experts.numel(), dtype=torch.int32, device=dev))
+    L.call("chelis_cuda_expert_sort", experts.data_ptr(), experts.shape[0], experts.shape[1],
+           n_experts, *(t.data_ptr() for t in order))
+    return order
+
+
+def expert_gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """Token rows x [tokens, hidden] to their experts' rows [tokens * k,
+    hidden]; rows that no pair takes (the last ones) are zeros."""
+    dt = _act("expert_gather", x)
+    _check_order("expert_gather", order)
+    _check(x.dim() == 2 and x.shape[0] == order.position.shape[0],
+           "expert_gather takes x [tokens, hidden]")
+    _prepare(x, *order)
+    tokens, k = order.position.shape
+    xs = torch.empty((tokens * k, x.shape[1]), dtype=x.dtype, device=x.device)
+    L.call("chelis_cuda_expert_spread", dt, x.data_ptr(), order.position.data_ptr(), _routed(order),
+           tokens, k, x.shape[1], xs.data_ptr())
+    return xs
+
+
+def _expert_combine(name, ys, weights, order):
+    dt = _act(name, ys)
+    _check_order(name, order)
+    tokens, k = order.position.shape
+    _check(ys.dim() == 2 and ys.shape[0] == tokens * k, f"{name} takes rows [tokens * k, hidden]")
+    _check(weights is None or (weights.dtype == torch.float32 and weights.shape == (tokens, k)),
+           f"{name} takes f32 weights [tokens, k]")
+    _prepare(ys, weights, *order)
+    y = torch.empty((tokens, ys.shape[1]), dtype=ys.dtype, device=ys.device)
+    L.call("chelis_cuda_expert_combine", dt, ys.data_ptr(), _ptr(weights), order.position.data_ptr(),
+           tokens, k, ys.shape[1], y.data_ptr())
+    return y
+
+
+def expert_gather_bwd(dxs: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """dx of expert_gather: each token's rows summed in slot order."""
+    return _expert_combine("expert_gather_bwd", dxs, None, order)
+
+
+def expert_combine(ys: torch.Tensor, weights: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """The way back: y[t] = sum_j weights[t, j] * ys[position[t, j]], f32 sums
+    in slot order."""
+    _check(weights is not None, "expert_combine takes weights")
+    return _expert_combine("expert_combine", ys, weights, order)
+
+
+def expert_combine_bwd(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, order: ExpertOrder):
+    """(dys, dweights) of expert_combine."""
+    dt = _act("expert_combine_bwd", dy)
+    _check_order("expert_combine_bwd", order)
+    tokens, k = order.position.shape
+    _check(ys.dtype == dy.dtype and dy.dim() == 2 and dy.shape[0] == tokens
+           and ys.shape == (tokens * k, dy.shape[1]),
+           "expert_combine_bwd takes dy [tokens, hidden] and rows [tokens * k, hidden] of one dtype")
+    _check(weights.dtype == torch.float32 and weights.shape == (tokens, k),
+           "expert_combine_bwd takes f32 weights [tokens, k]")
+    _prepare(dy, ys, weights, *order)
+    dys = torch.empty_like(ys)
+    dweights = torch.empty_like(weights)
+    L.call("chelis_cuda_expert_combine_bwd", dt, dy.data_ptr(), ys.data_ptr(), weights.data_ptr(),
+           order.position.data_ptr(), _routed(order), tokens, k, dy.shape[1], dys.data_ptr(),
+           dweights.data_ptr())
+    return dys, dweights
+
+
+def _ceil(a: int, b: int) -> int:
+    return -(-a // b)
+
+
+def quantize8(x: torch.Tensor, format: str = "e4m3", blocks: str = "rows") -> Blocks8:
+    """x in 8 bits (e4m3 or e5m2) with a power-of-two scale for each block of
+    128: along its rows ("rows", x [rows, cols]; activations, gradients) or
+    128 x 128 ("tiles", x [rows, cols] or [experts, rows, cols]; weights)."""
+    dt = _act("quantize8", x)
+    _check(format in _FLOAT8, "8-bit formats are e4m3 and e5m2")
+    _check(blocks in ("rows", "tiles"), "blocks are rows or tiles")
+    _check(x.dim() == 2 or (x.dim() == 3 and blocks == "tiles"),
+           "quantize8 takes a matrix, or a stack of matrices in tiles")
+    _prepare(x)
+    rows, cols = x.shape[-2:]
+    batch = x.shape[0] if x.dim() == 3 else 1
+    kb = _ceil(cols, 128)
+    data = torch.empty((*x.shape[:-1], _ceil(cols, 16) * 16), dtype=_FLOAT8[format], device=x.device)
+    shape = (kb, rows) if blocks == "rows" else (*x.shape[:-2], _ceil(rows, 128), kb)
+    scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    L.call("chelis_cuda_quantize8", dt, _FORMAT[data.dtype],
+           L.BLOCKS_ROWS if blocks == "rows" else L.BLOCKS_TILES, x.data_ptr(), batch, rows, cols,
+           data.data_ptr(), scales.data_ptr())
+    return Blocks8(data, scales, cols, blocks)
+
+
+def quantize8_transposed(x: torch.Tensor, format: str = "e4m3",
+                         offsets: torch.Tensor | None = None) -> Blocks8:
+    """x [rows, cols] turned over and in 8 bits, blocks of 128 of its rows: the
+    operand of matmul8_wgrad.  With offsets (expert_sort's) each expert's rows
+    start on a block of their own."""
+    dt = _act("quantize8_transposed", x)
+    _check(format in _FLOAT8, "8-bit formats are e4m3 and e5m2")
+    _check(x.dim() == 2, "quantize8_transposed takes a matrix")
+    groups = 0
+    if offsets is not None:
+        _check_i32("quantize8_transposed", offsets)
+        _check(offsets.dim() == 1 and offsets.numel() >= 2, "offsets are [experts + 1]")
+        groups = offsets.numel() - 1
+    _prepare(x, offsets)
+    rows, cols = x.shape
+    places = int(L.load().chelis_cuda_quantize8_places(rows, groups))
+    data = torch.empty((cols, places), dtype=_FLOAT8[format], device=x.device)
+    scales = torch.empty((places // 128, cols), dtype=torch.float32, device=x.device)
+    L.call("chelis_cuda_quantize8_transposed", dt, _FORMAT[data.dtype], x.data_ptr(), _ptr(offsets),
+           groups, rows, cols, data.data_ptr(), scales.data_ptr())
+    return Blocks8(data, scales, places, "rows")
+
+
+def _check_blocks8(name: str, b: Blocks8, blocks: str) -> None:
+    _check(b.blocks == blocks and b.data.dtype in _FORMAT and b.scales.dtype == torch.float32,
+           f"{name} takes 8-bit {blocks} with f32 scales here")
+    rows, kb = b.data.shape[-2], _ceil(b.cols, 128)
+    shape = (kb, rows) if blocks == "rows" else (*b.data.shape[:-2], _ceil(rows, 128), kb)
+    _check(b.data.shape[-1] == _ceil(b.cols, 16) * 16 and tuple(b.scales.shape) == shape,
+           f"{name}: data and scales do not belong together")
+
+
+def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor | None = None,
+            dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a . b^T (b [n, k]: a layer's product) or a . b (trans_b=False, b [k, n]:
+    its input gradient, from the same weights) of 8-bit row blocks a [rows, k]
+    and tiles b; f32 sums, rounded once to dtype.  With offsets (expert_sort's)
+    b is a stack of matrices and rows [offsets[e], offsets[e + 1]) meet matrix
+    e; rows that no expert holds come out as zeros."""
+    _check(dtype in _ACT, "matmul8 gives f32, bf16 or f16")
+    _check_blocks8("matmul8", a, "rows")
+    _check_blocks8("matmul8", b, "tiles")
+    _check(a.data.dim() == 2 and b.data.dim() == (2 if offsets is None else 3),
+           "matmul8 takes a matrix b, or a stack of them with offsets")
+    groups = 1
+    if offsets is not None:
+        _check_i32("matmul8", offsets)
+        groups = b.data.shape[0]
+        _check(offsets.shape == (groups + 1,), "offsets are [experts + 1]")
+    n, k = (b.data.shape[-2], b.cols) if trans_b else (b.cols, b.data.shape[-2])
+    _check(a.cols == k, f"contraction extents differ: {a.cols} vs {k}")
+    _prepare(a.data, a.scales, b.data, b.scales, offsets)
+    rows = a.data.shape[0]
+    out = torch.empty((rows, n), dtype=dtype, device=a.data.device)
+    L.call("chelis_cuda_matmul8", _FORMAT[a.data.dtype], _FORMAT[b.data.dtype], int(trans_b), rows, n,
+           k, a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
+           _ptr(offsets), groups, _ACT[dtype], out.data_ptr())
+    return out
+
+
+def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
+                  dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The weight gradient dy^T . x [n, k] from the transposed 8-bit forms of
+    dy [rows, n] and x [rows, k] (quantize8_transposed); with offsets one
+    matrix an expert, [experts, n, k], zeros for an expert without rows."""
+    _check(dtype in _ACT, "matmul8_wgrad gives f32, bf16 or f16")
+    _check_blocks8("matmul8_wgrad", dy, "rows")
+    _check_blocks8("matmul8_wgrad", x, "rows")
+    _check(dy.cols == x.cols and dy.cols % 128 == 0, "matmul8_wgrad takes operands over the same rows")
+    n, k = dy.data.shape[0], x.data.shape[0]
+    groups = 0
+    if offsets is not None:
+        _check_i32("matmul8_wgrad", offsets)
+        _check(offsets.dim() == 1 and offsets.numel() >= 2, "offsets are [experts + 1]")
+        groups = offsets.numel() - 1
+        _check(dy.cols >= 128 * groups, "the operands were not turned over with these offsets")
+    _prepare(dy.data, dy.scales, x.data, x.scales, offsets)
+    shape = (n, k) if offsets is None else (groups, n, k)
+    out = torch.empty(shape, dtype=dtype, device=dy.data.device)
+    L.call("chelis_cuda_matmul8_wgrad", _FORMAT[dy.data.dtype], _FORMAT[x.data.dtype], n, k, dy.cols,
+           dy.data.data_ptr(), dy.scales.data_ptr(), x.data.data_ptr(), x.scales.data_ptr(),
+           _ptr(offsets), max(groups, 1), _ACT[dtype], out.data_ptr())
+    return out

@@ -598,6 +598,85 @@ int chelis_cuda_dp_world(int32_t *nranks, int32_t *rank);
 int chelis_cuda_dp_finalize(int32_t abort);
 
 /* =========================================================================
+ * Routed (mixture-of-experts) feed-forward, new: the reference's DAG has no
+ * routed layer and no 8-bit dtype.  T tokens, E experts (at most 1024), k
+ * slots a token (at most 32); activations are f32, bf16 or f16.
+ * ========================================================================= */
+/* The k experts of each token with the largest logits [T][E] (ties: the
+ * lowest index first; an expert at -inf is never chosen) and their softmax
+ * probabilities, renormalize != 0: over the chosen alone.  ids [T][k] in
+ * falling order of the logit, -1 with weight 0 where fewer than k are left.
+ * A NaN anywhere in a row makes its weights NaN. */
+int chelis_cuda_expert_route(int32_t dtype, const void *logits, int64_t tokens, int32_t experts,
+                             int32_t k, int renormalize, float *weights, int32_t *ids);
+/* The gradient of the weights for the logits, through the chosen ids. */
+int chelis_cuda_expert_route_bwd(int32_t dtype, const void *logits, const int32_t *ids,
+                                 const float *dweights, int64_t tokens, int32_t experts, int32_t k,
+                                 int renormalize, void *dlogits);
+/* The T * k (token, slot) pairs sorted by expert, stable: expert e's rows are
+ * [offsets[e], offsets[e + 1]) (offsets [E + 1]); position [T][k] is each
+ * pair's row and source [T * k] each row's pair.  An id of -1 is a pair with
+ * no row (position -1); rows from offsets[E] on have source -1.  Any other id
+ * outside [0, E) is taken as -1 and reported by chelis_cuda_device_status. */
+int chelis_cuda_expert_sort(const int32_t *ids, int64_t tokens, int32_t k, int32_t experts,
+                            int32_t *offsets, int32_t *position, int32_t *source);
+/* xs[position[t][j]] = x[t]; rows from *routed (= offsets[E]) on are zeros. */
+int chelis_cuda_expert_spread(int32_t dtype, const void *x, const int32_t *position,
+                              const int32_t *routed, int64_t tokens, int32_t k, int64_t hidden,
+                              void *xs);
+/* y[t] = sum_j weights[t][j] * ys[position[t][j]] in slot order, f32 sums; a
+ * pair with no row adds nothing.  weights == NULL: all ones, which makes it
+ * the gradient of chelis_cuda_expert_spread. */
+int chelis_cuda_expert_combine(int32_t dtype, const void *ys, const float *weights,
+                               const int32_t *position, int64_t tokens, int32_t k, int64_t hidden,
+                               void *y);
+/* dys[position[t][j]] = weights[t][j] * dy[t], zeros from *routed on;
+ * dweights[t][j] = <dy[t], ys[position[t][j]]>, 0 for a pair with no row. */
+int chelis_cuda_expert_combine_bwd(int32_t dtype, const void *dy, const void *ys,
+                                   const float *weights, const int32_t *position,
+                                   const int32_t *routed, int64_t tokens, int32_t k, int64_t hidden,
+                                   void *dys, float *dweights);
+
+/* ---- 8-bit matrices with a scale for each block of 128 ----
+ * A block's scale is the least power of two s >= 2^-126 with max|x| / s <=
+ * the format's largest value (448, 57344), over its finite elements; 1 for a
+ * block of zeros.  data holds x / s rounded to nearest even; an infinity is
+ * kept in e5m2 and becomes NaN in e4m3.  Layouts, with ld(c) = c rounded up
+ * to 16 and the bytes past c zero:
+ *   rows   data [rows][ld(cols)], scales [ceil(cols/128)][rows]
+ *   tiles  data [batch][rows][ld(cols)],
+ *          scales [batch][ceil(rows/128)][ceil(cols/128)]
+ * The products below take any f32 scales in these layouts. */
+enum { CHELIS_FORMAT_E4M3 = 0, CHELIS_FORMAT_E5M2 = 1 };
+enum { CHELIS_BLOCKS_ROWS = 0, CHELIS_BLOCKS_TILES = 1 };
+int chelis_cuda_quantize8(int32_t dtype, int32_t format, int32_t layout, const void *x,
+                          int64_t batch, int64_t rows, int64_t cols, uint8_t *data, float *scales);
+/* x turned over, for products that sum over its rows: data [cols][places],
+ * scales [places/128][cols], blocks of 128 rows.  With groups > 0, group g
+ * holds rows [offsets[g], offsets[g + 1]) and starts on a block of its own
+ * (the places left over hold zero); places =
+ * chelis_cuda_quantize8_places(rows, groups). */
+int64_t chelis_cuda_quantize8_places(int64_t rows, int32_t groups);
+int chelis_cuda_quantize8_transposed(int32_t dtype, int32_t format, const void *x,
+                                     const int32_t *offsets, int32_t groups, int64_t rows,
+                                     int64_t cols, uint8_t *data, float *scales);
+/* out[rows][n] = a . b^T (trans_b != 0, b [groups][n][k]) or a . b (b
+ * [groups][k][n]): a in rows layout, b in tiles layout, f32 sums rounded once
+ * to out_dtype.  Row r meets the matrix of the group that holds it; offsets
+ * == NULL: one matrix.  Rows that no group holds are written as zeros. */
+int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows, int64_t n,
+                        int64_t k, const uint8_t *a, const float *scales_a, const uint8_t *b,
+                        const float *scales_b, const int32_t *offsets, int32_t groups,
+                        int32_t out_dtype, void *out);
+/* out[g][n][k] = sum over group g's rows t of A[t][n] * B[t][k], from the
+ * transposed forms a [n][places] and b [k][places]; zeros for a group with no
+ * rows. */
+int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int64_t k, int64_t places,
+                              const uint8_t *a, const float *scales_a, const uint8_t *b,
+                              const float *scales_b, const int32_t *offsets, int32_t groups,
+                              int32_t out_dtype, void *out);
+
+/* =========================================================================
  * Generated-entry device ABI (emit.rs:838-958, `f_device`): inputs borrowed,
  * outputs newly allocated owners the caller releases.  One entry per program
  * this backend ships whole.
