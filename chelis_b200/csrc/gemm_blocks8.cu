@@ -11,11 +11,15 @@
 // expert, the rows [offsets[e], offsets[e + 1]) of a meet matrix e of w, and
 // dw has one matrix an expert, summed over that expert's blocks.
 //
-// One thread block works on 128 x 256 tiles of the result, one after the
-// other (320 threads):
+// A thread block works on 128 x 256 tiles of the result, one after the other;
+// a pair of blocks (PAIR, cta_group::2) on 256 x 256 tiles, each with its 128
+// rows of a and half of b's columns in shared memory and its 128 rows of the
+// sums in tensor memory.  384 threads:
 //   warp 0      TMA producer (one elected lane)
-//   warp 1      TMEM allocator + tcgen05.mma kind::f8f6f4 issuer (one lane)
-//   warps 2-9   fold: the block's sum in tensor memory times its scales into
+//   warp 1      TMEM allocator + tcgen05.mma kind::f8f6f4 issuer (one lane,
+//               of a pair's first block)
+//   warp 2      the blocks' scales into a ring of their own (cp.async)
+//   warps 4-11  fold: a block's sum in tensor memory times its scales into
 //               f32 registers, then the store
 // The scales differ from block to block, so the tensor core sums one block
 // of 128 (four MMAs of K = 32) from a fresh start, alternating between two
@@ -38,15 +42,22 @@ extern std::atomic<uint64_t> g_launches;
 namespace gemm8 {
 
 constexpr int BM = 128, BN = 256, BK = 128;  // one scale block of K = 128 bytes = one swizzle row
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BOX_BYTES = 128 * BK;          // 128 rows or columns of one block
+constexpr int RING_BYTES = 12 * BOX_BYTES;   // 4 stages of 3 boxes, or 6 of 2 (PAIR)
+constexpr int SCALE_SLOTS = 8;
+constexpr int SLOT_FLOATS = BM + BN;  // row scales, then column scales (or one for each 128 columns)
 constexpr int FOLD_WARPS = 8;
-constexpr int THREADS = 64 + 32 * FOLD_WARPS;
+constexpr int THREADS = 128 + 32 * FOLD_WARPS;
+// Registers: a launch of 384 threads at 168 gives the first warpgroup's share
+// to the fold (128 x 56 + 256 x 224 = 384 x 168), which keeps 128 sums and
+// two 32-column loads of tensor memory in flight.
+constexpr int LAUNCH_REGS = 168, FEW_REGS = 56, FOLD_REGS = 224;
+static_assert(128 * FEW_REGS + 32 * FOLD_WARPS * FOLD_REGS <= THREADS * LAUNCH_REGS, "register split");
 constexpr uint32_t ACC_COLS = 256, TMEM_COLS = 512;
 constexpr int MAX_GROUPS = experts::MAX_EXPERTS;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ +
-                           FOLD_WARPS * BK * 4 /*column scales*/ + (MAX_GROUPS + 1) * 4 /*tile starts*/;
+constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + 512 /*barriers*/ +
+                           SCALE_SLOTS * SLOT_FLOATS * 4 + (MAX_GROUPS + 1) * 4 /*tile starts*/;
+constexpr uint64_t DRAIN_NS = 200000;  // bounded drain of an aborted pair's second block
 
 struct Params {
     int64_t rows;     // rows of a: tokens (forward, input gradient), outputs (weight gradient)
@@ -63,14 +74,55 @@ struct Params {
     uint32_t idesc;
 };
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                        uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// 4 bytes from global to shared memory, zero when !ok.
+__device__ __forceinline__ void cp_async4(float *dst, const float *src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(ok ? 4 : 0)
+                 : "memory");
+}
+// Arrive once this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Two f32 at a time: (lo, hi) in one 64-bit register pair.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // MN-major 8-bit operand: boxes of 128 (MN) x 128 (K) bytes, one 128-byte row
@@ -108,17 +160,17 @@ struct Tile {
     int kb0, kbs;       // contraction blocks
 };
 
-// `start` is, by group, the prefix of row tiles (forward, input gradient) or
-// of contraction blocks (weight gradient).
-template <bool WG>
+// `start` is, by group, the prefix of row tiles of TM rows (forward, input
+// gradient) or of contraction blocks (weight gradient).
+template <bool WG, int TM>
 __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, int64_t L) {
     const int64_t nt = (p.n + BN - 1) / BN;
     Tile t;
     if (WG) {
-        const int64_t mt = (p.rows + BM - 1) / BM;
+        const int64_t mt = (p.rows + TM - 1) / TM;
         t.group = static_cast<int>(L / (mt * nt));
         const int64_t in = L - t.group * mt * nt;
-        t.m0 = (in % mt) * BM;
+        t.m0 = (in % mt) * TM;
         t.n0 = (in / mt) * BN;
         t.m_end = p.rows;
         t.kb0 = start[t.group];
@@ -134,7 +186,7 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, i
         const int64_t in = L - start[lo] * nt, mt = start[lo + 1] - start[lo];
         int64_t a, b;
         group_span(p, p.rows, lo, &a, &b);
-        t.m0 = a + (in % mt) * BM;
+        t.m0 = a + (in % mt) * TM;
         t.n0 = (in / mt) * BN;
         t.m_end = b;
         t.kb0 = 0;
@@ -143,68 +195,135 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, i
     return t;
 }
 
-__device__ __forceinline__ void store_row(const Params &p, const float (&run)[128], int64_t index,
+// 32 bytes at once (a whole sector of a row).
+__device__ __forceinline__ void store32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t round2(float2 v, bool bf) {
+    if (bf) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// This thread's row, 128 columns of which `left` lie in the result.
+__device__ __forceinline__ void store_row(const Params &p, const f32x2 (&run)[64], int64_t index,
                                           int64_t left) {
     if (p.out_dtype == CHELIS_DTYPE_F32) {
         float *o = static_cast<float *>(p.out) + index;
-        if (left >= 128 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+        if (left >= 128 && (reinterpret_cast<uintptr_t>(o) & 31) == 0) {
 #pragma unroll
-            for (int j = 0; j < 128; j += 4)
-                *reinterpret_cast<float4 *>(o + j) = make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+            for (int j = 0; j < 64; j += 4) {
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = unpack2(run[j + i]);
+                    w[2 * i] = __float_as_uint(v.x);
+                    w[2 * i + 1] = __float_as_uint(v.y);
+                }
+                store32(o + 2 * j, w);
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 128; ++j)
-                if (j < left) o[j] = run[j];
+            for (int j = 0; j < 64; ++j) {
+                const float2 v = unpack2(run[j]);
+                if (2 * j < left) o[2 * j] = v.x;
+                if (2 * j + 1 < left) o[2 * j + 1] = v.y;
+            }
         }
         return;
     }
     const bool bf = p.out_dtype == CHELIS_DTYPE_BF16;
     uint16_t *o = static_cast<uint16_t *>(p.out) + index;
-    const bool vec = left >= 128 && (reinterpret_cast<uintptr_t>(o) & 15) == 0;
+    const bool vec = left >= 128 && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
 #pragma unroll
-    for (int j = 0; j < 128; j += 8) {
-        uint32_t w[4];
+    for (int j = 0; j < 64; j += 8) {
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float lo = run[j + 2 * i], hi = run[j + 2 * i + 1];
-            if (bf) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(lo, hi);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-        }
+        for (int i = 0; i < 8; ++i) w[i] = round2(unpack2(run[j + i]), bf);
         if (vec) {
-            *reinterpret_cast<uint4 *>(o + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            store32(o + 2 * j, w);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (j + i < left) o[j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 16; ++i)
+                if (2 * j + i < left) o[2 * j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
         }
     }
 }
 
+// The bounded wait of common.cuh with the limit held in a register: reading
+// it anew costs a trip to L2 at every wait, more than a block's MMAs take
+// (the dense product 16384 x 4096 x 1024 ran 172 us so, see gemm8_kernel).
+// Arrive on the pair's first block's barrier.  What it orders is the read of
+// tensor memory, which the tcgen05 fences around it carry, so it releases
+// nothing: a release at cluster scope waits for all of the thread's memory
+// traffic (with it the pair kernel took 2700 clocks a block, without it 1300).
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
+// A suspended try at cluster scope for the pair's arrivals (relaxed: see
+// arrive_relaxed).
+__device__ __forceinline__ bool try_wait_relaxed(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000u)
+        : "memory");
+    return ok != 0;
+}
+// The bounded wait of common.cuh with the limit held in a register: reading
+// it anew costs a trip to L2 at every wait, more than a block's MMAs take.
+// False on the limit, or once another role of the block has given up.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t tries,
+                                     volatile uint32_t *abort_flag, unsigned int code) {
+    for (uint32_t i = 0; i < tries; ++i) {
+        if (CLUSTER ? try_wait_relaxed(bar, parity) : mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    report_device_error(code);
+    *abort_flag = 1;
+    return false;
+}
+
 // BMN: b is read with its rows along the contraction (the input gradient).
 // WG: the weight gradient (groups along the contraction, scales on both sides).
-template <bool BMN, bool WG>
+template <bool BMN, bool WG, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const Params p) {
+    constexpr int TM = PAIR ? 2 * BM : BM;
+    constexpr int B_BOXES = PAIR ? 1 : 2;
+    constexpr int STAGE_BYTES = (1 + B_BOXES) * BOX_BYTES;
+    constexpr int STAGES = RING_BYTES / STAGE_BYTES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
+    // a pair's blocks have their shared memory at the same offsets
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + RING_BYTES);
     uint64_t *empty = full + STAGES;
-    uint64_t *acc_full = empty + STAGES;   // [2]
-    uint64_t *acc_empty = acc_full + 2;    // [2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    uint64_t *acc_full = empty + STAGES;  // [2]
+    uint64_t *acc_empty = acc_full + 2;   // [2]: of a pair, the first block's
+    uint64_t *scale_full = acc_empty + 2;
+    uint64_t *scale_empty = scale_full + SCALE_SLOTS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_empty + SCALE_SLOTS);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     volatile int32_t *consumed = reinterpret_cast<volatile int32_t *>(tmem_slot + 2);
-    float *col_scale = reinterpret_cast<float *>(smem + STAGES * STAGE_BYTES + 256);
-    int32_t *start = reinterpret_cast<int32_t *>(col_scale + FOLD_WARPS * BK);
+    float *scales = reinterpret_cast<float *>(smem + RING_BYTES + 512);
+    int32_t *start = reinterpret_cast<int32_t *>(scales + SCALE_SLOTS * SLOT_FLOATS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t tries = *static_cast<volatile uint32_t *>(&g_wait_tries);
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+    const int64_t worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
@@ -212,7 +331,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], FOLD_WARPS);
+            mbar_init(&acc_empty[b], PAIR ? 2 * FOLD_WARPS : FOLD_WARPS);
+        }
+        for (int q = 0; q < SCALE_SLOTS; ++q) {
+            mbar_init(&scale_full[q], 32);
+            mbar_init(&scale_empty[q], FOLD_WARPS);
         }
         *abort_flag = 0;
         *consumed = 0;
@@ -221,21 +344,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         prefetch_tensormap(&map_b);
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, TMEM_COLS);
-        tmem_relinquish();
+        if (PAIR) {
+            tmem_alloc_pair(tmem_slot, TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, TMEM_COLS);
+            tmem_relinquish();
+        }
     }
     if (warp == 2) {
-        // prefix over groups of row tiles or contraction blocks (both of 128),
-        // held to what ordered offsets give at most
+        // prefix over groups of row tiles or contraction blocks, held to what
+        // ordered offsets give at most
+        constexpr int HIGH = WG ? BK : TM;
         const int64_t count = WG ? p.group_rows : p.rows;
-        const int most = WG ? p.kblocks : static_cast<int>((count + 127) / 128) + p.groups;
+        const int most = WG ? p.kblocks : static_cast<int>((count + HIGH - 1) / HIGH) + p.groups;
         int base = 0;
         for (int g0 = 0; g0 < p.groups; g0 += 32) {
             int c = 0;
             if (g0 + lane < p.groups) {
                 int64_t lo, hi;
                 group_span(p, count, g0 + lane, &lo, &hi);
-                c = static_cast<int>((hi - lo + 127) / 128);
+                c = static_cast<int>((hi - lo + HIGH - 1) / HIGH);
             }
             int sum = c;
 #pragma unroll
@@ -249,136 +378,188 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) start[0] = 0;
     }
     tc_fence_before();
-    __syncthreads();
+    if (PAIR) cluster_sync_all();
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int64_t nt = (p.n + BN - 1) / BN;
-    const int64_t tiles = WG ? p.groups * nt * ((p.rows + BM - 1) / BM) : start[p.groups] * nt;
+    const int64_t tiles = WG ? p.groups * nt * ((p.rows + TM - 1) / TM) : start[p.groups] * nt;
     int32_t issued = 0;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
+        if (warp == 0 && lane == 0) {
+            // ---------------- TMA producer ----------------
             int32_t it = 0;
             bool ok = true;
-            for (int64_t L = blockIdx.x; ok && L < tiles; L += gridDim.x) {
-                const Tile t = tile_at<WG>(p, start, L);
+            for (int64_t L = worker; ok && L < tiles; L += workers) {
+                const Tile t = tile_at<WG, TM>(p, start, L);
+                const int32_t m0 = static_cast<int32_t>(t.m0) + static_cast<int32_t>(rank) * BM;
+                const int32_t n0 = static_cast<int32_t>(t.n0) + static_cast<int32_t>(rank) * 128;
                 for (int i = 0; i < t.kbs; ++i, ++it) {
                     const int s = it % STAGES;
-                    if (!mbar_wait_bounded(&empty[s], ((it / STAGES) & 1) ^ 1, DEVERR_TIMEOUT_PRODUCER)) {
-                        *abort_flag = 1;
+                    if (!wait(&empty[s], ((it / STAGES) & 1) ^ 1, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER)) {
                         ok = false;
                         break;
                     }
                     unsigned char *st = smem + s * STAGE_BYTES;
-                    mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
                     const int32_t k0 = (t.kb0 + i) * BK;
-                    tma_load_2d(st, &map_a, &full[s], k0, static_cast<int32_t>(t.m0));
+                    if (PAIR) {
+                        const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
+                        tma_load_2d_pair(st, &map_a, bar, k0, m0);
+                        if (WG) tma_load_2d_pair(st + BOX_BYTES, &map_b, bar, k0, n0);
+                        else if (BMN) tma_load_3d_pair(st + BOX_BYTES, &map_b, bar, n0, k0, t.group);
+                        else tma_load_3d_pair(st + BOX_BYTES, &map_b, bar, k0, n0, t.group);
+                    } else {
+                        mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+                        tma_load_2d(st, &map_a, &full[s], k0, m0);
 #pragma unroll
-                    for (int h = 0; h < BN / 128; ++h) {
-                        unsigned char *dst = st + A_BYTES + h * (128 * BK);
-                        const int32_t n0 = static_cast<int32_t>(t.n0) + h * 128;
-                        if (WG) tma_load_2d(dst, &map_b, &full[s], k0, n0);
-                        else if (BMN) tma_load_3d(dst, &map_b, &full[s], n0, k0, t.group);
-                        else tma_load_3d(dst, &map_b, &full[s], k0, n0, t.group);
+                        for (int h = 0; h < B_BOXES; ++h) {
+                            unsigned char *dst = st + (1 + h) * BOX_BYTES;
+                            if (WG) tma_load_2d(dst, &map_b, &full[s], k0, n0 + h * 128);
+                            else if (BMN) tma_load_3d(dst, &map_b, &full[s], n0 + h * 128, k0, t.group);
+                            else tma_load_3d(dst, &map_b, &full[s], k0, n0 + h * 128, t.group);
+                        }
                     }
                     issued = it + 1;
                 }
-                if (*abort_flag) ok = false;
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            // ---------------- MMA issuer ----------------
             int32_t it = 0;
-            int cur = 0;
             bool ok = true;
-            for (int64_t L = blockIdx.x; ok && L < tiles; L += gridDim.x) {
-                const Tile t = tile_at<WG>(p, start, L);
+            for (int64_t L = worker; ok && L < tiles; L += workers) {
+                const Tile t = tile_at<WG, TM>(p, start, L);
                 for (int i = 0; i < t.kbs; ++i, ++it) {
-                    cur = it & 1;
+                    const int cur = it & 1;
                     if (it >= 2) {
-                        if (!mbar_wait_bounded(&acc_empty[cur], ((it >> 1) - 1) & 1, DEVERR_TIMEOUT_MMA)) {
-                            *abort_flag = 1;
+                        const uint32_t parity = ((it >> 1) - 1) & 1;
+                        if (!(PAIR ? wait<true>(&acc_empty[cur], parity, tries, abort_flag, DEVERR_TIMEOUT_MMA)
+                                   : wait(&acc_empty[cur], parity, tries, abort_flag, DEVERR_TIMEOUT_MMA))) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
                     }
                     const int s = it % STAGES;
-                    if (!mbar_wait_bounded(&full[s], (it / STAGES) & 1, DEVERR_TIMEOUT_MMA)) {
-                        *abort_flag = 1;
+                    if (!wait(&full[s], (it / STAGES) & 1, tries, abort_flag, DEVERR_TIMEOUT_MMA)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * STAGE_BYTES), b = a + A_BYTES;
+                    const uint32_t a = smem_u32(smem + s * STAGE_BYTES), b = a + BOX_BYTES;
                     const uint32_t d = tmem_base + static_cast<uint32_t>(cur) * ACC_COLS;
 #pragma unroll
                     for (int kk = 0; kk < BK / 32; ++kk)
-                        mma_f8(d, sw128_kmajor_desc(a + kk * 32),
-                               BMN ? mnmajor_desc(b + kk * 32 * 128) : sw128_kmajor_desc(b + kk * 32),
-                               p.idesc, kk != 0);
-                    mma_commit(&empty[s]);
+                        mma_f8<PAIR>(d, sw128_kmajor_desc(a + kk * 32),
+                                     BMN ? mnmajor_desc(b + kk * 32 * 128) : sw128_kmajor_desc(b + kk * 32),
+                                     p.idesc, kk != 0);
+                    if (PAIR) mma_commit_pair(&empty[s], 0x3);
+                    else mma_commit(&empty[s]);
                     *consumed = it + 1;
-                    mma_commit(&acc_full[cur]);
+                    if (PAIR) mma_commit_pair(&acc_full[cur], 0x3);
+                    else mma_commit(&acc_full[cur]);
                 }
-                if (*abort_flag) ok = false;
             }
-            if (*abort_flag) mma_commit(&acc_full[cur]);  // let the fold see the flag
+        } else if (warp == 2) {
+            // ---------------- scales ----------------
+            int32_t it = 0;
+            bool ok = true;
+            for (int64_t L = worker; ok && L < tiles; L += workers) {
+                const Tile t = tile_at<WG, TM>(p, start, L);
+                const int64_t m0 = t.m0 + rank * BM;
+                const float *tile_sb = p.sb + t.group * p.sb_group + (t.n0 / 128) * p.sb_n;
+                for (int i = 0; i < t.kbs; ++i, ++it) {
+                    const int q = it % SCALE_SLOTS;
+                    if (!wait(&scale_empty[q], ((it / SCALE_SLOTS) & 1) ^ 1,
+                                           tries, abort_flag, DEVERR_TIMEOUT_PRODUCER)) {
+                        ok = false;
+                        break;
+                    }
+                    float *slot = scales + q * SLOT_FLOATS;
+                    const int64_t kb = t.kb0 + i;
+#pragma unroll
+                    for (int u = 0; u < BM / 32; ++u) {
+                        const int64_t row = m0 + u * 32 + lane;
+                        cp_async4(slot + u * 32 + lane, p.sa + kb * p.rows + (row < p.rows ? row : 0),
+                                  row < p.rows);
+                    }
+                    if (WG) {
+#pragma unroll
+                        for (int u = 0; u < BN / 32; ++u) {
+                            const int64_t c = t.n0 + u * 32 + lane;
+                            cp_async4(slot + BM + u * 32 + lane, p.sb + kb * p.n + (c < p.n ? c : 0), c < p.n);
+                        }
+                    } else if (lane < 2) {
+                        const bool in = t.n0 + lane * 128 < p.n;
+                        cp_async4(slot + BM + lane, in ? tile_sb + lane * p.sb_n + kb * p.sb_k : p.sb, in);
+                    }
+                    cp_async_arrive(&scale_full[q]);
+                }
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
-        const int quad = warp & 3, half = (warp - 2) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FOLD_REGS));
+        // ---------------- fold and store ----------------
+        const int quad = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        float *cs = col_scale + (warp - 2) * BK;
         int32_t it = 0;
         bool ok = true;
-        for (int64_t L = blockIdx.x; ok && L < tiles; L += gridDim.x) {
-            const Tile t = tile_at<WG>(p, start, L);
-            const int64_t row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * 128;
-            const int64_t srow = row < p.rows ? row : p.rows - 1;
-            float run[128];
+        for (int64_t L = worker; ok && L < tiles; L += workers) {
+            const Tile t = tile_at<WG, TM>(p, start, L);
+            const int64_t row = t.m0 + rank * BM + quad * 32 + lane, col0 = t.n0 + half * 128;
+            f32x2 run[64];
 #pragma unroll
-            for (int j = 0; j < 128; ++j) run[j] = 0.0f;
+            for (int j = 0; j < 64; ++j) run[j] = 0ull;
             for (int i = 0; i < t.kbs; ++i, ++it) {
-                const int64_t kb = t.kb0 + i;
-                float s = p.sa[kb * p.rows + srow];
-                if (WG) {
-                    __syncwarp();
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int64_t c = col0 + u * 32 + lane;
-                        cs[u * 32 + lane] = c < p.n ? p.sb[kb * p.n + c] : 0.0f;
-                    }
-                    __syncwarp();
-                } else if (col0 < p.n) {
-                    s *= p.sb[t.group * p.sb_group + (col0 / 128) * p.sb_n + kb * p.sb_k];
-                }
-                const int b = it & 1;
-                if (!mbar_wait_bounded(&acc_full[b], (it >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
-                    *abort_flag = 1;
-                    ok = false;
-                    break;
-                }
+                const int b = it & 1, q = it % SCALE_SLOTS;
+                const float *slot = scales + q * SLOT_FLOATS;
+                ok = wait(&scale_full[q], (it / SCALE_SLOTS) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE) &&
+                     wait(&acc_full[b], (it >> 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
                 tc_fence_after();
-                if (*abort_flag) {
-                    ok = false;
-                    break;
-                }
+                float s = slot[quad * 32 + lane];
+                if (!WG) s *= slot[BM + half];
+                const f32x2 s2 = pack2(s, s);
+                const float4 *cs = reinterpret_cast<const float4 *>(slot + BM + half * 128);
                 const uint32_t acc = tmem_base + lanes + static_cast<uint32_t>(b) * ACC_COLS + half * 128;
+                // 32 columns are added while the next 32 load
+                uint32_t r[2][32];
+                tmem_ld_32x32b_x32(acc, r[0]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(acc + j * 32, r);
                     tmem_wait_ld();
+                    if (j < 3) {
+                        tmem_ld_32x32b_x32(acc + (j + 1) * 32, r[(j + 1) & 1]);
+                    } else {
+                        // the accumulator has been read: the next block may have it
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) arrive_relaxed(mapa_shared(smem_u32(&acc_empty[b]), 0));
+                            else mbar_arrive(&acc_empty[b]);
+                        }
+                    }
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        float v = __uint_as_float(r[c]);
-                        if (WG) v *= cs[j * 32 + c];
-                        run[j * 32 + c] = fmaf(v, s, run[j * 32 + c]);
+                    for (int c = 0; c < 32; c += 4) {
+                        f32x2 v0 = pack2(__uint_as_float(r[j & 1][c]), __uint_as_float(r[j & 1][c + 1]));
+                        f32x2 v1 = pack2(__uint_as_float(r[j & 1][c + 2]), __uint_as_float(r[j & 1][c + 3]));
+                        if (WG) {
+                            const float4 w = cs[j * 8 + c / 4];
+                            v0 = mul2(v0, pack2(w.x, w.y));
+                            v1 = mul2(v1, pack2(w.z, w.w));
+                        }
+                        const int o = j * 16 + c / 2;
+                        run[o] = fma2(v0, s2, run[o]);
+                        run[o + 1] = fma2(v1, s2, run[o + 1]);
                     }
                 }
-                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[b]);
+                if (lane == 0) mbar_arrive(&scale_empty[q]);
             }
             if (ok && row < t.m_end && col0 < p.n) {
                 const int64_t base = WG ? t.group * p.rows * p.n : 0;
@@ -392,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             group_span(p, p.rows, p.groups - 1, &a, &last);
             const int64_t bytes = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
             unsigned char *o = static_cast<unsigned char *>(p.out);
-            const int64_t who = static_cast<int64_t>(blockIdx.x) * (FOLD_WARPS * 32) + threadIdx.x - 64;
+            const int64_t who = static_cast<int64_t>(blockIdx.x) * (FOLD_WARPS * 32) + threadIdx.x - 128;
             const int64_t step = static_cast<int64_t>(gridDim.x) * (FOLD_WARPS * 32);
             const int64_t loose = (first + p.rows - last) * p.n;
             for (int64_t i = who; i < loose; i += step) {
@@ -406,12 +587,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     // after an abort, copies that were issued but not consumed land first
-    if (warp == 0 && lane == 0 && *abort_flag)
-        for (int32_t it = *consumed; it < issued; ++it)
-            mbar_wait_bounded(&full[it % STAGES], (it / STAGES) & 1, DEVERR_TIMEOUT_PRODUCER);
+    if (warp == 0 && lane == 0 && *abort_flag) {
+        if (rank == 0) {
+            for (int32_t it = *consumed; it < issued; ++it)
+                wait(&full[it % STAGES], (it / STAGES) & 1, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER);
+        } else if (issued > 0) {
+            // this block's copies report to the first block's barriers
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < DRAIN_NS) __nanosleep(1000);
+        }
+    }
+    if (PAIR) {
+        // neither block leaves while the other may use its memory
+        tc_fence_before();
+        cluster_sync_all();
+    }
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, TMEM_COLS);
+        if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+        else tmem_dealloc(tmem_base, TMEM_COLS);
     }
 }
 
@@ -434,25 +628,51 @@ int make_map(CUtensorMap *map, const void *base, int64_t cols, int64_t ld, int64
     return CHELIS_CUDA_OK;
 }
 
-uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn) {
+uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn, bool pair) {
     return (1u << 4) |                                            // f32 sums
            (format_a == CHELIS_FORMAT_E5M2 ? 1u << 7 : 0u) |      // 0 e4m3, 1 e5m2
            (format_b == CHELIS_FORMAT_E5M2 ? 1u << 10 : 0u) |
            (bmn ? 1u << 16 : 0u) |                                // b MN-major
-           (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
+           (static_cast<uint32_t>(BN >> 3) << 17) |
+           (static_cast<uint32_t>((pair ? 2 * BM : BM) >> 4) << 24);
+}
+
+template <bool BMN, bool WG, bool PAIR>
+int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int64_t most_tiles) {
+    auto kernel = gemm8_kernel<BMN, WG, PAIR>;
+    CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+                          "cudaFuncSetAttribute"));
+    const int64_t workers = PAIR ? sm_count() / 2 : sm_count();
+    const int64_t used = most_tiles < workers ? (most_tiles < 1 ? 1 : most_tiles) : workers;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * used : used));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.stream = current_stream();
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = PAIR ? 2 : 1;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CHELIS_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p), "gemm8::gemm8_kernel"));
+    g_launches++;
+    return CHELIS_CUDA_OK;
+}
+
+// Tiles of 128 (or 256, pair) rows that the groups have at most.
+int64_t row_tiles(int64_t rows, int32_t groups, bool offsets, bool pair) {
+    const int64_t high = pair ? 2 * BM : BM;
+    return (rows + high - 1) / high + (offsets ? groups : 0);
 }
 
 template <bool BMN, bool WG>
-int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int64_t most_tiles) {
-    CHELIS_TRY(check_cuda(cudaFuncSetAttribute(gemm8_kernel<BMN, WG>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
-                          "cudaFuncSetAttribute"));
-    const int64_t sms = sm_count();
-    const unsigned grid = static_cast<unsigned>(most_tiles < sms ? (most_tiles < 1 ? 1 : most_tiles) : sms);
-    gemm8_kernel<BMN, WG><<<grid, THREADS, SMEM_BYTES, current_stream()>>>(ma, mb, p);
-    g_launches++;
-    CHELIS_LAUNCH_CHECK("gemm8::gemm8_kernel");
-    return CHELIS_CUDA_OK;
+int run(const CUtensorMap &ma, const CUtensorMap &mb, Params &p, int32_t fa, int32_t fb, bool pair) {
+    p.idesc = instruction(fa, fb, BMN, pair);
+    const int64_t nt = (p.n + BN - 1) / BN;
+    const int64_t most = WG ? p.groups * row_tiles(p.rows, 0, false, pair) * nt
+                            : row_tiles(p.rows, p.groups, p.offsets != nullptr, pair) * nt;
+    return pair ? launch<BMN, WG, true>(ma, mb, p, most) : launch<BMN, WG, false>(ma, mb, p, most);
 }
 
 int check_common(const char *op, int32_t fa, int32_t fb, int32_t out_dtype, int64_t rows, int64_t n,
@@ -511,9 +731,9 @@ extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans
     p.sb_k = trans_b ? 1 : nblocks;
     p.out = out;
     p.out_dtype = out_dtype;
-    p.idesc = gemm8::instruction(format_a, format_b, !trans_b);
-    const int64_t most = ((rows + 127) / 128 + (offsets ? groups : 0)) * ((n + gemm8::BN - 1) / gemm8::BN);
-    return trans_b ? gemm8::launch<false, false>(ma, mb, p, most) : gemm8::launch<true, false>(ma, mb, p, most);
+    const bool pair = rows >= 256 * static_cast<int64_t>(groups);
+    return trans_b ? gemm8::run<false, false>(ma, mb, p, format_a, format_b, pair)
+                   : gemm8::run<true, false>(ma, mb, p, format_a, format_b, pair);
 }
 
 extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int64_t k,
@@ -544,7 +764,6 @@ extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int
     p.sb = scales_b;
     p.out = out;
     p.out_dtype = out_dtype;
-    p.idesc = gemm8::instruction(format_a, format_b, false);
-    const int64_t most = groups * ((n + 127) / 128) * ((k + gemm8::BN - 1) / gemm8::BN);
-    return gemm8::launch<false, true>(ma, mb, p, most);
+    const bool pair = n > 128;
+    return gemm8::run<false, true>(ma, mb, p, format_a, format_b, pair);
 }
