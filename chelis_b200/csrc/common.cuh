@@ -61,6 +61,7 @@ enum : unsigned int {
     DEVERR_TRAP = 64u,         // a numeric trap recorded in g_trap_code (first one wins)
     DEVERR_SHIFT = 128u,       // a negative shift count, recorded in g_shift_count
     DEVERR_FAIL = 256u,        // a GuardedFail fired: its message id in g_fail_id
+    DEVERR_SCALE = 512u,       // a block scale that is no power of two
 };
 __device__ unsigned int g_fail_id = 0;  // the first fired guard's registered message id
 __device__ unsigned long long g_shift_count = 0;  // the first negative count reported (its bits)

@@ -11,21 +11,21 @@
 // expert, the rows [offsets[e], offsets[e + 1]) of a meet matrix e of w, and
 // dw has one matrix an expert, summed over that expert's blocks.
 //
-// A thread block works on 128 x 256 tiles of the result, one after the other;
-// a pair of blocks (PAIR, cta_group::2) on 256 x 256 tiles, each with its 128
-// rows of a and half of b's columns in shared memory and its 128 rows of the
-// sums in tensor memory.  384 threads:
-//   warp 0      TMA producer (one elected lane)
-//   warp 1      TMEM allocator + tcgen05.mma kind::f8f6f4 issuer (one lane,
-//               of a pair's first block)
+// This file has what the three product kernels share, and the one that takes
+// any f32 scales: gemm8_kernel, one thread block for a 128 x 256 tile of the
+// result at a time, 384 threads:
+//   warp 0      TMA producer
+//   warp 1      TMEM allocator + tcgen05.mma kind::f8f6f4 issuer
 //   warp 2      the blocks' scales into a ring of their own (cp.async)
 //   warps 4-11  fold: a block's sum in tensor memory times its scales into
 //               f32 registers, then the store
 // The scales differ from block to block, so the tensor core sums one block
 // of 128 (four MMAs of K = 32) from a fresh start, alternating between two
 // 256-column accumulators, and the fold adds it in IEEE f32 while the next
-// block runs.  That also keeps the sum as exact as f32: one long TMEM
-// accumulator truncates, and its error grows with K.
+// block runs.  The round trip between the two, about twice a block's 512
+// clocks of MMAs, is what bounds it; gemm_scaled8.cu has none.
+// Scales that are powers of two come here too where the product is too small
+// for that kernel's second launch (see gemm_scaled8.cu's entries).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,7 +43,8 @@ namespace gemm8 {
 
 constexpr int BM = 128, BN = 256, BK = 128;  // one scale block of K = 128 bytes = one swizzle row
 constexpr int BOX_BYTES = 128 * BK;          // 128 rows or columns of one block
-constexpr int RING_BYTES = 12 * BOX_BYTES;   // 4 stages of 3 boxes, or 6 of 2 (PAIR)
+constexpr int STAGES = 4, STAGE_BYTES = 3 * BOX_BYTES;
+constexpr int RING_BYTES = STAGES * STAGE_BYTES;
 constexpr int SCALE_SLOTS = 8;
 constexpr int SLOT_FLOATS = BM + BN;  // row scales, then column scales (or one for each 128 columns)
 constexpr int FOLD_WARPS = 8;
@@ -57,7 +58,6 @@ constexpr uint32_t ACC_COLS = 256, TMEM_COLS = 512;
 constexpr int MAX_GROUPS = experts::MAX_EXPERTS;
 constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + 512 /*barriers*/ +
                            SCALE_SLOTS * SLOT_FLOATS * 4 + (MAX_GROUPS + 1) * 4 /*tile starts*/;
-constexpr uint64_t DRAIN_NS = 200000;  // bounded drain of an aborted pair's second block
 
 struct Params {
     int64_t rows;     // rows of a: tokens (forward, input gradient), outputs (weight gradient)
@@ -74,23 +74,14 @@ struct Params {
     uint32_t idesc;
 };
 
-template <bool PAIR>
 __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                        uint32_t accumulate) {
-    if (PAIR)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 // 4 bytes from global to shared memory, zero when !ok.
 __device__ __forceinline__ void cp_async4(float *dst, const float *src, bool ok) {
@@ -117,6 +108,11 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     f32x2 r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
@@ -152,13 +148,52 @@ __device__ __forceinline__ void group_span(const Params &p, int64_t rows, int g,
     *hi = b;
 }
 
+// start[g], one warp: the row tiles (or contraction blocks) of HIGH rows before
+// group g, held to what ordered offsets give at most (`most`, or the tiles).
+template <int HIGH>
+__device__ __forceinline__ void group_starts(const Params &p, int64_t rows, int lane, int32_t *start,
+                                             int most = -1) {
+    if (most < 0) most = static_cast<int>((rows + HIGH - 1) / HIGH) + p.groups;
+    int base = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        int c = 0;
+        if (g0 + lane < p.groups) {
+            int64_t lo, hi;
+            group_span(p, rows, g0 + lane, &lo, &hi);
+            c = static_cast<int>((hi - lo + HIGH - 1) / HIGH);
+        }
+        int sum = c;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += o;
+        }
+        if (g0 + lane < p.groups) start[g0 + lane + 1] = min(base + sum, most);
+        base = min(base + __shfl_sync(0xffffffffu, sum, 31), most);
+    }
+    if (lane == 0) start[0] = 0;
+}
+
 // One tile of the result.
 struct Tile {
     int group;
+    int m_tile;         // its row tile, counted over all groups (weight gradient: in its matrix)
     int64_t m0, m_end;  // rows of the result, this tile's first and the group's last + 1
     int64_t n0;
     int kb0, kbs;       // contraction blocks
 };
+
+// Tiles of one group's matrix (mt x nt) in bands of BAND row tiles, column by
+// column within a band: the tiles in flight then share a few panels of a and
+// b in L2 however tall the matrix is (8192^3: 4, 8 and 16 within 1 %, whole
+// columns 3 % slower).
+constexpr int BAND = 8;
+__device__ __forceinline__ void band_order(int64_t in, int64_t mt, int64_t nt, int64_t *m, int64_t *n) {
+    const int64_t band = in / (BAND * nt), first = band * BAND;
+    const int64_t high = mt - first < BAND ? mt - first : BAND, r = in - band * (BAND * nt);
+    *n = r / high;
+    *m = first + (r - *n * high);
+}
 
 // `start` is, by group, the prefix of row tiles of TM rows (forward, input
 // gradient) or of contraction blocks (weight gradient).
@@ -170,8 +205,11 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, i
         const int64_t mt = (p.rows + TM - 1) / TM;
         t.group = static_cast<int>(L / (mt * nt));
         const int64_t in = L - t.group * mt * nt;
-        t.m0 = (in % mt) * TM;
-        t.n0 = (in / mt) * BN;
+        int64_t m, n;
+        band_order(in, mt, nt, &m, &n);
+        t.m_tile = static_cast<int>(m);
+        t.m0 = m * TM;
+        t.n0 = n * BN;
         t.m_end = p.rows;
         t.kb0 = start[t.group];
         t.kbs = start[t.group + 1] - t.kb0;
@@ -186,8 +224,11 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, i
         const int64_t in = L - start[lo] * nt, mt = start[lo + 1] - start[lo];
         int64_t a, b;
         group_span(p, p.rows, lo, &a, &b);
-        t.m0 = a + (in % mt) * TM;
-        t.n0 = (in / mt) * BN;
+        int64_t m, n;
+        band_order(in, mt, nt, &m, &n);
+        t.m_tile = start[lo] + static_cast<int>(m);
+        t.m0 = a + m * TM;
+        t.n0 = n * BN;
         t.m_end = b;
         t.kb0 = 0;
         t.kbs = p.kblocks;
@@ -255,9 +296,6 @@ __device__ __forceinline__ void store_row(const Params &p, const f32x2 (&run)[64
     }
 }
 
-// The bounded wait of common.cuh with the limit held in a register: reading
-// it anew costs a trip to L2 at every wait, more than a block's MMAs take
-// (the dense product 16384 x 4096 x 1024 ran 172 us so, see gemm8_kernel).
 // Arrive on the pair's first block's barrier.  What it orders is the read of
 // tensor memory, which the tcgen05 fences around it carry, so it releases
 // nothing: a release at cluster scope waits for all of the thread's memory
@@ -279,6 +317,18 @@ __device__ __forceinline__ bool try_wait_relaxed(uint64_t *bar, uint32_t parity)
         : "memory");
     return ok != 0;
 }
+// One look at an mbarrier's phase, without suspending.
+__device__ __forceinline__ bool probe(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // The bounded wait of common.cuh with the limit held in a register: reading
 // it anew costs a trip to L2 at every wait, more than a block's MMAs take.
 // False on the limit, or once another role of the block has given up.
@@ -294,24 +344,53 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, uint32_t tr
     return false;
 }
 
+// One lane of a converged warp.  The producer's and the issuer's loops run in
+// the whole warp, with only the instructions themselves under this predicate:
+// their descriptors and coordinates then live in uniform registers.  In code
+// under `lane == 0` each MMA took about 80 clocks to issue, more than half of
+// what it runs.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// The result of a wait as a vote, so that the branch on it is uniform too.
+__device__ __forceinline__ bool all(bool ok) { return __all_sync(0xffffffffu, ok); }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Rows of the result that no group holds, by all blocks' fold warps.
+__device__ __forceinline__ void zero_loose_rows(const Params &p) {
+    int64_t a, b, first, last;
+    group_span(p, p.rows, 0, &first, &b);
+    group_span(p, p.rows, p.groups - 1, &a, &last);
+    const int64_t who = static_cast<int64_t>(blockIdx.x) * (FOLD_WARPS * 32) + threadIdx.x - (THREADS - FOLD_WARPS * 32);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (FOLD_WARPS * 32);
+    const int64_t loose = (first + p.rows - last) * p.n;
+    for (int64_t i = who; i < loose; i += step) {
+        const int64_t e = i < first * p.n ? i : last * p.n + (i - first * p.n);
+        if (p.out_dtype == CHELIS_DTYPE_F32) static_cast<float *>(p.out)[e] = 0.0f;
+        else static_cast<uint16_t *>(p.out)[e] = 0;
+    }
+}
+// Copies that were issued but not consumed land before an aborted block leaves.
+__device__ __forceinline__ void landed(uint64_t *bar, uint32_t parity, uint32_t tries) {
+    for (uint32_t i = 0; i < tries; ++i)
+        if (mbar_try_wait(bar, parity)) return;
+}
+
 // BMN: b is read with its rows along the contraction (the input gradient).
 // WG: the weight gradient (groups along the contraction, scales on both sides).
-template <bool BMN, bool WG, bool PAIR>
+template <bool BMN, bool WG>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const Params p) {
-    constexpr int TM = PAIR ? 2 * BM : BM;
-    constexpr int B_BOXES = PAIR ? 1 : 2;
-    constexpr int STAGE_BYTES = (1 + B_BOXES) * BOX_BYTES;
-    constexpr int STAGES = RING_BYTES / STAGE_BYTES;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    // a pair's blocks have their shared memory at the same offsets
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + RING_BYTES);
     uint64_t *empty = full + STAGES;
     uint64_t *acc_full = empty + STAGES;  // [2]
-    uint64_t *acc_empty = acc_full + 2;   // [2]: of a pair, the first block's
+    uint64_t *acc_empty = acc_full + 2;   // [2]
     uint64_t *scale_full = acc_empty + 2;
     uint64_t *scale_empty = scale_full + SCALE_SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_empty + SCALE_SLOTS);
@@ -322,8 +401,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t tries = *static_cast<volatile uint32_t *>(&g_wait_tries);
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-    const int64_t worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
@@ -331,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], PAIR ? 2 * FOLD_WARPS : FOLD_WARPS);
+            mbar_init(&acc_empty[b], FOLD_WARPS);
         }
         for (int q = 0; q < SCALE_SLOTS; ++q) {
             mbar_init(&scale_full[q], 32);
@@ -344,144 +421,106 @@ __global__ void __launch_bounds__(THREADS, 1)
         prefetch_tensormap(&map_b);
     }
     if (warp == 1) {
-        if (PAIR) {
-            tmem_alloc_pair(tmem_slot, TMEM_COLS);
-            tmem_relinquish_pair();
-        } else {
-            tmem_alloc(tmem_slot, TMEM_COLS);
-            tmem_relinquish();
-        }
+        tmem_alloc(tmem_slot, TMEM_COLS);
+        tmem_relinquish();
     }
-    if (warp == 2) {
-        // prefix over groups of row tiles or contraction blocks, held to what
-        // ordered offsets give at most
-        constexpr int HIGH = WG ? BK : TM;
-        const int64_t count = WG ? p.group_rows : p.rows;
-        const int most = WG ? p.kblocks : static_cast<int>((count + HIGH - 1) / HIGH) + p.groups;
-        int base = 0;
-        for (int g0 = 0; g0 < p.groups; g0 += 32) {
-            int c = 0;
-            if (g0 + lane < p.groups) {
-                int64_t lo, hi;
-                group_span(p, count, g0 + lane, &lo, &hi);
-                c = static_cast<int>((hi - lo + HIGH - 1) / HIGH);
-            }
-            int sum = c;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= off) sum += o;
-            }
-            if (g0 + lane < p.groups) start[g0 + lane + 1] = min(base + sum, most);
-            base = min(base + __shfl_sync(0xffffffffu, sum, 31), most);
-        }
-        if (lane == 0) start[0] = 0;
-    }
+    if (warp == 2) group_starts<WG ? BK : BM>(p, WG ? p.group_rows : p.rows, lane, start, WG ? p.kblocks : -1);
     tc_fence_before();
-    if (PAIR) cluster_sync_all();
-    else __syncthreads();
+    __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int64_t nt = (p.n + BN - 1) / BN;
-    const int64_t tiles = WG ? p.groups * nt * ((p.rows + TM - 1) / TM) : start[p.groups] * nt;
+    const int tiles = uniform(static_cast<int>(WG ? p.groups * nt * ((p.rows + BM - 1) / BM) : start[p.groups] * nt));
+    const int first = static_cast<int>(blockIdx.x), step = static_cast<int>(gridDim.x);
     int32_t issued = 0;
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
-        if (warp == 0 && lane == 0) {
+        if (warp == 0) {
             // ---------------- TMA producer ----------------
-            int32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 1;
             bool ok = true;
-            for (int64_t L = worker; ok && L < tiles; L += workers) {
-                const Tile t = tile_at<WG, TM>(p, start, L);
-                const int32_t m0 = static_cast<int32_t>(t.m0) + static_cast<int32_t>(rank) * BM;
-                const int32_t n0 = static_cast<int32_t>(t.n0) + static_cast<int32_t>(rank) * 128;
-                for (int i = 0; i < t.kbs; ++i, ++it) {
-                    const int s = it % STAGES;
-                    if (!wait(&empty[s], ((it / STAGES) & 1) ^ 1, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER)) {
-                        ok = false;
-                        break;
-                    }
-                    unsigned char *st = smem + s * STAGE_BYTES;
-                    const int32_t k0 = (t.kb0 + i) * BK;
-                    if (PAIR) {
-                        const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
-                        tma_load_2d_pair(st, &map_a, bar, k0, m0);
-                        if (WG) tma_load_2d_pair(st + BOX_BYTES, &map_b, bar, k0, n0);
-                        else if (BMN) tma_load_3d_pair(st + BOX_BYTES, &map_b, bar, n0, k0, t.group);
-                        else tma_load_3d_pair(st + BOX_BYTES, &map_b, bar, k0, n0, t.group);
-                    } else {
-                        mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
-                        tma_load_2d(st, &map_a, &full[s], k0, m0);
+            for (int L = first; ok && L < tiles; L += step) {
+                const Tile t = tile_at<WG, BM>(p, start, L);
+                const int group = uniform(t.group), kbs = uniform(t.kbs);
+                const int32_t m0 = uniform(static_cast<int32_t>(t.m0)), n0 = uniform(static_cast<int32_t>(t.n0));
+                int32_t k0 = uniform(t.kb0) * BK;
+                for (int i = 0; i < kbs; ++i, k0 += BK) {
+                    ok = all(wait(&empty[stage], phase, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER));
+                    if (!ok) break;
+                    unsigned char *st = smem + stage * STAGE_BYTES;
+                    uint64_t *bar = &full[stage];
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar, STAGE_BYTES);
+                        tma_load_2d(st, &map_a, bar, k0, m0);
 #pragma unroll
-                        for (int h = 0; h < B_BOXES; ++h) {
+                        for (int h = 0; h < BN / 128; ++h) {
                             unsigned char *dst = st + (1 + h) * BOX_BYTES;
-                            if (WG) tma_load_2d(dst, &map_b, &full[s], k0, n0 + h * 128);
-                            else if (BMN) tma_load_3d(dst, &map_b, &full[s], n0 + h * 128, k0, t.group);
-                            else tma_load_3d(dst, &map_b, &full[s], k0, n0 + h * 128, t.group);
+                            if (WG) tma_load_2d(dst, &map_b, bar, k0, n0 + h * 128);
+                            else if (BMN) tma_load_3d(dst, &map_b, bar, n0 + h * 128, k0, group);
+                            else tma_load_3d(dst, &map_b, bar, k0, n0 + h * 128, group);
                         }
                     }
-                    issued = it + 1;
+                    ++issued;
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp == 1) {
             // ---------------- MMA issuer ----------------
+            const uint32_t tb = uniform(static_cast<int>(tmem_base));
             int32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 0;
             bool ok = true;
-            for (int64_t L = worker; ok && L < tiles; L += workers) {
-                const Tile t = tile_at<WG, TM>(p, start, L);
-                for (int i = 0; i < t.kbs; ++i, ++it) {
+            for (int L = first; ok && L < tiles; L += step) {
+                const int kbs = WG ? uniform(tile_at<WG, BM>(p, start, L).kbs) : p.kblocks;
+                for (int i = 0; i < kbs; ++i, ++it) {
                     const int cur = it & 1;
-                    if (it >= 2) {
-                        const uint32_t parity = ((it >> 1) - 1) & 1;
-                        if (!(PAIR ? wait<true>(&acc_empty[cur], parity, tries, abort_flag, DEVERR_TIMEOUT_MMA)
-                                   : wait(&acc_empty[cur], parity, tries, abort_flag, DEVERR_TIMEOUT_MMA))) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                    }
-                    const int s = it % STAGES;
-                    if (!wait(&full[s], (it / STAGES) & 1, tries, abort_flag, DEVERR_TIMEOUT_MMA)) {
-                        ok = false;
-                        break;
-                    }
+                    if (it >= 2)
+                        ok = all(wait(&acc_empty[cur], ((it >> 1) - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_MMA));
+                    if (ok) ok = all(wait(&full[stage], phase, tries, abort_flag, DEVERR_TIMEOUT_MMA));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * STAGE_BYTES), b = a + BOX_BYTES;
-                    const uint32_t d = tmem_base + static_cast<uint32_t>(cur) * ACC_COLS;
+                    const uint32_t a = smem_u32(smem) + stage * STAGE_BYTES, b = a + BOX_BYTES;
+                    const uint32_t d = tb + static_cast<uint32_t>(cur) * ACC_COLS;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < BK / 32; ++kk)
-                        mma_f8<PAIR>(d, sw128_kmajor_desc(a + kk * 32),
-                                     BMN ? mnmajor_desc(b + kk * 32 * 128) : sw128_kmajor_desc(b + kk * 32),
-                                     p.idesc, kk != 0);
-                    if (PAIR) mma_commit_pair(&empty[s], 0x3);
-                    else mma_commit(&empty[s]);
-                    *consumed = it + 1;
-                    if (PAIR) mma_commit_pair(&acc_full[cur], 0x3);
-                    else mma_commit(&acc_full[cur]);
+                        for (int kk = 0; kk < BK / 32; ++kk)
+                            mma_f8(d, sw128_kmajor_desc(a + kk * 32),
+                                   BMN ? mnmajor_desc(b + kk * 32 * 128) : sw128_kmajor_desc(b + kk * 32), p.idesc,
+                                   kk != 0);
+                        mma_commit(&empty[stage]);
+                        mma_commit(&acc_full[cur]);
+                    }
+                    __syncwarp();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
+            if (lane == 0) *consumed = it;
         } else if (warp == 2) {
             // ---------------- scales ----------------
             int32_t it = 0;
             bool ok = true;
-            for (int64_t L = worker; ok && L < tiles; L += workers) {
-                const Tile t = tile_at<WG, TM>(p, start, L);
-                const int64_t m0 = t.m0 + rank * BM;
+            for (int L = first; ok && L < tiles; L += step) {
+                const Tile t = tile_at<WG, BM>(p, start, L);
                 const float *tile_sb = p.sb + t.group * p.sb_group + (t.n0 / 128) * p.sb_n;
                 for (int i = 0; i < t.kbs; ++i, ++it) {
                     const int q = it % SCALE_SLOTS;
-                    if (!wait(&scale_empty[q], ((it / SCALE_SLOTS) & 1) ^ 1,
-                                           tries, abort_flag, DEVERR_TIMEOUT_PRODUCER)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = all(wait(&scale_empty[q], ((it / SCALE_SLOTS) & 1) ^ 1, tries, abort_flag,
+                                  DEVERR_TIMEOUT_PRODUCER));
+                    if (!ok) break;
                     float *slot = scales + q * SLOT_FLOATS;
                     const int64_t kb = t.kb0 + i;
 #pragma unroll
                     for (int u = 0; u < BM / 32; ++u) {
-                        const int64_t row = m0 + u * 32 + lane;
+                        const int64_t row = t.m0 + u * 32 + lane;
                         cp_async4(slot + u * 32 + lane, p.sa + kb * p.rows + (row < p.rows ? row : 0),
                                   row < p.rows);
                     }
@@ -497,7 +536,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     cp_async_arrive(&scale_full[q]);
                 }
-                ok = __all_sync(0xffffffffu, ok);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
@@ -508,9 +546,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         int32_t it = 0;
         bool ok = true;
-        for (int64_t L = worker; ok && L < tiles; L += workers) {
-            const Tile t = tile_at<WG, TM>(p, start, L);
-            const int64_t row = t.m0 + rank * BM + quad * 32 + lane, col0 = t.n0 + half * 128;
+        for (int L = first; ok && L < tiles; L += step) {
+            const Tile t = tile_at<WG, BM>(p, start, L);
+            const int64_t row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * 128;
+            const bool live = row - lane < t.m_end && col0 < p.n;  // else nothing to read or store
             f32x2 run[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) run[j] = 0ull;
@@ -519,9 +558,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float *slot = scales + q * SLOT_FLOATS;
                 ok = wait(&scale_full[q], (it / SCALE_SLOTS) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE) &&
                      wait(&acc_full[b], (it >> 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = all(ok);
                 if (!ok) break;
                 tc_fence_after();
+                auto release = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[b]);
+                };
+                if (!live) {
+                    release();
+                    if (lane == 0) mbar_arrive(&scale_empty[q]);
+                    continue;
+                }
                 float s = slot[quad * 32 + lane];
                 if (!WG) s *= slot[BM + half];
                 const f32x2 s2 = pack2(s, s);
@@ -533,17 +582,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     tmem_wait_ld();
-                    if (j < 3) {
-                        tmem_ld_32x32b_x32(acc + (j + 1) * 32, r[(j + 1) & 1]);
-                    } else {
-                        // the accumulator has been read: the next block may have it
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) arrive_relaxed(mapa_shared(smem_u32(&acc_empty[b]), 0));
-                            else mbar_arrive(&acc_empty[b]);
-                        }
-                    }
+                    if (j < 3) tmem_ld_32x32b_x32(acc + (j + 1) * 32, r[(j + 1) & 1]);
+                    else release();  // the accumulator has been read: the next block may have it
 #pragma unroll
                     for (int c = 0; c < 32; c += 4) {
                         f32x2 v0 = pack2(__uint_as_float(r[j & 1][c]), __uint_as_float(r[j & 1][c + 1]));
@@ -561,51 +601,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scale_empty[q]);
             }
-            if (ok && row < t.m_end && col0 < p.n) {
+            if (ok && live && row < t.m_end) {
                 const int64_t base = WG ? t.group * p.rows * p.n : 0;
                 store_row(p, run, base + row * p.n + col0, p.n - col0);
             }
         }
-        // rows of the result that no group holds
-        if (!WG && p.offsets) {
-            int64_t a, b, first, last;
-            group_span(p, p.rows, 0, &first, &b);
-            group_span(p, p.rows, p.groups - 1, &a, &last);
-            const int64_t bytes = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
-            unsigned char *o = static_cast<unsigned char *>(p.out);
-            const int64_t who = static_cast<int64_t>(blockIdx.x) * (FOLD_WARPS * 32) + threadIdx.x - 128;
-            const int64_t step = static_cast<int64_t>(gridDim.x) * (FOLD_WARPS * 32);
-            const int64_t loose = (first + p.rows - last) * p.n;
-            for (int64_t i = who; i < loose; i += step) {
-                const int64_t e = i < first * p.n ? i : last * p.n + (i - first * p.n);
-                if (bytes == 4) reinterpret_cast<float *>(o)[e] = 0.0f;
-                else reinterpret_cast<uint16_t *>(o)[e] = 0;
-            }
-        }
+        if (!WG && p.offsets) zero_loose_rows(p);
     }
 
     tc_fence_before();
     __syncthreads();
-    // after an abort, copies that were issued but not consumed land first
-    if (warp == 0 && lane == 0 && *abort_flag) {
-        if (rank == 0) {
-            for (int32_t it = *consumed; it < issued; ++it)
-                wait(&full[it % STAGES], (it / STAGES) & 1, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER);
-        } else if (issued > 0) {
-            // this block's copies report to the first block's barriers
-            const uint64_t t0 = globaltimer_ns();
-            while (globaltimer_ns() - t0 < DRAIN_NS) __nanosleep(1000);
-        }
-    }
-    if (PAIR) {
-        // neither block leaves while the other may use its memory
-        tc_fence_before();
-        cluster_sync_all();
-    }
+    if (warp == 0 && lane == 0 && *abort_flag)
+        for (int32_t it = *consumed; it < issued; ++it)
+            landed(&full[it % STAGES], (it / STAGES) & 1, tries);
     if (warp == 1) {
         tc_fence_after();
-        if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
-        else tmem_dealloc(tmem_base, TMEM_COLS);
+        tmem_dealloc(tmem_base, TMEM_COLS);
     }
 }
 
@@ -628,51 +639,30 @@ int make_map(CUtensorMap *map, const void *base, int64_t cols, int64_t ld, int64
     return CHELIS_CUDA_OK;
 }
 
-uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn, bool pair) {
-    return (1u << 4) |                                            // f32 sums
-           (format_a == CHELIS_FORMAT_E5M2 ? 1u << 7 : 0u) |      // 0 e4m3, 1 e5m2
-           (format_b == CHELIS_FORMAT_E5M2 ? 1u << 10 : 0u) |
-           (bmn ? 1u << 16 : 0u) |                                // b MN-major
-           (static_cast<uint32_t>(BN >> 3) << 17) |
-           (static_cast<uint32_t>((pair ? 2 * BM : BM) >> 4) << 24);
-}
-
-template <bool BMN, bool WG, bool PAIR>
-int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int64_t most_tiles) {
-    auto kernel = gemm8_kernel<BMN, WG, PAIR>;
-    CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
-                          "cudaFuncSetAttribute"));
-    const int64_t workers = PAIR ? sm_count() / 2 : sm_count();
-    const int64_t used = most_tiles < workers ? (most_tiles < 1 ? 1 : most_tiles) : workers;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * used : used));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM_BYTES;
-    cfg.stream = current_stream();
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = PAIR ? 2 : 1;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    CHELIS_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p), "gemm8::gemm8_kernel"));
-    g_launches++;
-    return CHELIS_CUDA_OK;
-}
-
-// Tiles of 128 (or 256, pair) rows that the groups have at most.
-int64_t row_tiles(int64_t rows, int32_t groups, bool offsets, bool pair) {
-    const int64_t high = pair ? 2 * BM : BM;
+// Tiles of `high` rows that the groups have at most.
+int64_t row_tiles(int64_t rows, int32_t groups, bool offsets, int64_t high) {
     return (rows + high - 1) / high + (offsets ? groups : 0);
 }
 
 template <bool BMN, bool WG>
-int run(const CUtensorMap &ma, const CUtensorMap &mb, Params &p, int32_t fa, int32_t fb, bool pair) {
-    p.idesc = instruction(fa, fb, BMN, pair);
+int run(const CUtensorMap &ma, const CUtensorMap &mb, Params p, int32_t fa, int32_t fb) {
+    p.idesc = (1u << 4) |                                    // f32 sums
+              (fa == CHELIS_FORMAT_E5M2 ? 1u << 7 : 0u) |    // 0 e4m3, 1 e5m2
+              (fb == CHELIS_FORMAT_E5M2 ? 1u << 10 : 0u) |
+              (BMN ? 1u << 16 : 0u) |                        // b MN-major
+              (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
     const int64_t nt = (p.n + BN - 1) / BN;
-    const int64_t most = WG ? p.groups * row_tiles(p.rows, 0, false, pair) * nt
-                            : row_tiles(p.rows, p.groups, p.offsets != nullptr, pair) * nt;
-    return pair ? launch<BMN, WG, true>(ma, mb, p, most) : launch<BMN, WG, false>(ma, mb, p, most);
+    const int64_t most = (WG ? p.groups * row_tiles(p.rows, 0, false, BM)
+                             : row_tiles(p.rows, p.groups, p.offsets != nullptr, BM)) * nt;
+    auto kernel = gemm8_kernel<BMN, WG>;
+    CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+                          "cudaFuncSetAttribute"));
+    const int64_t sms = sm_count();
+    kernel<<<static_cast<unsigned>(most < sms ? (most < 1 ? 1 : most) : sms), THREADS, SMEM_BYTES, current_stream()>>>(
+        ma, mb, p);
+    g_launches++;
+    CHELIS_LAUNCH_CHECK("gemm8::gemm8_kernel");
+    return CHELIS_CUDA_OK;
 }
 
 int check_common(const char *op, int32_t fa, int32_t fb, int32_t out_dtype, int64_t rows, int64_t n,
@@ -698,72 +688,3 @@ int zero_out(void *out, int32_t dtype, int64_t count) {
 
 }  // namespace gemm8
 }  // namespace chelis
-
-using namespace chelis;
-
-extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows,
-                                   int64_t n, int64_t k, const uint8_t *a, const float *scales_a,
-                                   const uint8_t *b, const float *scales_b, const int32_t *offsets,
-                                   int32_t groups, int32_t out_dtype, void *out) {
-    CHELIS_TRY(gemm8::check_common("matmul8", format_a, format_b, out_dtype, rows, n, k, offsets, groups));
-    if (rows == 0 || n == 0) return CHELIS_CUDA_OK;
-    if (!out) return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8: null operand");
-    if (k == 0) return gemm8::zero_out(out, out_dtype, rows * n);
-    if (!a || !scales_a || !b || !scales_b)
-        return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8: null operand");
-    if (!experts::aligned16(a) || !experts::aligned16(b))
-        return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8: 8-bit data must lie on 16 bytes");
-    const int64_t kblocks = (k + 127) / 128, nblocks = (n + 127) / 128;
-    CUtensorMap ma, mb;
-    CHELIS_TRY(gemm8::make_map(&ma, a, k, blocks8::round16(k), rows, 1, false));
-    if (trans_b) CHELIS_TRY(gemm8::make_map(&mb, b, k, blocks8::round16(k), n, groups, true));
-    else CHELIS_TRY(gemm8::make_map(&mb, b, n, blocks8::round16(n), k, groups, true));
-    gemm8::Params p{};
-    p.rows = rows;
-    p.n = n;
-    p.kblocks = static_cast<int32_t>(kblocks);
-    p.groups = groups;
-    p.offsets = offsets;
-    p.sa = scales_a;
-    p.sb = scales_b;
-    p.sb_group = kblocks * nblocks;
-    p.sb_n = trans_b ? kblocks : 1;
-    p.sb_k = trans_b ? 1 : nblocks;
-    p.out = out;
-    p.out_dtype = out_dtype;
-    const bool pair = rows >= 256 * static_cast<int64_t>(groups);
-    return trans_b ? gemm8::run<false, false>(ma, mb, p, format_a, format_b, pair)
-                   : gemm8::run<true, false>(ma, mb, p, format_a, format_b, pair);
-}
-
-extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int64_t k,
-                                         int64_t places, const uint8_t *a, const float *scales_a,
-                                         const uint8_t *b, const float *scales_b,
-                                         const int32_t *offsets, int32_t groups, int32_t out_dtype,
-                                         void *out) {
-    CHELIS_TRY(gemm8::check_common("matmul8_wgrad", format_a, format_b, out_dtype, places, n, k, offsets, groups));
-    if (places % 128 != 0) return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8_wgrad: places in blocks of 128");
-    if (n == 0 || k == 0) return CHELIS_CUDA_OK;
-    if (!out) return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8_wgrad: null operand");
-    if (places == 0) return gemm8::zero_out(out, out_dtype, groups * n * k);
-    if (!a || !scales_a || !b || !scales_b)
-        return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8_wgrad: null operand");
-    if (!experts::aligned16(a) || !experts::aligned16(b))
-        return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8_wgrad: 8-bit data must lie on 16 bytes");
-    CUtensorMap ma, mb;
-    CHELIS_TRY(gemm8::make_map(&ma, a, places, places, n, 1, false));
-    CHELIS_TRY(gemm8::make_map(&mb, b, places, places, k, 1, false));
-    gemm8::Params p{};
-    p.rows = n;
-    p.n = k;
-    p.kblocks = static_cast<int32_t>(places / 128);
-    p.groups = groups;
-    p.offsets = offsets;
-    p.group_rows = places;  // the rows are no more
-    p.sa = scales_a;
-    p.sb = scales_b;
-    p.out = out;
-    p.out_dtype = out_dtype;
-    const bool pair = n > 128;
-    return gemm8::run<false, true>(ma, mb, p, format_a, format_b, pair);
-}

@@ -348,6 +348,8 @@ int chelis_cuda_device_status(void) {
         }
         if (word & DEVERR_BAD_INDEX)
             return set_error(CHELIS_CUDA_ERR_DOMAIN, "numeric trap: domain in gather at i64");
+        if (word & DEVERR_SCALE)
+            return set_error(CHELIS_CUDA_ERR_DOMAIN, "matmul8: a block scale is no power of two (any_scales admits it)");
         if (word & (DEVERR_DROPOUT_F32 | DEVERR_DROPOUT_F64))
             return set_error(CHELIS_CUDA_ERR_DOMAIN, "numeric trap: domain in dropout at %s",
                              (word & DEVERR_DROPOUT_F32) ? "f32" : "f64");

@@ -178,8 +178,8 @@ SIGNATURES = {
     "chelis_cuda_quantize8": (c_int, [c_i32, c_i32, c_i32, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "chelis_cuda_quantize8_places": (c_i64, [c_i64, c_i32]),
     "chelis_cuda_quantize8_transposed": (c_int, [c_i32, c_i32, c_vp, c_vp, c_i32, c_i64, c_i64, c_vp, c_vp]),
-    "chelis_cuda_matmul8": (c_int, [c_i32, c_i32, c_int, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_i32, c_vp]),
-    "chelis_cuda_matmul8_wgrad": (c_int, [c_i32, c_i32, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_i32, c_vp]),
+    "chelis_cuda_matmul8": (c_int, [c_i32, c_i32, c_int, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_int, c_i32, c_vp]),
+    "chelis_cuda_matmul8_wgrad": (c_int, [c_i32, c_i32, c_i64, c_i64, c_i64] + [c_vp] * 5 + [c_i32, c_int, c_i32, c_vp]),
     "chelis_cuda_dp_shard": (c_int, [c_i64, c_i32, c_i32, ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "chelis_cuda_dp_unique_id": (c_int, [c_vp]),
     "chelis_cuda_dp_init": (c_int, [c_i32, c_i32, c_vp]),

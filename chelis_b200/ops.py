@@ -737,12 +737,14 @@ def _check_blocks8(name: str, b: Blocks8, blocks: str) -> None:
 
 
 def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor | None = None,
-            dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+            dtype: torch.dtype = torch.bfloat16, any_scales: bool = False) -> torch.Tensor:
     """a . b^T (b [n, k]: a layer's product) or a . b (trans_b=False, b [k, n]:
     its input gradient, from the same weights) of 8-bit row blocks a [rows, k]
     and tiles b; f32 sums, rounded once to dtype.  With offsets (expert_sort's)
     b is a stack of matrices and rows [offsets[e], offsets[e + 1]) meet matrix
-    e; rows that no expert holds come out as zeros."""
+    e; rows that no expert holds come out as zeros.  Scales are powers of two,
+    as quantize8 makes them (others give NaN and raise at the next
+    device_status()); any_scales admits every scale, at a lower rate."""
     _check(dtype in _ACT, "matmul8 gives f32, bf16 or f16")
     _check_blocks8("matmul8", a, "rows")
     _check_blocks8("matmul8", b, "tiles")
@@ -760,15 +762,16 @@ def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor 
     out = torch.empty((rows, n), dtype=dtype, device=a.data.device)
     L.call("chelis_cuda_matmul8", _FORMAT[a.data.dtype], _FORMAT[b.data.dtype], int(trans_b), rows, n,
            k, a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
-           _ptr(offsets), groups, _ACT[dtype], out.data_ptr())
+           _ptr(offsets), groups, int(any_scales), _ACT[dtype], out.data_ptr())
     return out
 
 
 def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
-                  dtype: torch.dtype = torch.float32) -> torch.Tensor:
+                  dtype: torch.dtype = torch.float32, any_scales: bool = False) -> torch.Tensor:
     """The weight gradient dy^T . x [n, k] from the transposed 8-bit forms of
     dy [rows, n] and x [rows, k] (quantize8_transposed); with offsets one
-    matrix an expert, [experts, n, k], zeros for an expert without rows."""
+    matrix an expert, [experts, n, k], zeros for an expert without rows.
+    any_scales as in matmul8."""
     _check(dtype in _ACT, "matmul8_wgrad gives f32, bf16 or f16")
     _check_blocks8("matmul8_wgrad", dy, "rows")
     _check_blocks8("matmul8_wgrad", x, "rows")
@@ -785,5 +788,5 @@ def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
     out = torch.empty(shape, dtype=dtype, device=dy.data.device)
     L.call("chelis_cuda_matmul8_wgrad", _FORMAT[dy.data.dtype], _FORMAT[x.data.dtype], n, k, dy.cols,
            dy.data.data_ptr(), dy.scales.data_ptr(), x.data.data_ptr(), x.scales.data_ptr(),
-           _ptr(offsets), max(groups, 1), _ACT[dtype], out.data_ptr())
+           _ptr(offsets), max(groups, 1), int(any_scales), _ACT[dtype], out.data_ptr())
     return out

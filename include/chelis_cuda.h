@@ -646,7 +646,7 @@ int chelis_cuda_expert_combine_bwd(int32_t dtype, const void *dy, const void *ys
  *   rows   data [rows][ld(cols)], scales [ceil(cols/128)][rows]
  *   tiles  data [batch][rows][ld(cols)],
  *          scales [batch][ceil(rows/128)][ceil(cols/128)]
- * The products below take any f32 scales in these layouts. */
+ */
 enum { CHELIS_FORMAT_E4M3 = 0, CHELIS_FORMAT_E5M2 = 1 };
 enum { CHELIS_BLOCKS_ROWS = 0, CHELIS_BLOCKS_TILES = 1 };
 int chelis_cuda_quantize8(int32_t dtype, int32_t format, int32_t layout, const void *x,
@@ -663,18 +663,22 @@ int chelis_cuda_quantize8_transposed(int32_t dtype, int32_t format, const void *
 /* out[rows][n] = a . b^T (trans_b != 0, b [groups][n][k]) or a . b (b
  * [groups][k][n]): a in rows layout, b in tiles layout, f32 sums rounded once
  * to out_dtype.  Row r meets the matrix of the group that holds it; offsets
- * == NULL: one matrix.  Rows that no group holds are written as zeros. */
+ * == NULL: one matrix.  Rows that no group holds are written as zeros.
+ * any_scales == 0: the scales are powers of two, as quantize8 makes them, and
+ * the tensor core applies them; another scale makes the numbers under it NaN
+ * and is reported by chelis_cuda_device_status.  any_scales != 0 admits every
+ * f32 scale, at a lower rate. */
 int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows, int64_t n,
                         int64_t k, const uint8_t *a, const float *scales_a, const uint8_t *b,
                         const float *scales_b, const int32_t *offsets, int32_t groups,
-                        int32_t out_dtype, void *out);
+                        int any_scales, int32_t out_dtype, void *out);
 /* out[g][n][k] = sum over group g's rows t of A[t][n] * B[t][k], from the
  * transposed forms a [n][places] and b [k][places]; zeros for a group with no
  * rows. */
 int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int64_t k, int64_t places,
                               const uint8_t *a, const float *scales_a, const uint8_t *b,
                               const float *scales_b, const int32_t *offsets, int32_t groups,
-                              int32_t out_dtype, void *out);
+                              int any_scales, int32_t out_dtype, void *out);
 
 /* =========================================================================
  * Generated-entry device ABI (emit.rs:838-958, `f_device`): inputs borrowed,

@@ -55,15 +55,15 @@ def test_8_bit_entries_refuse():
     assert turned(L.DTYPE_F32, 0, one, one, 0, 4, 4, one, one) == DOMAIN
     assert turned(L.DTYPE_F32, 0, one, one, 1025, 4, 4, one, one) == UNSUPPORTED
     product = lib.chelis_cuda_matmul8
-    assert product(0, 0, 1, 0, 4, 4, None, None, None, None, None, 1, L.DTYPE_F32, None) == OK
-    assert product(0, 2, 1, 4, 4, 4, one, one, one, one, None, 1, L.DTYPE_F32, one) == UNSUPPORTED
-    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, None, 1, L.DTYPE_F64, one) == UNSUPPORTED
-    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, None, 2, L.DTYPE_F32, one) == DOMAIN
-    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, one, 1025, L.DTYPE_F32, one) == UNSUPPORTED
-    assert product(0, 0, 1, 4, 4, 4, odd, one, one, one, None, 1, L.DTYPE_F32, one) == DOMAIN
-    assert product(0, 0, 1, 4, -4, 4, one, one, one, one, None, 1, L.DTYPE_F32, one) == DOMAIN
-    assert product(0, 0, 1, 4, 1 << 31, 4, one, one, one, one, None, 1, L.DTYPE_F32, one) == UNSUPPORTED
+    assert product(0, 0, 1, 0, 4, 4, None, None, None, None, None, 1, 0, L.DTYPE_F32, None) == OK
+    assert product(0, 2, 1, 4, 4, 4, one, one, one, one, None, 1, 0, L.DTYPE_F32, one) == UNSUPPORTED
+    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, None, 1, 0, L.DTYPE_F64, one) == UNSUPPORTED
+    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, None, 2, 0, L.DTYPE_F32, one) == DOMAIN
+    assert product(0, 0, 1, 4, 4, 4, one, one, one, one, one, 1025, 0, L.DTYPE_F32, one) == UNSUPPORTED
+    assert product(0, 0, 1, 4, 4, 4, odd, one, one, one, None, 1, 0, L.DTYPE_F32, one) == DOMAIN
+    assert product(0, 0, 1, 4, -4, 4, one, one, one, one, None, 1, 0, L.DTYPE_F32, one) == DOMAIN
+    assert product(0, 0, 1, 4, 1 << 31, 4, one, one, one, one, None, 1, 0, L.DTYPE_F32, one) == UNSUPPORTED
     wgrad = lib.chelis_cuda_matmul8_wgrad
-    assert wgrad(0, 0, 4, 4, 100, one, one, one, one, None, 1, L.DTYPE_F32, one) == DOMAIN
+    assert wgrad(0, 0, 4, 4, 100, one, one, one, one, None, 1, 0, L.DTYPE_F32, one) == DOMAIN
     assert "places" in L.last_error()
-    assert wgrad(0, 0, 0, 4, 128, None, None, None, None, None, 1, L.DTYPE_F32, None) == OK
+    assert wgrad(0, 0, 0, 4, 128, None, None, None, None, None, 1, 0, L.DTYPE_F32, None) == OK

@@ -250,8 +250,72 @@ def test_matmul8_takes_any_scales(cuda):
     vb = R.values(_values(b8.data)[:, :300], b8.scales.cpu().double().numpy(), 128).T
     for rows in (150, 4):
         part = a8._replace(data=a8.data[:rows].contiguous(), scales=a8.scales[:, :rows].contiguous())
-        y = cuda.matmul8(part, b8, dtype=torch.float32)
+        y = cuda.matmul8(part, b8, dtype=torch.float32, any_scales=True)
         _near(y, va[:rows] @ vb, np.abs(va[:rows]) @ np.abs(vb), 300, "f32")
+
+
+@pytest.mark.parametrize("rows,n,k,counts,fa,fb,dtype,trans_b", [
+    (2100, 1000, 4100, None, "e4m3", "e4m3", "f32", True), (2049, 4096, 1000, None, "e5m2", "e4m3", "bf16", True),
+    (2100, 1000, 4100, None, "e5m2", "e4m3", "f32", False), (1500, 3001, 1500, None, "e4m3", "e5m2", "f16", True),
+    (2200, 2040, 900, [1000, 0, 7, 513, 670], "e4m3", "e4m3", "f32", True),
+    (4700, 520, 4200, [2500, 2190], "e4m3", "e4m3", "bf16", False),
+    (1700, 2055, 1300, [0, 900, 800, 0], "e5m2", "e5m2", "f32", False)])
+def test_matmul8_large(cuda, rows, n, k, counts, fa, fb, dtype, trans_b):
+    """Enough work for the kernel that leaves the scales to the tensor core, in
+    single blocks and in pairs, with ragged rows and columns."""
+    import torch
+    rng = np.random.default_rng(rows + n + k)
+    a8, b8, va, vb = _operands(cuda, rng, rows, n, k, None if counts is None else len(counts), trans_b, fa, fb)
+    off = None if counts is None else _offsets(counts)
+    y = cuda.matmul8(a8, b8, trans_b, off, _dtype(dtype))
+    at = 0
+    for e, c in enumerate([rows] if counts is None else counts):
+        w = vb if counts is None else vb[e]
+        _near(y[at:at + c], va[at:at + c] @ w, np.abs(va[at:at + c]) @ np.abs(w), k, dtype)
+        at += c
+    assert not y[at:].any()
+    assert torch.equal(y, cuda.matmul8(a8, b8, trans_b, off, _dtype(dtype)))
+    cuda.device_status()
+
+
+@pytest.mark.parametrize("counts,n,k,dtype", [([4300], 1500, 1300, "f32"), ([1700], 2000, 2300, "bf16"),
+                                              ([3000, 0, 130, 5000, 1], 1100, 1030, "f32"),
+                                              ([128, 640, 500, 700], 2048, 2048, "f16")])
+def test_matmul8_wgrad_large(cuda, counts, n, k, dtype):
+    rng = np.random.default_rng(n + k)
+    rows = sum(counts)
+    dy, _ = _input(rng, (rows, n), "f32")
+    x, _ = _input(rng, (rows, k), "f32")
+    off = _offsets(counts) if len(counts) > 1 else None
+    a8, b8 = cuda.quantize8_transposed(dy, "e5m2", off), cuda.quantize8_transposed(x, "e4m3", off)
+    va = R.values(_values(a8.data), a8.scales.cpu().double().numpy().T, 1)
+    vb = R.values(_values(b8.data), b8.scales.cpu().double().numpy().T, 1)
+    got = cuda.matmul8_wgrad(a8, b8, off, _dtype(dtype))
+    at = 0
+    for e, c in enumerate(counts):
+        end = at + -(-c // 128) * 128
+        _near(got[e] if off is not None else got, va[:, at:end] @ vb[:, at:end].T,
+              np.abs(va[:, at:end]) @ np.abs(vb[:, at:end]).T, c, dtype)
+        at = end
+    cuda.device_status()
+
+
+def test_matmul8_reports_scales_that_are_no_powers_of_two(cuda):
+    """Where the tensor core applies the scales it takes powers of two; another
+    one makes the numbers under it NaN, is reported, and any_scales admits it."""
+    import torch
+    from chelis_b200 import lib as L
+    a8 = cuda.quantize8(torch.ones((2048, 1024), device="cuda"))
+    b8 = cuda.quantize8(torch.ones((4096, 1024), device="cuda"), "e4m3", "tiles")
+    a8.scales[3, 77] *= 1.5
+    y = cuda.matmul8(a8, b8)
+    torch.cuda.synchronize()
+    with pytest.raises(L.ChelisCudaError, match="power of two"):
+        cuda.device_status()
+    assert y[77].isnan().all() and not y[:77].isnan().any() and not y[78:].isnan().any()
+    z = cuda.matmul8(a8, b8, any_scales=True)
+    cuda.device_status()
+    assert (z[77] == 1024 + 64).all() and (z[78:] == 1024).all()
 
 
 def test_matmul8_keeps_nan_to_its_row(cuda):
