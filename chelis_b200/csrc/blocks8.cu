@@ -36,129 +36,251 @@ constexpr int MAX_GROUPS = experts::MAX_EXPERTS;
 using experts::Pack;
 using experts::to_f32;
 
-// 8 consecutive elements from p[0..valid), zeros beyond.
+// 8 consecutive elements, held as they were loaded (16-bit ones in half the
+// registers, so that more thread blocks are resident) and read as f32.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *p, int64_t valid, float (&v)[8]) {
-    if (VEC && valid >= 8) {
-        constexpr int N = 16 / static_cast<int>(sizeof(T));
+struct Eight {
+    static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+    Pack<T, VEC> r[8 / N];
+    __device__ __forceinline__ float operator[](int i) const { return to_f32(r[i / N].v[i % N]); }
+};
+// From p[0..valid), zeros beyond.  VEC: in 16-byte packs, none of which
+// straddles the end (the width is a multiple of one).
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T, VEC> load8(const T *p, int valid) {
+    using E = Eight<T, VEC>;
+    E v{};
 #pragma unroll
-        for (int u = 0; u < 8 / N; ++u) {
-            const Pack<T, true> r = experts::load_pack<T, true>(p + u * N);
+    for (int u = 0; u < 8 / E::N; ++u)
+        if (u * E::N < valid) v.r[u] = experts::load_pack<T, VEC>(p + u * E::N);
+    return v;
+}
+
+// Magnitudes are compared as bits, which order as the numbers do, 16-bit ones
+// two at a time: nothing is converted before the scale is known, so a block
+// waits for it in the registers that it was loaded into (as f32 it took twice
+// as many, and spilled).  A running maximum holds bits of T (two halves of it
+// for a 16-bit T), magnitude_key turns it into f32 bits.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint32_t max8(const Eight<T, VEC> &v, uint32_t most) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[u * N + i] = to_f32(r.v[i]);
-        }
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+    } else if constexpr (VEC) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(&v);
+        most = __vmaxu2(most, w.x & 0x7fff7fffu);
+        most = __vmaxu2(most, w.y & 0x7fff7fffu);
+        most = __vmaxu2(most, w.z & 0x7fff7fffu);
+        most = __vmaxu2(most, w.w & 0x7fff7fffu);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            most = max(most, static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&v.r[i].v[0])) & 0x7fffu);
+    }
+    return most;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t key_of_bits(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) {
+        return bits;
+    } else {
+        const uint16_t h = static_cast<uint16_t>(bits);
+        return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
     }
 }
-
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a < INFINITY ? a : 0.0f;
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude_key(uint32_t most) {
+    return sizeof(T) == 4 ? most : key_of_bits<T>(max(most & 0xffffu, most >> 16));
 }
+// An infinity or a NaN is among them: the block goes the slow way.
+__device__ __forceinline__ bool special(uint32_t key) { return key >= 0x7f800000u; }
 
-// Exponent of the scale from the block's largest finite magnitude.  The
+// Exponent of the scale from the bits of the block's largest finite magnitude.  The
 // largest value is 1.75 * 2^TOP in both formats, so amax = m * 2^x needs
 // x - TOP, one more when m > 1.75.
 template <bool E5M2>
-__device__ __forceinline__ int scale_exponent(float amax) {
+__device__ __forceinline__ int scale_exponent(uint32_t b) {
     constexpr int TOP = E5M2 ? 15 : 8;
-    if (amax == 0.0f) return 0;
-    const uint32_t b = __float_as_uint(amax);
+    if (b == 0) return 0;
     const int e = static_cast<int>(b >> 23) - 127 - TOP + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
 }
 __device__ __forceinline__ float power2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-// 8 numbers times inv to 8 bytes (element 0 lowest).
-template <bool E5M2>
-__device__ __forceinline__ uint2 convert8(const float (&v)[8], float inv) {
+// 8 numbers times inv to 8 bytes (element 0 lowest).  The conversion keeps
+// NaNs; a block with an infinity, which it would saturate, does not come here.
+template <bool E5M2, typename V>
+__device__ __forceinline__ uint2 convert8(const V &v, float inv) {
     uint16_t h[4];
-    bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float lo = v[2 * i] * inv, hi = v[2 * i + 1] * inv;
-        odd |= !(fabsf(lo) < INFINITY) || !(fabsf(hi) < INFINITY);
         if (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(h[i]) : "f"(hi), "f"(lo));
         else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h[i]) : "f"(hi), "f"(lo));
     }
-    uint2 r = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
-    if (odd) {  // the conversion saturates infinities: put them right
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (fabsf(v[i]) < INFINITY) continue;
-            uint32_t code = (E5M2 && v[i] == v[i]) ? 0x7cu : 0x7fu;
-            if (v[i] < 0.0f) code |= 0x80u;
-            uint32_t &w = i < 4 ? r.x : r.y;
-            w = (w & ~(0xffu << (8 * (i & 3)))) | (code << (8 * (i & 3)));
-        }
-    }
-    return r;
+    return make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+}
+// Blocks with an infinity or a NaN are done again one number at a time, from
+// memory, by functions of their own: kept out of line and called last, they
+// cost the usual blocks no registers (inlined, or called where a block is
+// held, they made the kernels below spill).
+template <bool E5M2>
+__device__ __forceinline__ uint8_t convert1(float v, float inv) {
+    uint16_t h;
+    const float x = v * inv;
+    if (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(h) : "f"(0.0f), "f"(x));
+    else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(0.0f), "f"(x));
+    if (fabsf(v) == INFINITY) h = (E5M2 ? 0x7c : 0x7f) | (v < 0.0f ? 0x80 : 0);
+    return static_cast<uint8_t>(h);
+}
+__device__ __forceinline__ uint32_t finite_key(float v, uint32_t most) {
+    const uint32_t key = __float_as_uint(fabsf(v));
+    return special(key) ? most : max(most, key);
+}
+// One thread, up to 128 numbers `step` apart.
+template <typename T, bool E5M2>
+__device__ __noinline__ void slow_block(const T *x, int64_t step, int n, uint8_t *q, float *scale) {
+    uint32_t key = 0;
+    for (int i = 0; i < n; ++i) key = finite_key(to_f32(x[i * step]), key);
+    const int e = scale_exponent<E5M2>(key);
+    *scale = power2(e);
+    for (int i = 0; i < n; ++i) q[i] = convert1<E5M2>(to_f32(x[i * step]), power2(-e));
 }
 
-// Blocks of a row: 16 lanes hold one, 8 elements a lane; a thread block takes
-// 16 rows of one column block, so a warp reads two rows' 128 elements and
-// the 16 scales go out together.
+// Blocks of a row: LANES lanes hold one, 8 elements a lane at a time; a thread
+// block takes ROWS rows of RUN consecutive column blocks, whose loads are all
+// in flight before the first maximum is formed, and the rows' scales of a
+// block go out together.  f32 is bound by memory with 16 lanes; 16-bit types
+// were bound by the ALU's work around each maximum (71 % busy, 48 us for
+// 16384 x 4096) and take 8 lanes of 16 elements, which halves it.
+constexpr int RUN = 4;
+template <typename T>
+struct RowShape {
+    static constexpr int LANES = sizeof(T) == 2 ? 8 : 16;
+    static constexpr int EIGHTS = 16 / LANES;  // of a lane
+    static constexpr int ROWS = THREADS / LANES;
+};
+
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     rows_kernel(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, int64_t kb,
                 uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;
-    const int64_t row_tiles = (rows + 15) / 16;
-    for (int64_t w = blockIdx.x; w < row_tiles * kb; w += gridDim.x) {
-        const int64_t row = (w / kb) * 16 + sub, b = w % kb;
-        const int64_t col = b * BLOCK + part * 8;
-        float v[8] = {};
-        if (row < rows && col < cols) load8<T, VEC>(x + row * cols + col, cols - col, v);
-        float amax = 0.0f;
+    constexpr int LANES = RowShape<T>::LANES, EIGHTS = RowShape<T>::EIGHTS, ROWS = RowShape<T>::ROWS;
+    const int part = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    const int64_t row_tiles = (rows + ROWS - 1) / ROWS, runs = (kb + RUN - 1) / RUN;
+    for (int64_t w = blockIdx.x; w < row_tiles * runs; w += gridDim.x) {
+        const int64_t tile = w / runs, b0 = (w - tile * runs) * RUN;
+        const int64_t row = tile * ROWS + sub, col0 = b0 * BLOCK;
+        const bool in = row < rows;
+        const T *src = x + row * cols + col0 + part * 8;
+        uint8_t *dst = q + row * ld + col0 + part * 8;
+        // columns from this lane's first on, of the data and of its padded row
+        const int left = in ? static_cast<int>(cols - col0 < RUN * BLOCK ? cols - col0 : RUN * BLOCK) - part * 8 : 0;
+        const int wide = in ? static_cast<int>(ld - col0 < RUN * BLOCK ? ld - col0 : RUN * BLOCK) - part * 8 : 0;
+        Eight<T, VEC> v[RUN][EIGHTS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[i]));
+        for (int u = 0; u < RUN; ++u)
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        const int e = scale_exponent<E5M2>(amax);
-        if (row < rows) {
-            if (part == 0) scales[b * rows + row] = power2(e);
-            if (col < ld) *reinterpret_cast<uint2 *>(q + row * ld + col) = convert8<E5M2>(v, power2(-e));
+            for (int h = 0; h < EIGHTS; ++h) {
+                const int o = u * BLOCK + h * LANES * 8;
+                v[u][h] = load8<T, VEC>(src + o, left - o);
+            }
+        uint32_t odd = 0;
+#pragma unroll
+        for (int u = 0; u < RUN; ++u) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int h = 0; h < EIGHTS; ++h) most = max8(v[u][h], most);
+            uint32_t key = magnitude_key<T>(most);
+#pragma unroll
+            for (int off = LANES / 2; off > 0; off >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, off));
+            if (special(key)) {
+                odd |= 1u << u;
+                continue;
+            }
+            const int e = scale_exponent<E5M2>(key);
+            if (part == 0 && in && b0 + u < kb) scales[(b0 + u) * rows + row] = power2(e);
+            const float inv = power2(-e);
+#pragma unroll
+            for (int h = 0; h < EIGHTS; ++h) {
+                const int o = u * BLOCK + h * LANES * 8;
+                if (wide > o) *reinterpret_cast<uint2 *>(dst + o) = convert8<E5M2>(v[u][h], inv);
+            }
         }
+        if (odd && part == 0 && in)
+            for (int u = 0; u < RUN; ++u)
+                if (odd >> u & 1) {
+                    const int64_t col = col0 + u * BLOCK;
+                    const int n = static_cast<int>(cols - col < BLOCK ? cols - col : BLOCK);
+                    slow_block<T, E5M2>(x + row * cols + col, 1, n, q + row * ld + col, scales + (b0 + u) * rows + row);
+                    for (int64_t c = cols; c < ld && c < col + BLOCK; ++c) q[row * ld + c] = 0;
+                }
+    }
+}
+
+// The largest of the thread block's numbers.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *warp_part) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();  // the last use of warp_part is over
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) v = max(v, warp_part[i]);
+    return v;
+}
+
+template <typename T, bool E5M2>
+__device__ __noinline__ void slow_tile(const T *x, int64_t rows, int64_t cols, int64_t ld, int64_t row0,
+                                       int64_t col0, uint8_t *q, float *scale, uint32_t *warp_part) {
+    uint32_t key = 0;
+    for (int i = threadIdx.x; i < BLOCK * BLOCK; i += THREADS) {
+        const int64_t row = row0 + i / BLOCK, col = col0 + i % BLOCK;
+        if (row < rows && col < cols) key = finite_key(to_f32(x[row * cols + col]), key);
+    }
+    const int e = scale_exponent<E5M2>(block_max(key, warp_part));
+    if (threadIdx.x == 0) *scale = power2(e);
+    for (int i = threadIdx.x; i < BLOCK * BLOCK; i += THREADS) {
+        const int64_t row = row0 + i / BLOCK, col = col0 + i % BLOCK;
+        if (row < rows && col < ld)
+            q[row * ld + col] = col < cols ? convert1<E5M2>(to_f32(x[row * cols + col]), power2(-e)) : 0;
     }
 }
 
 // A 128 x 128 tile a thread block: 8 rows a thread, 8 elements of each.
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 3 : 2)
     tiles_kernel(const T *__restrict__ x, int64_t batch, int64_t rows, int64_t cols, int64_t ld,
                  uint8_t *__restrict__ q, float *__restrict__ scales) {
-    __shared__ float warp_amax[THREADS / 32];
+    __shared__ uint32_t warp_most[THREADS / 32];
     const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;
     const int64_t rb = (rows + BLOCK - 1) / BLOCK, kb = (cols + BLOCK - 1) / BLOCK;
     for (int64_t w = blockIdx.x; w < batch * rb * kb; w += gridDim.x) {
         const int64_t b = w / (rb * kb), in = w - b * rb * kb;
-        const int64_t row0 = (in / kb) * BLOCK + sub, col = (in % kb) * BLOCK + part * 8;
-        float v[8][8];
-        float amax = 0.0f;
+        const int64_t trow = in / kb, row0 = trow * BLOCK + sub, col = (in - trow * kb) * BLOCK + part * 8;
+        const T *src = x + (b * rows + row0) * cols + col;
+        uint8_t *dst = q + (b * rows + row0) * ld + col;
+        const int64_t src_step = 16 * cols, dst_step = 16 * ld;
+        const int high = static_cast<int>(rows - row0 < BLOCK ? rows - row0 : BLOCK);  // rows from this one on
+        const int left = static_cast<int>(cols - col < 8 ? cols - col : 8);
+        const bool store = col < ld;
+        Eight<T, VEC> v[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int64_t row = row0 + r * 16;
+        for (int r = 0; r < 8; ++r) v[r] = load8<T, VEC>(src + r * src_step, r * 16 < high ? left : 0);
+        uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
-            if (row < rows && col < cols) load8<T, VEC>(x + (b * rows + row) * cols + col, cols - col, v[r]);
+        for (int r = 0; r < 8; ++r) most = max8(v[r], most);
+        const uint32_t key = block_max(magnitude_key<T>(most), warp_most);
+        if (!special(key)) {
+            const int e = scale_exponent<E5M2>(key);
+            if (threadIdx.x == 0) scales[w] = power2(e);
+            const float inv = power2(-e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[r][i]));
-        }
-        amax = warp_max(amax);
-        __syncthreads();  // the previous tile's maxima have been read
-        if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < THREADS / 32; ++i) amax = fmaxf(amax, warp_amax[i]);
-        const int e = scale_exponent<E5M2>(amax);
-        if (threadIdx.x == 0) scales[w] = power2(e);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int64_t row = row0 + r * 16;
-            if (row < rows && col < ld)
-                *reinterpret_cast<uint2 *>(q + (b * rows + row) * ld + col) = convert8<E5M2>(v[r], power2(-e));
+            for (int r = 0; r < 8; ++r)
+                if (r * 16 < high && store)
+                    *reinterpret_cast<uint2 *>(dst + r * dst_step) = convert8<E5M2>(v[r], inv);
+        } else {  // the whole block
+            slow_tile<T, E5M2>(x + b * rows * cols, rows, cols, ld, trow * BLOCK, (in - trow * kb) * BLOCK,
+                               q + b * rows * ld, scales + w, warp_most);
         }
     }
 }
@@ -192,17 +314,45 @@ __device__ __forceinline__ void block_rows(const int32_t *offsets, int groups, i
     }
 }
 
+// f32 bits of the largest magnitude in each of the 8 columns of 8 rows.
+template <typename T, bool VEC>
+__device__ __forceinline__ void column_keys(const Eight<T, VEC> (&v)[8], uint32_t (&key)[8]) {
+    if constexpr (sizeof(T) == 2 && VEC) {
+        uint4 m = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(&v[r]);
+            m.x = __vmaxu2(m.x, w.x & 0x7fff7fffu);
+            m.y = __vmaxu2(m.y, w.y & 0x7fff7fffu);
+            m.z = __vmaxu2(m.z, w.z & 0x7fff7fffu);
+            m.w = __vmaxu2(m.w, w.w & 0x7fff7fffu);
+        }
+        const uint32_t w[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) key[i] = key_of_bits<T>((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            key[i] = 0;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) key[i] = max(key[i], __float_as_uint(fabsf(v[r][i])));
+        }
+    }
+}
+
 // 128 rows x 128 columns a thread block, turned over in shared memory as
 // bytes.  A thread holds rows 8 sub .. 8 sub + 7 of 8 columns: its 8 bytes of
 // a column are consecutive places.
 template <typename T, bool E5M2, bool VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 3 : 2)
     transposed_kernel(const T *__restrict__ x, const int32_t *__restrict__ offsets, int groups,
                       int64_t rows, int64_t cols, int64_t blocks, uint8_t *__restrict__ q,
                       float *__restrict__ scales) {
+    // column c's eight bytes of rows 8 s .. 8 s + 7 lie in slot s ^ (c / 8 mod
+    // 16) of its 128, so that neither the threads' stores nor the loads collide
     constexpr int PITCH = BLOCK + 16;
     __shared__ __align__(16) uint8_t tile[BLOCK * PITCH];
-    __shared__ float amax_part[16][BLOCK];
+    __shared__ __align__(16) uint32_t most_part[16][BLOCK];
     __shared__ int64_t row_s;
     __shared__ int len_s;
     const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;
@@ -214,28 +364,31 @@ __global__ void __launch_bounds__(THREADS)
         __syncthreads();
         const int64_t row0 = row_s, col = col0 + part * 8;
         const int len = len_s;
-        float v[8][8], amax[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax[i] = 0.0f;
+        const T *src = x + (row0 + sub * 8) * cols + col;
+        const int left = static_cast<int>(cols - col < 8 ? cols - col : 8);
+        Eight<T, VEC> v[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const int in = sub * 8 + r;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
-            if (in < len && col < cols) load8<T, VEC>(x + (row0 + in) * cols + col, cols - col, v[r]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax[i] = fmaxf(amax[i], finite_abs(v[r][i]));
+            v[r] = load8<T, VEC>(src + r * cols, in < len ? left : 0);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax_part[sub][part * 8 + i] = amax[i];
+        {
+            uint32_t key[8];
+            column_keys(v, key);
+            uint4 *to = reinterpret_cast<uint4 *>(&most_part[sub][part * 8]);
+            to[0] = make_uint4(key[0], key[1], key[2], key[3]);
+            to[1] = make_uint4(key[4], key[5], key[6], key[7]);
+        }
         __syncthreads();
+        bool odd = false;  // this thread's column
         if (threadIdx.x < BLOCK) {
-            float a = 0.0f;
+            uint32_t a = 0;
 #pragma unroll
-            for (int s = 0; s < 16; ++s) a = fmaxf(a, amax_part[s][threadIdx.x]);
-            amax_part[0][threadIdx.x] = a;
-            if (col0 + threadIdx.x < cols)
-                scales[b * cols + col0 + threadIdx.x] = power2(scale_exponent<E5M2>(a));
+            for (int s = 0; s < 16; ++s) a = max(a, most_part[s][threadIdx.x]);
+            const int e = special(a) ? 0 : scale_exponent<E5M2>(a);
+            most_part[0][threadIdx.x] = static_cast<uint32_t>(127 - e) << 23;  // bits of 1 / scale
+            odd = special(a);
+            if (col0 + threadIdx.x < cols) scales[b * cols + col0 + threadIdx.x] = power2(e);
         }
         __syncthreads();
 #pragma unroll
@@ -243,16 +396,21 @@ __global__ void __launch_bounds__(THREADS)
             float c[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) c[r] = v[r][i];
-            const int e = scale_exponent<E5M2>(amax_part[0][part * 8 + i]);
-            *reinterpret_cast<uint2 *>(tile + (part * 8 + i) * PITCH + sub * 8) = convert8<E5M2>(c, power2(-e));
+            uint8_t *to = tile + (part * 8 + i) * PITCH + (sub ^ part) * 8;
+            *reinterpret_cast<uint2 *>(to) = convert8<E5M2>(c, __uint_as_float(most_part[0][part * 8 + i]));
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < BLOCK * BLOCK / (16 * THREADS); ++u) {
-            const int i = u * THREADS + threadIdx.x, c = i >> 3, o = (i & 7) * 16;
-            if (col0 + c < cols)
-                *reinterpret_cast<uint4 *>(q + (col0 + c) * places + b * BLOCK + o) =
-                    *reinterpret_cast<const uint4 *>(tile + c * PITCH + o);
+            const int i = u * THREADS + threadIdx.x, c = i >> 3, pair = i & 7, turn = (c >> 3) & 15;
+            uint4 w = *reinterpret_cast<const uint4 *>(tile + c * PITCH + (pair ^ (turn >> 1)) * 16);
+            if (turn & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+            if (col0 + c < cols) *reinterpret_cast<uint4 *>(q + (col0 + c) * places + b * BLOCK + pair * 16) = w;
+        }
+        if (__syncthreads_or(odd)) {  // columns done again, over what was just written
+            const int64_t c = col0 + threadIdx.x;
+            if (odd && c < cols)
+                slow_block<T, E5M2>(x + row0 * cols + c, cols, len, q + c * places + b * BLOCK, scales + b * cols + c);
         }
     }
 }
@@ -305,7 +463,8 @@ extern "C" int chelis_cuda_quantize8(int32_t dtype, int32_t format, int32_t layo
         constexpr bool E5M2 = decltype(f)::value, VEC = decltype(v)::value;
         if (layout == CHELIS_BLOCKS_ROWS)
             blocks8::rows_kernel<T, E5M2, VEC>
-                <<<blocks8::grid_for((rows + 15) / 16 * kb, 32), blocks8::THREADS, 0, s>>>(
+                <<<blocks8::grid_for((rows + blocks8::RowShape<T>::ROWS - 1) / blocks8::RowShape<T>::ROWS *
+                                        ((kb + blocks8::RUN - 1) / blocks8::RUN), 32), blocks8::THREADS, 0, s>>>(
                     static_cast<const T *>(x), rows, cols, ld, kb, data, scales);
         else
             blocks8::tiles_kernel<T, E5M2, VEC>

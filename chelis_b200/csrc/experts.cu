@@ -388,7 +388,10 @@ __global__ void __launch_bounds__(ROW_THREADS)
 }
 
 // y[t] = sum_j w[t, j] ys[position[t, j]] in f32, slot order, rounded once.
-// Without weights it is the gradient of spread_kernel.
+// Without weights it is the gradient of spread_kernel.  A warp takes DEEP
+// packs a lane of one token; its lanes hold the token's positions and weights.
+constexpr int DEEP = 2;
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS)
     combine_kernel(const T *__restrict__ ys, const float *__restrict__ weights,
@@ -396,31 +399,48 @@ __global__ void __launch_bounds__(ROW_THREADS)
                    T *__restrict__ y) {
     using P = Pack<T, VEC>;
     const int lane = threadIdx.x & 31;
-    const int64_t span = static_cast<int64_t>(32) * P::N;
+    const int64_t span = static_cast<int64_t>(32) * DEEP * P::N;
     const int64_t pieces = (hidden + span - 1) / span;
     const int64_t warps = static_cast<int64_t>(gridDim.x) * (ROW_THREADS / 32);
     const int64_t rows = tokens * k;
     for (int64_t w = (static_cast<int64_t>(blockIdx.x) * ROW_THREADS + threadIdx.x) >> 5;
          w < tokens * pieces; w += warps) {
-        const int64_t t = w / pieces, c = (w - t * pieces) * span + lane * P::N;
-        if (c >= hidden) continue;
-        float acc[P::N] = {};
-        for (int j = 0; j < k; ++j) {
-            const int64_t at = position[t * k + j];
-            if (at < 0) continue;
-            if (at >= rows) {
+        const int64_t t = w / pieces, c0 = (w - t * pieces) * span + lane * P::N;
+        int at_lane = -1;
+        float w_lane = 0.0f;
+        if (lane < k) {
+            at_lane = position[t * k + lane];
+            w_lane = weights ? weights[t * k + lane] : 1.0f;
+            if (at_lane >= rows) {
                 report_device_error(DEVERR_BAD_INDEX);
-                continue;
+                at_lane = -1;
             }
-            const float wj = weights ? weights[t * k + j] : 1.0f;
-            const P r = load_pack<T, VEC>(ys + at * hidden + c);
-#pragma unroll
-            for (int i = 0; i < P::N; ++i) acc[i] = fmaf(wj, to_f32(r.v[i]), acc[i]);
         }
-        P out;
+        float acc[DEEP][P::N] = {};
+#pragma unroll 2
+        for (int j = 0; j < k; ++j) {
+            const int64_t at = __shfl_sync(0xffffffffu, at_lane, j);
+            const float wj = __shfl_sync(0xffffffffu, w_lane, j);
+            if (at < 0) continue;
+            P r[DEEP];
 #pragma unroll
-        for (int i = 0; i < P::N; ++i) out.v[i] = from_f32<T>(acc[i]);
-        store_pack<T, VEC>(y + t * hidden + c, out);
+            for (int u = 0; u < DEEP; ++u) {
+                r[u] = P{};
+                if (c0 + u * 32 * P::N < hidden) r[u] = load_pack<T, VEC>(ys + at * hidden + c0 + u * 32 * P::N);
+            }
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u)
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) acc[u][i] = fmaf(wj, to_f32(r[u].v[i]), acc[u][i]);
+        }
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            const int64_t c = c0 + u * 32 * P::N;
+            P out;
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) out.v[i] = from_f32<T>(acc[u][i]);
+            if (c < hidden) store_pack<T, VEC>(y + t * hidden + c, out);
+        }
     }
 }
 
@@ -649,7 +669,7 @@ extern "C" int chelis_cuda_expert_combine(int32_t dtype, const void *ys, const f
     experts::by_type(dtype, vec, [&](auto t, auto v) {
         using T = decltype(t);
         constexpr bool VEC = decltype(v)::value;
-        const int64_t span = static_cast<int64_t>(32) * experts::Pack<T, VEC>::N;
+        const int64_t span = static_cast<int64_t>(32) * experts::DEEP * experts::Pack<T, VEC>::N;
         experts::combine_kernel<T, VEC>
             <<<experts::row_grid(tokens * ((hidden + span - 1) / span)), experts::ROW_THREADS, 0, s>>>(
                 static_cast<const T *>(ys), weights, position, tokens, k, hidden, static_cast<T *>(y));

@@ -23,8 +23,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the handle of a device's current stream; torch.cuda.current_stream makes a
+# Stream object around it, a microsecond more at every call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _prepare(*tensors: torch.Tensor) -> None:
-    dev = None
+    last = None
     for t in tensors:
         if t is None:
             continue
@@ -32,13 +38,12 @@ def _prepare(*tensors: torch.Tensor) -> None:
             raise ValueError("chelis_b200 ops take CUDA tensors (device memory)")
         if not t.is_contiguous():
             raise ValueError("chelis_b200 ops take contiguous tensors")
-        dev = t.device.index
-    if dev is None:
-        dev = torch.cuda.current_device()
+        last = t
+    dev = torch.cuda.current_device() if last is None else last.device.index
     if dev not in _initialised:
         L.call("chelis_cuda_init", dev)
         _initialised.add(dev)
-    L.load().chelis_cuda_set_stream(torch.cuda.current_stream(dev).cuda_stream)
+    L.load().chelis_cuda_set_stream(_raw_stream(dev))
 
 
 @contextlib.contextmanager
@@ -556,13 +561,17 @@ def _check(ok: bool, message: str) -> None:
 
 
 def _check_i32(name: str, *tensors: torch.Tensor) -> None:
-    _check(all(t.dtype == torch.int32 for t in tensors), f"{name} takes int32 indices")
+    for t in tensors:
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} takes int32 indices")
 
 
 def _check_order(name: str, order: ExpertOrder) -> None:
-    _check_i32(name, *order)
-    _check(order.position.dim() == 2 and order.offsets.dim() == 1 and order.offsets.numel() >= 2
-           and order.source.shape == (order.position.numel(),), f"{name} takes expert_sort's order")
+    offsets, position, source = order
+    _check_i32(name, offsets, position, source)
+    if not (position.dim() == 2 and offsets.dim() == 1 and offsets.numel() >= 2
+            and source.dim() == 1 and source.numel() == position.numel()):
+        raise ValueError(f"{name} takes expert_sort's order")
 
 
 def _routed(order: ExpertOrder) -> int:
@@ -579,8 +588,9 @@ def expert_route(logits: torch.Tensor, k: int, renormalize: bool = True):
     _check(logits.dim() == 2, "expert_route takes logits [tokens, experts]")
     _prepare(logits)
     tokens, experts = logits.shape
-    weights = torch.empty((tokens, max(k, 0)), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((tokens, max(k, 0)), dtype=torch.int32, device=logits.device)
+    slots, dev = max(k, 0), logits.device
+    weights = torch.empty(tokens, slots, dtype=torch.float32, device=dev)
+    ids = torch.empty(tokens, slots, dtype=torch.int32, device=dev)
     L.call("chelis_cuda_expert_route", dt, logits.data_ptr(), tokens, experts, k, int(renormalize),
            weights.data_ptr(), ids.data_ptr())
     return weights, ids
@@ -627,7 +637,7 @@ def expert_gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
            "expert_gather takes x [tokens, hidden]")
     _prepare(x, *order)
     tokens, k = order.position.shape
-    xs = torch.empty((tokens * k, x.shape[1]), dtype=x.dtype, device=x.device)
+    xs = torch.empty(tokens * k, x.shape[1], dtype=x.dtype, device=x.device)
     L.call("chelis_cuda_expert_spread", dt, x.data_ptr(), order.position.data_ptr(), _routed(order),
            tokens, k, x.shape[1], xs.data_ptr())
     return xs
@@ -641,7 +651,7 @@ def _expert_combine(name, ys, weights, order):
     _check(weights is None or (weights.dtype == torch.float32 and weights.shape == (tokens, k)),
            f"{name} takes f32 weights [tokens, k]")
     _prepare(ys, weights, *order)
-    y = torch.empty((tokens, ys.shape[1]), dtype=ys.dtype, device=ys.device)
+    y = torch.empty(tokens, ys.shape[1], dtype=ys.dtype, device=ys.device)
     L.call("chelis_cuda_expert_combine", dt, ys.data_ptr(), _ptr(weights), order.position.data_ptr(),
            tokens, k, ys.shape[1], y.data_ptr())
     return y
@@ -695,9 +705,9 @@ def quantize8(x: torch.Tensor, format: str = "e4m3", blocks: str = "rows") -> Bl
     rows, cols = x.shape[-2:]
     batch = x.shape[0] if x.dim() == 3 else 1
     kb = _ceil(cols, 128)
-    data = torch.empty((*x.shape[:-1], _ceil(cols, 16) * 16), dtype=_FLOAT8[format], device=x.device)
+    data = torch.empty(*x.shape[:-1], _ceil(cols, 16) * 16, dtype=_FLOAT8[format], device=x.device)
     shape = (kb, rows) if blocks == "rows" else (*x.shape[:-2], _ceil(rows, 128), kb)
-    scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    scales = torch.empty(*shape, dtype=torch.float32, device=x.device)
     L.call("chelis_cuda_quantize8", dt, _FORMAT[data.dtype],
            L.BLOCKS_ROWS if blocks == "rows" else L.BLOCKS_TILES, x.data_ptr(), batch, rows, cols,
            data.data_ptr(), scales.data_ptr())
@@ -720,8 +730,8 @@ def quantize8_transposed(x: torch.Tensor, format: str = "e4m3",
     _prepare(x, offsets)
     rows, cols = x.shape
     places = int(L.load().chelis_cuda_quantize8_places(rows, groups))
-    data = torch.empty((cols, places), dtype=_FLOAT8[format], device=x.device)
-    scales = torch.empty((places // 128, cols), dtype=torch.float32, device=x.device)
+    data = torch.empty(cols, places, dtype=_FLOAT8[format], device=x.device)
+    scales = torch.empty(places // 128, cols, dtype=torch.float32, device=x.device)
     L.call("chelis_cuda_quantize8_transposed", dt, _FORMAT[data.dtype], x.data_ptr(), _ptr(offsets),
            groups, rows, cols, data.data_ptr(), scales.data_ptr())
     return Blocks8(data, scales, places, "rows")
@@ -759,7 +769,7 @@ def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor 
     _check(a.cols == k, f"contraction extents differ: {a.cols} vs {k}")
     _prepare(a.data, a.scales, b.data, b.scales, offsets)
     rows = a.data.shape[0]
-    out = torch.empty((rows, n), dtype=dtype, device=a.data.device)
+    out = torch.empty(rows, n, dtype=dtype, device=a.data.device)
     L.call("chelis_cuda_matmul8", _FORMAT[a.data.dtype], _FORMAT[b.data.dtype], int(trans_b), rows, n,
            k, a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
            _ptr(offsets), groups, int(any_scales), _ACT[dtype], out.data_ptr())
@@ -785,7 +795,7 @@ def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
         _check(dy.cols >= 128 * groups, "the operands were not turned over with these offsets")
     _prepare(dy.data, dy.scales, x.data, x.scales, offsets)
     shape = (n, k) if offsets is None else (groups, n, k)
-    out = torch.empty(shape, dtype=dtype, device=dy.data.device)
+    out = torch.empty(*shape, dtype=dtype, device=dy.data.device)
     L.call("chelis_cuda_matmul8_wgrad", _FORMAT[dy.data.dtype], _FORMAT[x.data.dtype], n, k, dy.cols,
            dy.data.data_ptr(), dy.scales.data_ptr(), x.data.data_ptr(), x.scales.data_ptr(),
            _ptr(offsets), max(groups, 1), int(any_scales), _ACT[dtype], out.data_ptr())
