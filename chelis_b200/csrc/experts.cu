@@ -211,10 +211,13 @@ __global__ void route_bwd_kernel(const T *__restrict__ logits, const int32_t *__
 // A stable counting sort of the n = tokens * k pairs.  sort_count_kernel
 // counts each segment's pairs by expert; sort_place_kernel adds up the
 // segments before its own, ranks its pairs in order and writes the places.
-// One segment (n <= SEGMENT) needs the second kernel alone.
+// One segment (n <= SEGMENT) needs the second kernel alone.  Latency bounds
+// both.  Segments of 512 / 1024 / 2048 pairs, us: 16384 x 2 by 8 experts 9.1 /
+// 7.5 / 8.9, 16384 x 8 by 64 19.7 / 10.9 / 11.5 (a segment reads the counts of
+// all the others), 1024 x 8 by 64 6.3 / 7.1 / 9.8 (before the launches overlapped).
 constexpr int SORT_THREADS = 256;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
-constexpr int SEGMENT = 2048;
+constexpr int SEGMENT = 1024;
 constexpr int PER_WARP = SEGMENT / SORT_WARPS;  // consecutive pairs of a warp
 
 __device__ __forceinline__ int sort_id(const int32_t *ids, int64_t i, int64_t n, int experts) {
@@ -229,6 +232,7 @@ __global__ void __launch_bounds__(SORT_THREADS)
     sort_count_kernel(const int32_t *__restrict__ ids, int64_t n, int experts,
                       int32_t *__restrict__ counts) {
     __shared__ int hist[MAX_EXPERTS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int e = threadIdx.x; e < experts; e += SORT_THREADS) hist[e] = 0;
     __syncthreads();
     const int64_t first = static_cast<int64_t>(blockIdx.x) * SEGMENT;
@@ -262,7 +266,8 @@ __global__ void __launch_bounds__(SORT_THREADS)
         if (mine[c] >= 0) atomicAdd(&next[warp * experts + mine[c]], 1);
     }
     __syncthreads();
-    // before[w] = pairs of earlier segments and earlier warps
+    // before[w] = pairs of earlier segments and earlier warps, once those are counted
+    if (segments > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int e = threadIdx.x; e < experts; e += SORT_THREADS) {
         int before = 0, all = 0;
         for (int s = 0; s < segments && segments > 1; ++s) {
@@ -626,10 +631,23 @@ extern "C" int chelis_cuda_expert_sort(const int32_t *ids, int64_t tokens, int32
         g_launches++;
     }
     const size_t smem = sizeof(int) * (experts::SORT_WARPS + 1) * n_experts;
-    experts::sort_place_kernel<<<segments, experts::SORT_THREADS, smem, s>>>(
-        ids, n, n_experts, static_cast<const int32_t *>(counts), offsets, position, source);
+    // the second kernel counts its own pairs while the first one finishes
+    // (16384 x 2 by 8 6.8 us against 7.6; with more segments its waiting blocks
+    // are in the way, 16384 x 8 by 64 12.4 against 11.0)
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(segments);
+    cfg.blockDim = dim3(experts::SORT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = segments > 1 && segments <= 64 ? 1 : 0;
+    const int rc = check_cuda(cudaLaunchKernelEx(&cfg, experts::sort_place_kernel, ids, n, static_cast<int>(n_experts),
+                                                 static_cast<const int32_t *>(counts), offsets, position, source),
+                              "experts::sort_place_kernel");
     g_launches++;
-    const int rc = check_cuda(cudaGetLastError(), "experts::sort_place_kernel");
     scratch_free(counts, s);
     return rc;
 }

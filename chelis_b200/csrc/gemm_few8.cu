@@ -53,8 +53,13 @@ __device__ __forceinline__ uint4 load16(const uint8_t *p, bool ok) {
 }
 
 // NT: tokens of one pass over the weights, in eights.
+// Three blocks a multiprocessor with two blocks of K in flight a warp: 10.4 us
+// for 16 rows by 8 matrices of 4096 x 1024 out of memory (3.2 TB/s), against
+// 11.5 us for two with four.  What is left is latency (a strip's loads start
+// once its expert's rows are known) and the 8-bit MMA itself, which this
+// machine runs by converting its operands to 16 bits (ALU 36 % busy).
 template <bool E5A, bool E5B, int NT>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 1)
     few8_kernel(const Params p, const uint8_t *__restrict__ a, const uint8_t *__restrict__ w, int64_t ld,
                 int share) {
     __shared__ float part[WARPS * NT * COLS * STRIP];
@@ -101,7 +106,7 @@ __global__ void __launch_bounds__(WARPS * 32)
             for (int i = 0; i < 4; ++i) run[j][i] = 0.0f;
         }
         if (live) {
-#pragma unroll 4
+#pragma unroll 2
             for (int kb = turn; kb < p.kblocks; kb += share) {
                 const int64_t k = static_cast<int64_t>(kb) * 128 + t * 16;
                 const bool ok0 = k < ld, ok1 = k + 64 < ld;
@@ -162,7 +167,10 @@ void launch(const uint8_t *a, const uint8_t *w, const Params &p, int64_t ld, boo
 }
 
 int run(const uint8_t *a, const uint8_t *w, const Params &p, int64_t ld, int32_t fa, int32_t fb) {
-    int share = p.kblocks >= 32 ? 8 : 4;
+    // measured with 2048 strips 4 against 8 warps a strip 10.4 and 12.1 us, with
+    // 256 strips of 64 rows 10.9 and 9.0, of one row and K = 4096 10.1 and 7.4
+    const int64_t strips = (p.n + STRIP - 1) / STRIP * p.groups;
+    int share = strips <= 512 ? 8 : 4;
     while (share > p.kblocks) share /= 2;
     const int64_t per = WARPS / share * STRIP;
     const dim3 grid(static_cast<unsigned>((p.n + per - 1) / per),

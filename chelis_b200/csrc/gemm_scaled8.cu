@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(PACK_THREADS)
                        uint4 *__restrict__ sfb) {
     __shared__ int32_t start[MAX_GROUPS + 1], quad_start[MAX_GROUPS + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
         group_starts<WG ? BK : TM>(p, WG ? p.group_rows : p.rows, lane, start, WG ? p.kblocks : -1);
         __syncwarp();
@@ -387,6 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             int stage = 0;
             uint32_t phase = 1;
             bool ok = true;
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // the packed scales are written
             for (int L = static_cast<int>(worker); ok && L < all_tiles; L += static_cast<int>(workers)) {
                 const Tile t = tile_at<WG, TM>(p, start, L);
                 const int group = uniform(t.group), kbs = uniform(t.kbs), kb0 = uniform(t.kb0);
@@ -675,12 +677,16 @@ int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_
         cfg.blockDim = dim3(THREADS);
         cfg.dynamicSmemBytes = Shape<PAIR>::SMEM;
         cfg.stream = s;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = PAIR ? 2 : 1;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        // the set-up of the product's blocks overlaps the packing of the scales,
+        // which only its producer waits for
+        cudaLaunchAttribute attr[2]{};
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
         CHELIS_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kernel, ma, mb, msa, msb, mo, q), "scaled8::scaled8_kernel"));
         g_launches++;
         return CHELIS_CUDA_OK;
@@ -742,9 +748,9 @@ extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans
     p.out = out;
     p.out_dtype = out_dtype;
     // Few rows for each matrix (measured at 1024 x 4096 weights, rotated through
-    // memory; few8 against gemm8, us): one matrix, 1 row 3.6 and 10.1, 64 rows
-    // 8.9 and 10.7, 128 rows 15 and 11; 64 matrices, 8 rows 7.8 and 11; 8
-    // matrices, 16 rows 11.0 and 11.6, 64 rows 18 and 13; 32 of 4096 x 1024, 64
+    // memory; few8 against gemm8, us): one matrix, 1 row 3.1 and 10.1, 64 rows
+    // 9.0 and 10.7, 128 rows 15 and 11; 64 matrices, 8 rows 7.4 and 11; 8
+    // matrices, 16 rows 10.4 and 11.6, 64 rows 18 and 13; 32 of 4096 x 1024, 64
     // rows 32 and 26.
     if (trans_b && (offsets ? rows <= 2 * static_cast<int64_t>(groups) && kblocks < 32 : rows <= 64))
         return few8::run(a, b, p, blocks8::round16(k), format_a, format_b);
