@@ -10,10 +10,13 @@
 // from the f32 scales in the order in which tcgen05.cp takes them: 512 bytes
 // for 128 rows of a quad, row r's word at 16 (r mod 32) + 4 (r / 32).
 //
-// Block and warp roles are gemm8_kernel's (384 threads, PAIR: two blocks on a
-// 256 x 256 tile), but warp 0 loads the packed scales with the operands, warp
-// 1 copies them to tensor memory ahead of a quad's MMAs, and the fold runs
-// once in CHUNK blocks.
+// A pair of thread blocks (cta_group::2) works on a 256 x 256 tile of the
+// result, each with its 128 rows of a and half of b's columns in shared memory
+// and its 128 rows of the sums in tensor memory: a block of 128 x 256 alone
+// loads half as much again (16384 x 4096 x 1024 91 us against 82, 8192^3 485
+// against 408).  Warp roles are gemm8_kernel's, but warp 0 loads the packed
+// scales with the operands, warp 1 of the first block copies them to tensor
+// memory ahead of a quad's MMAs, and the fold runs once in CHUNK blocks.
 //
 // CHUNK: the accumulator truncates where IEEE rounds, and its error grows with
 // the number of MMAs on it, so after 32 blocks (128 MMAs) it is added to f32
@@ -46,15 +49,12 @@ constexpr int OUT_BOX = 2048;             // 32 rows x 64 bytes on the way out
 constexpr int OUT_BUFS = 1;               // of them a warp
 constexpr int OUT_BYTES = FOLD_WARPS * OUT_BUFS * OUT_BOX;
 
-template <bool PAIR>
-struct Shape {
-    static constexpr int B_BOXES = PAIR ? 1 : 2;
-    static constexpr int STAGE = (1 + B_BOXES) * BOX_BYTES;
-    static constexpr int STAGES = PAIR ? 6 : 4;
-    // scales lie beside the stage of their quad's first block
-    static constexpr int SMEM = STAGES * (STAGE + SF_SLOT) + OUT_BYTES + 1024 /*align*/ +
-                                512 /*barriers*/ + 2 * (MAX_GROUPS + 1) * 4;
-};
+constexpr int TM = 2 * BM;                // rows of a pair's tile
+constexpr int PAIR_STAGE = 2 * BOX_BYTES;  // a block's rows of a, its columns of b
+constexpr int PAIR_STAGES = 6;
+// scales lie beside the stage of their quad's first block
+constexpr int PAIR_SMEM = PAIR_STAGES * (PAIR_STAGE + SF_SLOT) + OUT_BYTES + 1024 /*align*/ + 512 /*barriers*/ +
+                          2 * (MAX_GROUPS + 1) * 4;
 
 struct Params8 {
     Params p;
@@ -111,7 +111,7 @@ __device__ __forceinline__ int group_of(const int32_t *start, int groups, int v)
 // ([groups][quads][ceil(n/128)], or [quads][ceil(n/128)] for the weight
 // gradient, whose quads are counted through the groups).  Rows that a tile
 // does not have, and blocks past the last, get 1.
-template <bool WG, int TM>
+template <bool WG>
 __global__ void __launch_bounds__(PACK_THREADS)
     pack_scales_kernel(const Params p, int32_t quads, int32_t m_atoms, uint4 *__restrict__ sfa,
                        uint4 *__restrict__ sfb) {
@@ -190,33 +190,21 @@ __global__ void __launch_bounds__(PACK_THREADS)
 }
 
 // 512 bytes of scales to 4 columns of tensor memory (every lane quadrant).
-template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
     // 32 rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle
     const uint64_t d = static_cast<uint64_t>((smem >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
                        (static_cast<uint64_t>(1u) << 46);
-    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
 }
-template <bool PAIR>
 __device__ __forceinline__ void mma_scaled(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if (PAIR)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X "
-            "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X "
-            "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X "
+        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
 
 // ---- fold -----------------------------------------------------------------
@@ -310,19 +298,17 @@ __device__ __forceinline__ void store_tma(const Params &p, const CUtensorMap *ma
     }
 }
 
-template <bool BMN, bool WG, bool PAIR>
+template <bool BMN, bool WG>
 __global__ void __launch_bounds__(THREADS, 1)
     scaled8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfb,
                    const __grid_constant__ CUtensorMap map_out, const Params8 q) {
-    using S = Shape<PAIR>;
-    constexpr int TM = PAIR ? 2 * BM : BM;
-    constexpr int STAGES = S::STAGES;
+    constexpr int STAGES = PAIR_STAGES, STAGE = PAIR_STAGE;
     const Params &p = q.p;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    unsigned char *out_stage = smem + STAGES * S::STAGE, *sf_ring = out_stage + OUT_BYTES;
+    unsigned char *out_stage = smem + STAGES * STAGE, *sf_ring = out_stage + OUT_BYTES;
     uint64_t *full = reinterpret_cast<uint64_t *>(sf_ring + STAGES * SF_SLOT);
     uint64_t *empty = full + STAGES;
     uint64_t *acc_full = empty + STAGES;  // [2]
@@ -336,8 +322,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t tries = *static_cast<volatile uint32_t *>(&g_wait_tries);
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-    const int64_t worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const uint32_t rank = cluster_ctarank();
+    const int worker = static_cast<int>(blockIdx.x >> 1), workers = static_cast<int>(gridDim.x >> 1);
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
@@ -345,9 +331,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], PAIR ? 2 * FOLD_WARPS : FOLD_WARPS);
+            mbar_init(&acc_empty[b], 2 * FOLD_WARPS);
         }
-        mbar_init(shared_cols, PAIR ? FOLD_WARPS : FOLD_WARPS / 2);
+        mbar_init(shared_cols, FOLD_WARPS);  // half of each block's
         *abort_flag = 0;
         *consumed = 0;
         fence_mbarrier_init();
@@ -358,13 +344,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (q.tma_out) prefetch_tensormap(&map_out);
     }
     if (warp == 1) {
-        if (PAIR) {
-            tmem_alloc_pair(tmem_slot, TMEM_COLS);
-            tmem_relinquish_pair();
-        } else {
-            tmem_alloc(tmem_slot, TMEM_COLS);
-            tmem_relinquish();
-        }
+        tmem_alloc_pair(tmem_slot, TMEM_COLS);
+        tmem_relinquish_pair();
     }
     if (warp == 2) {
         group_starts<WG ? BK : TM>(p, WG ? p.group_rows : p.rows, lane, start, WG ? p.kblocks : -1);
@@ -372,8 +353,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (WG) quad_starts(p, lane, start, quad_start);
     }
     tc_fence_before();
-    if (PAIR) cluster_sync_all();
-    else __syncthreads();
+    cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int64_t nt = (p.n + BN - 1) / BN;
@@ -389,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t phase = 1;
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");  // the packed scales are written
-            for (int L = static_cast<int>(worker); ok && L < all_tiles; L += static_cast<int>(workers)) {
+            for (int L = worker; ok && L < all_tiles; L += workers) {
                 const Tile t = tile_at<WG, TM>(p, start, L);
                 const int group = uniform(t.group), kbs = uniform(t.kbs), kb0 = uniform(t.kb0);
                 const int32_t m0 = uniform(static_cast<int32_t>(t.m0)) + static_cast<int32_t>(rank) * BM;
@@ -402,36 +382,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int i = 0; i < kbs; ++i) {
                     ok = all(wait(&empty[stage], phase, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER));
                     if (!ok) break;
-                    unsigned char *st = smem + stage * S::STAGE, *sf = sf_ring + stage * SF_SLOT;
+                    unsigned char *st = smem + stage * STAGE, *sf = sf_ring + stage * SF_SLOT;
                     uint64_t *bar = &full[stage];
                     const bool quad = i % QUAD == 0;
-                    const uint32_t bytes = S::STAGE + (quad ? SF_SLOT : 0);
+                    const uint32_t bytes = STAGE + (quad ? SF_SLOT : 0);
                     if (elect_one()) {
-                        if (PAIR) {
-                            const uint32_t bar0 = mapa_shared(smem_u32(bar), 0);
-                            if (rank == 0) mbar_arrive_expect_tx(bar, 2 * bytes);
-                            tma_load_2d_pair(st, &map_a, bar0, k0, m0);
-                            if (WG) tma_load_2d_pair(st + BOX_BYTES, &map_b, bar0, k0, n0);
-                            else if (BMN) tma_load_3d_pair(st + BOX_BYTES, &map_b, bar0, n0, k0, group);
-                            else tma_load_3d_pair(st + BOX_BYTES, &map_b, bar0, k0, n0, group);
-                            if (quad) {
-                                tma_load_2d_pair(sf, &map_sfa, bar0, 0, sfa);
-                                tma_load_2d_pair(sf + SF_BYTES, &map_sfb, bar0, 0, sfb);
-                            }
-                        } else {
-                            mbar_arrive_expect_tx(bar, bytes);
-                            tma_load_2d(st, &map_a, bar, k0, m0);
-#pragma unroll
-                            for (int h = 0; h < S::B_BOXES; ++h) {
-                                unsigned char *dst = st + (1 + h) * BOX_BYTES;
-                                if (WG) tma_load_2d(dst, &map_b, bar, k0, n0 + h * 128);
-                                else if (BMN) tma_load_3d(dst, &map_b, bar, n0 + h * 128, k0, group);
-                                else tma_load_3d(dst, &map_b, bar, k0, n0 + h * 128, group);
-                            }
-                            if (quad) {
-                                tma_load_2d(sf, &map_sfa, bar, 0, sfa);
-                                tma_load_2d(sf + SF_BYTES, &map_sfb, bar, 0, sfb);
-                            }
+                        const uint32_t bar0 = mapa_shared(smem_u32(bar), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(bar, 2 * bytes);
+                        tma_load_2d_pair(st, &map_a, bar0, k0, m0);
+                        if (WG) tma_load_2d_pair(st + BOX_BYTES, &map_b, bar0, k0, n0);
+                        else if (BMN) tma_load_3d_pair(st + BOX_BYTES, &map_b, bar0, n0, k0, group);
+                        else tma_load_3d_pair(st + BOX_BYTES, &map_b, bar0, k0, n0, group);
+                        if (quad) {
+                            tma_load_2d_pair(sf, &map_sfa, bar0, 0, sfa);
+                            tma_load_2d_pair(sf + SF_BYTES, &map_sfb, bar0, 0, sfb);
                         }
                     }
                     ++issued;
@@ -453,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             int stage = 0, slot = 0;
             uint32_t phase = 0;
             bool ok = true, ready = false;
-            for (int L = static_cast<int>(worker); ok && L < all_tiles; L += static_cast<int>(workers)) {
+            for (int L = worker; ok && L < all_tiles; L += workers) {
                 const int kbs = WG ? uniform(tile_at<WG, TM>(p, start, L).kbs) : p.kblocks;
                 uint32_t d = 0;
                 int cur = 0;
@@ -465,11 +429,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                         // this accumulator's last chunk but one has been read,
                         // and of the other's the columns they share
                         if (chunk >= 2)
-                            ok = all(wait<PAIR>(&acc_empty[cur], ((chunk >> 1) - 1) & 1, tries, abort_flag,
+                            ok = all(wait<true>(&acc_empty[cur], ((chunk >> 1) - 1) & 1, tries, abort_flag,
                                                 DEVERR_TIMEOUT_MMA));
                         if (!ok) break;
                         if (chunk >= 1)
-                            ok = all(wait<PAIR>(shared_cols, (chunk - 1) & 1, tries, abort_flag,
+                            ok = all(wait<true>(shared_cols, (chunk - 1) & 1, tries, abort_flag,
                                                 DEVERR_TIMEOUT_MMA));
                         if (!ok) break;
                     }
@@ -481,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int next = stage + 1 == STAGES ? 0 : stage + 1;
                     const uint32_t next_phase = next ? phase : phase ^ 1;
                     const bool peek = probe(&full[next], next_phase);
-                    const uint32_t a = smem_u32(smem) + stage * S::STAGE, b = a + BOX_BYTES;
+                    const uint32_t a = smem_u32(smem) + stage * STAGE, b = a + BOX_BYTES;
                     if (i % QUAD == 0) slot ^= 1;
                     const uint32_t sf = smem_u32(sf_ring) + stage * SF_SLOT;
                     const uint32_t sfa = tb + SF_COL + slot * 12, sfb = sfa + 4;
@@ -491,21 +455,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const bool end = i % CHUNK == CHUNK - 1 || i == kbs - 1;
                     if (elect_one()) {
                         if (i % QUAD == 0) {
-                            copy_scales<PAIR>(sfa, sf);
-                            copy_scales<PAIR>(sfb, sf + SF_BYTES);
-                            copy_scales<PAIR>(sfb + 4, sf + 2 * SF_BYTES);
+                            copy_scales(sfa, sf);
+                            copy_scales(sfb, sf + SF_BYTES);
+                            copy_scales(sfb + 4, sf + 2 * SF_BYTES);
                         }
 #pragma unroll
                         for (int kk = 0; kk < BK / 32; ++kk)
-                            mma_scaled<PAIR>(d, sw128_kmajor_desc(a + kk * 32),
+                            mma_scaled(d, sw128_kmajor_desc(a + kk * 32),
                                              BMN ? mnmajor_desc(b + kk * 32 * 128) : sw128_kmajor_desc(b + kk * 32),
                                              idesc, sfa, sfb, !(first && kk == 0));
-                        if (PAIR) mma_commit_pair(&empty[stage], 0x3);
-                        else mma_commit(&empty[stage]);
-                        if (end) {
-                            if (PAIR) mma_commit_pair(&acc_full[cur], 0x3);
-                            else mma_commit(&acc_full[cur]);
-                        }
+                        mma_commit_pair(&empty[stage], 0x3);
+                        if (end) mma_commit_pair(&acc_full[cur], 0x3);
                     }
                     __syncwarp();
                     if (end) ++chunk;
@@ -524,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         unsigned char *stage = out_stage + (warp - 4) * (OUT_BUFS * OUT_BOX);
         int32_t chunk = 0;
         bool ok = true;
-        for (int64_t L = worker; ok && L < tiles; L += workers) {
+        for (int L = worker; ok && L < all_tiles; L += workers) {
             const Tile t = tile_at<WG, TM>(p, start, L);
             const int64_t row0 = t.m0 + rank * BM + quad * 32, col0 = t.n0 + half * 128;
             const bool live = row0 < t.m_end && col0 < p.n;  // else nothing to read or store
@@ -541,10 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 auto arrive = [&](uint64_t *bar) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (PAIR) arrive_relaxed(mapa_shared(smem_u32(bar), 0));
-                        else mbar_arrive(bar);
-                    }
+                    if (lane == 0) arrive_relaxed(mapa_shared(smem_u32(bar), 0));
                 };
                 // accumulator 0 shares its last 32 columns, 1 its first
                 auto none = [] {};
@@ -583,14 +540,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             while (globaltimer_ns() - t0 < DRAIN_NS) __nanosleep(1000);
         }
     }
-    if (PAIR) {
-        tc_fence_before();
-        cluster_sync_all();
-    }
+    // neither block leaves while the other may use its memory
+    tc_fence_before();
+    cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
-        else tmem_dealloc(tmem_base, TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
 }
 
@@ -627,23 +582,22 @@ int make_out_map(CUtensorMap *map, void *base, int32_t dtype, int64_t n, int64_t
     return CHELIS_CUDA_OK;
 }
 
-uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn, bool pair) {
+uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn) {
     return (format_a == CHELIS_FORMAT_E5M2 ? 1u << 7 : 0u) |  // 0 e4m3, 1 e5m2
            (format_b == CHELIS_FORMAT_E5M2 ? 1u << 10 : 0u) |
            (bmn ? 1u << 16 : 0u) |                             // b MN-major
            (static_cast<uint32_t>(BN >> 3) << 17) | (1u << 23) |  // scales are exponents
-           (static_cast<uint32_t>((pair ? 2 * BM : BM) >> 7) << 27);
+           (static_cast<uint32_t>(TM >> 7) << 27);
 }
 
-template <bool BMN, bool WG, bool PAIR>
-int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
-    constexpr int TM = PAIR ? 2 * BM : BM;
+template <bool BMN, bool WG>
+int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
     cudaStream_t s = current_stream();
     const int64_t nt = (p.n + BN - 1) / BN, nb = (p.n + 127) / 128;
     const int64_t mt = WG ? (p.rows + TM - 1) / TM : row_tiles(p.rows, p.groups, p.offsets != nullptr, TM);
     Params8 q{};
     q.p = p;
-    q.p.idesc = instruction(fa, fb, BMN, PAIR);
+    q.p.idesc = instruction(fa, fb, BMN);
     q.m_atoms = static_cast<int32_t>(mt * (TM / 128));
     // by expert, each group's last quad may be a short one
     q.quads = (p.kblocks + QUAD - 1) / QUAD + (WG && p.offsets ? p.groups : 0);
@@ -662,26 +616,26 @@ int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_
         CHELIS_TRY(make_scale_map(&msb, sfb, b_atoms, 2));
         q.tma_out = p.n * experts::width(p.out_dtype) % 16 == 0 && experts::aligned16(p.out);
         if (q.tma_out) CHELIS_TRY(make_out_map(&mo, p.out, p.out_dtype, p.n, p.rows, WG ? p.groups : 1));
-        pack_scales_kernel<WG, TM><<<blocks8::grid_for((a_atoms + b_atoms + 15) / 16, 8), PACK_THREADS, 0, s>>>(
+        pack_scales_kernel<WG><<<blocks8::grid_for((a_atoms + b_atoms + 15) / 16, 8), PACK_THREADS, 0, s>>>(
             q.p, q.quads, q.m_atoms, static_cast<uint4 *>(scratch), reinterpret_cast<uint4 *>(sfb));
         g_launches++;
         CHELIS_LAUNCH_CHECK("scaled8::pack_scales_kernel");
-        auto kernel = scaled8_kernel<BMN, WG, PAIR>;
+        auto kernel = scaled8_kernel<BMN, WG>;
         CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   Shape<PAIR>::SMEM), "cudaFuncSetAttribute"));
+                                                   PAIR_SMEM), "cudaFuncSetAttribute"));
         const int64_t most = (WG ? p.groups : 1) * mt * nt;
-        const int64_t workers = PAIR ? sm_count() / 2 : sm_count();
+        const int64_t workers = sm_count() / 2;
         const int64_t used = most < workers ? (most < 1 ? 1 : most) : workers;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * used : used));
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * used));
         cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = Shape<PAIR>::SMEM;
+        cfg.dynamicSmemBytes = PAIR_SMEM;
         cfg.stream = s;
         // the set-up of the product's blocks overlaps the packing of the scales,
         // which only its producer waits for
         cudaLaunchAttribute attr[2]{};
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+        attr[0].val.clusterDim.x = 2;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -696,11 +650,6 @@ int launch(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_
     return rc;
 }
 
-template <bool BMN, bool WG>
-int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb, bool pair) {
-    return pair ? launch<BMN, WG, true>(ma, mb, p, fa, fb) : launch<BMN, WG, false>(ma, mb, p, fa, fb);
-}
-
 }  // namespace scaled8
 }  // namespace chelis
 
@@ -709,16 +658,10 @@ using namespace chelis;
 namespace {
 // Too little work (blocks of 128 x 256 x 128) for the launch that packs the
 // scales: gemm8 then takes powers of two as well.  Measured, gemm8 against
-// scaled8, us: 4096 x 1024 x 1024 (7 blocks a multiprocessor) 14.5 and 19.5,
-// 1024 x 4096 x 1024 by 8 experts (14) 24.2 and 23.1, 2048 (20) 34.6 and 27.5.
+// scaled8, us (blocks a multiprocessor): 4096 x 1024 x 1024 (7) 14.5 and 19.5,
+// 1024 x 4096 x 1024 by 8 experts (14) 23 and 25, 2048 (20) 33 and 28, 16384 x
+// 1024 x 1024 by 64 (41) 55 and 48.
 bool small(int64_t blocks) { return blocks < 12 * static_cast<int64_t>(sm_count()); }
-// Block pairs for a long contraction and tall matrices, where they halve the
-// loads of b; single blocks otherwise, whose tiles are finer and whose stages
-// hold more.  Measured, pairs against single, us: 32768 x 1024 x 4096 by 8
-// experts 129 and 140, 8192 by 4 46 and 44, 16384 x 4096 x 1024 91 and 86; the
-// weight gradient 4096 x 1024 from 32768 rows of 8 experts 135 and 151, 1024 x
-// 4096 from 16384 rows 71 and 82.
-bool pairs(int64_t kblocks, int64_t rows, int64_t groups) { return kblocks >= 32 && rows >= 2048 * groups; }
 }  // namespace
 
 extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows,
@@ -762,9 +705,8 @@ extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans
     if (any_scales || small(tiles * kblocks))
         return trans_b ? gemm8::run<false, false>(ma, mb, p, format_a, format_b)
                        : gemm8::run<true, false>(ma, mb, p, format_a, format_b);
-    const bool pair = pairs(kblocks, rows, groups);
-    return trans_b ? scaled8::run<false, false>(ma, mb, p, format_a, format_b, pair)
-                   : scaled8::run<true, false>(ma, mb, p, format_a, format_b, pair);
+    return trans_b ? scaled8::run<false, false>(ma, mb, p, format_a, format_b)
+                   : scaled8::run<true, false>(ma, mb, p, format_a, format_b);
 }
 
 extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int64_t k,
@@ -798,5 +740,5 @@ extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int
     const int64_t each = (p.kblocks + groups - 1) / groups;  // blocks of a group, about
     if (any_scales || small(groups * ((n + 127) / 128) * ((k + 255) / 256) * each))
         return gemm8::run<false, true>(ma, mb, p, format_a, format_b);
-    return scaled8::run<false, true>(ma, mb, p, format_a, format_b, n > 128 && pairs(each, 2048, 1));
+    return scaled8::run<false, true>(ma, mb, p, format_a, format_b);
 }
