@@ -95,32 +95,27 @@ __global__ void route_kernel(const T *__restrict__ logits, int64_t tokens, int e
         key[v] = order_key(l[v]);
     }
     nan = __any_sync(0xffffffffu, nan);
-    float mine = -INFINITY, top = -INFINITY;  // lane j: the logit chosen in round j
-    int id = -1;
+    int id = -1;  // lane j: the expert chosen in round j
     for (int j = 0; j < k; ++j) {
         uint32_t best = 0;
         int at = 0;
-        float val = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
             if (key[v] > best) {
                 best = key[v];
                 at = v * 32 + lane;
-                val = l[v];
             }
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
         if (most == 0) break;  // nothing left to choose
         const int which = __reduce_min_sync(0xffffffffu, best == most ? at : INT_MAX);
-        const float chosen = __shfl_sync(0xffffffffu, val, which & 31);
-        if (j == 0) top = chosen;
-        if (lane == j) {
-            id = which;
-            mine = chosen;
-        }
+        if (lane == j) id = which;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
             if (which == v * 32 + lane) key[v] = 0;
     }
+    // the chosen logits, read again (from L1) rather than carried through the rounds
+    const float mine = id >= 0 ? to_f32(logits[t * experts + id]) : -INFINITY;
+    const float top = __shfl_sync(0xffffffffu, mine, 0);
     const float e = id >= 0 ? expf(mine - top) : 0.0f;
     float z = e;
     if (!renormalize) {
@@ -212,9 +207,10 @@ __global__ void route_bwd_kernel(const T *__restrict__ logits, const int32_t *__
 // counts each segment's pairs by expert; sort_place_kernel adds up the
 // segments before its own, ranks its pairs in order and writes the places.
 // One segment (n <= SEGMENT) needs the second kernel alone.  Latency bounds
-// both.  Segments of 512 / 1024 / 2048 pairs, us: 16384 x 2 by 8 experts 9.1 /
-// 7.5 / 8.9, 16384 x 8 by 64 19.7 / 10.9 / 11.5 (a segment reads the counts of
-// all the others), 1024 x 8 by 64 6.3 / 7.1 / 9.8 (before the launches overlapped).
+// both: 16384 x 2 pairs by 8 experts 5.2 us, 16384 x 8 by 64 8.7 us, by 1024
+// 33 us, 8 x 2 2.8 us.  Shorter segments read too many others' counts, longer
+// ones leave the machine idle (512 / 1024 / 2048 pairs, before the counts were
+// shared out among the threads: 9.1 / 7.5 / 8.9 us for the first of these).
 constexpr int SORT_THREADS = 256;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SEGMENT = 1024;
@@ -255,7 +251,8 @@ __global__ void __launch_bounds__(SORT_THREADS)
     __shared__ int routed, warp_part[SORT_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int segments = gridDim.x, seg = blockIdx.x;
-    for (int i = threadIdx.x; i < SORT_WARPS * experts; i += SORT_THREADS) next[i] = 0;
+    int *earlier = total + experts;             // [experts]: pairs of earlier segments
+    for (int i = threadIdx.x; i < (SORT_WARPS + 2) * experts; i += SORT_THREADS) next[i] = 0;
     __syncthreads();
     // pairs of each warp by expert
     const int64_t first = static_cast<int64_t>(seg) * SEGMENT + warp * PER_WARP;
@@ -268,20 +265,32 @@ __global__ void __launch_bounds__(SORT_THREADS)
     __syncthreads();
     // before[w] = pairs of earlier segments and earlier warps, once those are counted
     if (segments > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int e = threadIdx.x; e < experts; e += SORT_THREADS) {
-        int before = 0, all = 0;
-        for (int s = 0; s < segments && segments > 1; ++s) {
-            const int c = counts[static_cast<int64_t>(s) * experts + e];
-            if (s < seg) before += c;
-            all += c;
+    if (segments > 1) {
+        // `shares` threads add up an expert's segments, every shares-th each
+        const int shares = experts < SORT_THREADS ? SORT_THREADS / experts : 1;
+        for (int i = threadIdx.x; i < shares * experts; i += SORT_THREADS) {
+            const int e = i % experts;
+            int before = 0, all = 0;
+#pragma unroll 8
+            for (int s = i / experts; s < segments; s += shares) {
+                const int c = counts[static_cast<int64_t>(s) * experts + e];
+                if (s < seg) before += c;
+                all += c;
+            }
+            atomicAdd(&total[e], all);
+            atomicAdd(&earlier[e], before);
         }
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < experts; e += SORT_THREADS) {
+        int before = earlier[e];
 #pragma unroll
         for (int w = 0; w < SORT_WARPS; ++w) {
             const int c = next[w * experts + e];
             next[w * experts + e] = before;
             before += c;
         }
-        total[e] = segments > 1 ? all : before;
+        if (segments == 1) total[e] = before;
     }
     __syncthreads();
     // exclusive scan over experts: SORT_THREADS chunks of consecutive experts
@@ -630,7 +639,7 @@ extern "C" int chelis_cuda_expert_sort(const int32_t *ids, int64_t tokens, int32
             ids, n, n_experts, static_cast<int32_t *>(counts));
         g_launches++;
     }
-    const size_t smem = sizeof(int) * (experts::SORT_WARPS + 1) * n_experts;
+    const size_t smem = sizeof(int) * (experts::SORT_WARPS + 2) * n_experts;
     // the second kernel counts its own pairs while the first one finishes
     // (16384 x 2 by 8 6.8 us against 7.6; with more segments its waiting blocks
     // are in the way, 16384 x 8 by 64 12.4 against 11.0)

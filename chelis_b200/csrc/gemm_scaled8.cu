@@ -66,16 +66,10 @@ struct Params8 {
 };
 
 // ---- scales ---------------------------------------------------------------
-// The exponent byte of a power of two; NaN (0xff) and an error report for
-// anything else.
-__device__ __forceinline__ uint32_t exponent_byte(float s) {
-    const uint32_t b = __float_as_uint(s);
-    const uint32_t e = b >> 23;
-    if ((b & 0x7fffffu) != 0 || e == 0 || e >= 255) {
-        report_device_error(DEVERR_SCALE);
-        return 0xffu;
-    }
-    return e;
+// The exponent byte of a power of two, NaN (0xff) for anything else.
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t bits) {
+    const uint32_t e = bits >> 23;
+    return (bits & 0x7fffffu) != 0 || e == 0 || e >= 255 ? 0xffu : e;
 }
 
 constexpr int PACK_THREADS = 256;
@@ -110,7 +104,8 @@ __device__ __forceinline__ int group_of(const int32_t *start, int groups, int v)
 // l, l + 32, l + 64, l + 96.  a's atoms first ([quads][m_atoms]), then b's
 // ([groups][quads][ceil(n/128)], or [quads][ceil(n/128)] for the weight
 // gradient, whose quads are counted through the groups).  Rows that a tile
-// does not have, and blocks past the last, get 1.
+// does not have, and blocks past the last, get 1.  Latency bounds it (a few
+// hundred KB): one atom a warp, its sixteen loads in flight together.
 template <bool WG>
 __global__ void __launch_bounds__(PACK_THREADS)
     pack_scales_kernel(const Params p, int32_t quads, int32_t m_atoms, uint4 *__restrict__ sfa,
@@ -171,20 +166,30 @@ __global__ void __launch_bounds__(PACK_THREADS)
                 kb_step = p.sb_k;
             }
         }
+        // all loads first: a report between them would make each wait for the last
+        constexpr uint32_t ONE = 127u << 23;
+        uint32_t bits[4][QUAD];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < QUAD; ++j) {
+                const bool in = j < kbs && (row_step ? u * 32 + lane < rows : u == 0);
+                bits[u][j] = in ? __float_as_uint(src[(u * 32 + lane) * row_step + j * kb_step]) : ONE;
+            }
         uint32_t r[4];
+        bool bad = false;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            r[u] = 0x7f7f7f7fu;
-            if (u * 32 + lane < rows && (u == 0 || row_step)) {
-                uint32_t v = 0;
+            r[u] = 0;
 #pragma unroll
-                for (int j = 0; j < QUAD; ++j)
-                    v |= (j < kbs ? exponent_byte(src[(u * 32 + lane) * row_step + j * kb_step]) : 127u) << (8 * j);
-                r[u] = v;
-            } else if (!row_step) {
-                r[u] = r[0];
+            for (int j = 0; j < QUAD; ++j) {
+                const uint32_t e = exponent_byte(bits[u][j]);
+                bad |= e == 0xffu;
+                r[u] |= e << (8 * j);
             }
         }
+        if (!row_step) r[1] = r[2] = r[3] = r[0];
+        if (bad) report_device_error(DEVERR_SCALE);
         (is_a ? sfa : sfb)[i * 32 + lane] = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
@@ -616,7 +621,7 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t f
         CHELIS_TRY(make_scale_map(&msb, sfb, b_atoms, 2));
         q.tma_out = p.n * experts::width(p.out_dtype) % 16 == 0 && experts::aligned16(p.out);
         if (q.tma_out) CHELIS_TRY(make_out_map(&mo, p.out, p.out_dtype, p.n, p.rows, WG ? p.groups : 1));
-        pack_scales_kernel<WG><<<blocks8::grid_for((a_atoms + b_atoms + 15) / 16, 8), PACK_THREADS, 0, s>>>(
+        pack_scales_kernel<WG><<<blocks8::grid_for((a_atoms + b_atoms + 7) / 8, 8), PACK_THREADS, 0, s>>>(
             q.p, q.quads, q.m_atoms, static_cast<uint4 *>(scratch), reinterpret_cast<uint4 *>(sfb));
         g_launches++;
         CHELIS_LAUNCH_CHECK("scaled8::pack_scales_kernel");

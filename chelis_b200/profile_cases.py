@@ -16,6 +16,9 @@
                                                     # batched call (persistent CTA-pair kernel)
     python -m chelis_b200.profile_cases mlp         # config 1 step, called 4 times: a direct run,
                                                     # the capture, then two replays of its CUDA graph
+    python -m chelis_b200.profile_cases experts     # routed feed-forward: 8-bit quantisers of 16384 x
+                                                    # 4096 bf16, an 8-bit product 16384 x 1024 x 4096,
+                                                    # the way back of 8 rows a token of 1024 bf16
 
 Each case builds its inputs on the device, runs the hot path once and
 synchronises; inputs exceed the 126 MB L2 except where the case is smaller
@@ -70,6 +73,19 @@ def run(case: str) -> None:
         x, labels, w1, b1, w2, b2 = W.torch_mlp_inputs()
         for _ in range(4):  # outputs dropped at once: the next call reuses their memory
             ops.mlp_step(x, labels, w1, b1, w2, b2)
+    elif case == "experts":
+        g = torch.Generator(device="cuda").manual_seed(5)
+        x = torch.randn(16384, 4096, device="cuda", generator=g).to(torch.bfloat16)
+        w = torch.randn(1024, 4096, device="cuda", generator=g).to(torch.bfloat16)
+        x8, w8 = ops.quantize8(x), ops.quantize8(w, "e4m3", "tiles")
+        ops.quantize8_transposed(x)
+        ops.matmul8(x8, w8)
+        _, ids = ops.expert_route(torch.randn(16384, 64, device="cuda", generator=g), 8)
+        order = ops.expert_sort(ids, 64)
+        dy = x[:, :1024].contiguous()
+        ys, weights = ops.expert_gather(dy, order), torch.rand(16384, 8, device="cuda", generator=g)
+        ops.expert_combine(ys, weights, order)
+        ops.expert_combine_bwd(dy, ys, weights, order)
     else:
         raise SystemExit(f"unknown case {case!r}")
     torch.cuda.synchronize()
