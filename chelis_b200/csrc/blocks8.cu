@@ -150,12 +150,14 @@ __device__ __noinline__ void slow_block(const T *x, int64_t step, int n, uint8_t
 // Blocks of a row: LANES lanes hold one, 8 elements a lane at a time; a thread
 // block takes ROWS rows of RUN consecutive column blocks, whose loads are all
 // in flight before the first maximum is formed, and the rows' scales of a
-// block go out together.  f32 is bound by memory with 16 lanes; 16-bit types
-// were bound by the ALU's work around each maximum (71 % busy, 48 us for
-// 16384 x 4096) and take 8 lanes of 16 elements, which halves it.
-constexpr int RUN = 4;
+// block go out together.  f32 is bound by memory with 16 lanes and runs of 4
+// (16384 x 4096 in 50.5 us, 6.7 TB/s; runs of 2 54.5).  16-bit types were bound
+// by the ALU's work around each maximum (71 % busy, 48 us) and take 8 lanes of
+// 16 elements, which halves it, and runs of 2, which leave more blocks resident
+// (41 us, 4.9 TB/s; runs of 4 44 us); latency is what is left.
 template <typename T>
 struct RowShape {
+    static constexpr int RUN = sizeof(T) == 2 ? 2 : 4;
     static constexpr int LANES = sizeof(T) == 2 ? 8 : 16;
     static constexpr int EIGHTS = 16 / LANES;  // of a lane
     static constexpr int ROWS = THREADS / LANES;
@@ -166,6 +168,7 @@ __global__ void __launch_bounds__(THREADS)
     rows_kernel(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, int64_t kb,
                 uint8_t *__restrict__ q, float *__restrict__ scales) {
     constexpr int LANES = RowShape<T>::LANES, EIGHTS = RowShape<T>::EIGHTS, ROWS = RowShape<T>::ROWS;
+    constexpr int RUN = RowShape<T>::RUN;
     const int part = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const int64_t row_tiles = (rows + ROWS - 1) / ROWS, runs = (kb + RUN - 1) / RUN;
     for (int64_t w = blockIdx.x; w < row_tiles * runs; w += gridDim.x) {
@@ -246,7 +249,11 @@ __device__ __noinline__ void slow_tile(const T *x, int64_t rows, int64_t cols, i
     }
 }
 
-// A 128 x 128 tile a thread block: 8 rows a thread, 8 elements of each.
+// A 128 x 128 tile a thread block: 8 rows a thread, 8 elements of each, all
+// loaded before the block's maximum is formed.  Memory bounds f32 (16384 x 4096
+// in 52.7 us, 6.4 TB/s); a 16-bit tile is half the bytes behind the same two
+// barriers, and three resident blocks a multiprocessor do not hide them (53 us,
+// 3.8 TB/s; two 98 us, four spill: 69 us).
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 3 : 2)
     tiles_kernel(const T *__restrict__ x, int64_t batch, int64_t rows, int64_t cols, int64_t ld,
@@ -342,7 +349,9 @@ __device__ __forceinline__ void column_keys(const Eight<T, VEC> (&v)[8], uint32_
 
 // 128 rows x 128 columns a thread block, turned over in shared memory as
 // bytes.  A thread holds rows 8 sub .. 8 sub + 7 of 8 columns: its 8 bytes of
-// a column are consecutive places.
+// a column are consecutive places.  16384 x 4096: bf16 48 us (4.2 TB/s), f32 57
+// us (5.9 TB/s), bound by the barriers between load, maximum and store; before
+// the bytes were swizzled bank conflicts made it 64 and 71 us.
 template <typename T, bool E5M2, bool VEC>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 3 : 2)
     transposed_kernel(const T *__restrict__ x, const int32_t *__restrict__ offsets, int groups,
@@ -464,7 +473,7 @@ extern "C" int chelis_cuda_quantize8(int32_t dtype, int32_t format, int32_t layo
         if (layout == CHELIS_BLOCKS_ROWS)
             blocks8::rows_kernel<T, E5M2, VEC>
                 <<<blocks8::grid_for((rows + blocks8::RowShape<T>::ROWS - 1) / blocks8::RowShape<T>::ROWS *
-                                        ((kb + blocks8::RUN - 1) / blocks8::RUN), 32), blocks8::THREADS, 0, s>>>(
+                                        ((kb + blocks8::RowShape<T>::RUN - 1) / blocks8::RowShape<T>::RUN), 32), blocks8::THREADS, 0, s>>>(
                     static_cast<const T *>(x), rows, cols, ld, kb, data, scales);
         else
             blocks8::tiles_kernel<T, E5M2, VEC>

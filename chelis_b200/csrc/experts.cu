@@ -78,6 +78,8 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 // One warp a token, expert v * 32 + lane in the lane's value v: k rounds of a
 // warp maximum over the keys, then over the indices that hold it (the lowest
 // wins).  The softmax is taken against the first chosen logit, the largest.
+// 16384 x 64, k = 8 in 9.5 us: bound by the rounds' instructions (about 350 a
+// token, ALU 71 % busy), not by its 5 MB; 8 tokens take 2.8 us, a launch.
 template <typename T, int NV>
 __global__ void route_kernel(const T *__restrict__ logits, int64_t tokens, int experts, int k,
                              int renormalize, float *__restrict__ weights, int32_t *__restrict__ ids) {
@@ -134,7 +136,7 @@ __global__ void route_kernel(const T *__restrict__ logits, int64_t tokens, int e
 
 // dl_i = p_i (g_i - sum_j p_j g_j): over the chosen experts when the weights
 // were renormalised (p their softmax alone), over all of them otherwise (g_i
-// = 0 off the chosen).
+// = 0 off the chosen).  16384 x 64, k = 8 in 6.6 us, bound as route_kernel.
 template <typename T, int NV>
 __global__ void route_bwd_kernel(const T *__restrict__ logits, const int32_t *__restrict__ ids,
                                  const float *__restrict__ dweights, int64_t tokens, int experts,
@@ -350,7 +352,9 @@ __global__ void __launch_bounds__(SORT_THREADS)
 // ---- rows to their experts, and back --------------------------------------
 // xs[position[t, j]] = x[t]: one read of a token's row, k writes.  A warp
 // moves WIDE packs a lane of one row at a time.  Rows that no pair takes
-// (from *routed on) are written as zeros.
+// (from *routed on) are written as zeros.  Bound by memory: 16384 tokens of
+// 1024 f32 to two rows each in 32 us (6.3 TB/s), of 1024 bf16 to eight 54 us
+// (5.6 TB/s, eight writes to a read).
 constexpr int ROW_THREADS = 256;
 constexpr int WIDE = 4;
 
@@ -404,6 +408,10 @@ __global__ void __launch_bounds__(ROW_THREADS)
 // y[t] = sum_j w[t, j] ys[position[t, j]] in f32, slot order, rounded once.
 // Without weights it is the gradient of spread_kernel.  A warp takes DEEP
 // packs a lane of one token; its lanes hold the token's positions and weights.
+// Bound by memory: 16384 tokens of 1024 f32 from two rows each 35 us (5.8 TB/s;
+// one pack 37), of 1024 bf16 from eight 56 us (5.4 TB/s).  Loading four rows
+// before adding the first took 61 to 86 us: the registers cost more resident
+// warps than the loads in flight gained.
 constexpr int DEEP = 2;
 
 template <typename T, bool VEC>
@@ -459,7 +467,10 @@ __global__ void __launch_bounds__(ROW_THREADS)
 }
 
 // dys[position[t, j]] = w[t, j] dy[t] and dw[t, j] = <dy[t], ys[position[t, j]]>:
-// one block a token, the k dot products reduced by warp, then over warps.
+// one block a token, the k dot products reduced by warp, then over warps (a
+// fixed order).  dy stays in L1 over the slots.  Bound by memory: 16384 tokens
+// of 1024 bf16, k = 8, 95 us (6.0 TB/s); four rows at a time halved the
+// resident blocks and took 132 us.
 constexpr int BWD_THREADS = 128;
 
 template <typename T, bool VEC>

@@ -600,7 +600,8 @@ int chelis_cuda_dp_finalize(int32_t abort);
 /* =========================================================================
  * Routed (mixture-of-experts) feed-forward, new: the reference's DAG has no
  * routed layer and no 8-bit dtype.  T tokens, E experts (at most 1024), k
- * slots a token (at most 32); activations are f32, bf16 or f16.
+ * slots a token (at most 32); activations are f32, bf16 or f16.  Arguments of
+ * one call must not overlap.
  * ========================================================================= */
 /* The k experts of each token with the largest logits [T][E] (ties: the
  * lowest index first; an expert at -inf is never chosen) and their softmax
