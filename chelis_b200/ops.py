@@ -555,11 +555,6 @@ def _act(name: str, t: torch.Tensor) -> int:
     return _ACT[t.dtype]
 
 
-def _check(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def _check_i32(name: str, *tensors: torch.Tensor) -> None:
     for t in tensors:
         if t.dtype != torch.int32:
@@ -585,7 +580,8 @@ def expert_route(logits: torch.Tensor, k: int, renormalize: bool = True):
     the chosen alone.  Ties go to the lowest index; an expert at -inf is never
     chosen (id -1, weight 0 where fewer than k are left)."""
     dt = _act("expert_route", logits)
-    _check(logits.dim() == 2, "expert_route takes logits [tokens, experts]")
+    if logits.dim() != 2:
+        raise ValueError("expert_route takes logits [tokens, experts]")
     _prepare(logits)
     tokens, experts = logits.shape
     slots, dev = max(k, 0), logits.device
@@ -601,9 +597,9 @@ def expert_route_bwd(logits: torch.Tensor, experts: torch.Tensor, dweights: torc
     """dlogits of expert_route, given the experts that it chose."""
     dt = _act("expert_route_bwd", logits)
     _check_i32("expert_route_bwd", experts)
-    _check(logits.dim() == 2 and experts.dim() == 2 and experts.shape == dweights.shape
-           and experts.shape[0] == logits.shape[0] and dweights.dtype == torch.float32,
-           "expert_route_bwd takes logits [tokens, experts] and experts, f32 dweights [tokens, k]")
+    if not (logits.dim() == 2 and experts.dim() == 2 and experts.shape == dweights.shape
+            and experts.shape[0] == logits.shape[0] and dweights.dtype == torch.float32):
+        raise ValueError("expert_route_bwd takes logits [tokens, experts] and experts, f32 dweights [tokens, k]")
     _prepare(logits, experts, dweights)
     dlogits = torch.empty_like(logits)
     L.call("chelis_cuda_expert_route_bwd", dt, logits.data_ptr(), experts.data_ptr(),
@@ -617,7 +613,8 @@ def expert_sort(experts: torch.Tensor, n_experts: int) -> ExpertOrder:
     [tokens, k]; an id of -1 is a pair that goes nowhere.  Other ids outside
     [0, n_experts) count as -1 and raise at the next device_status()."""
     _check_i32("expert_sort", experts)
-    _check(experts.dim() == 2, "expert_sort takes experts [tokens, k]")
+    if experts.dim() != 2:
+        raise ValueError("expert_sort takes experts [tokens, k]")
     _prepare(experts)
     dev = experts.device
     order = ExpertOrder(torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev),
@@ -633,8 +630,8 @@ def expert_gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     hidden]; rows that no pair takes (the last ones) are zeros."""
     dt = _act("expert_gather", x)
     _check_order("expert_gather", order)
-    _check(x.dim() == 2 and x.shape[0] == order.position.shape[0],
-           "expert_gather takes x [tokens, hidden]")
+    if x.dim() != 2 or x.shape[0] != order.position.shape[0]:
+        raise ValueError("expert_gather takes x [tokens, hidden]")
     _prepare(x, *order)
     tokens, k = order.position.shape
     xs = torch.empty(tokens * k, x.shape[1], dtype=x.dtype, device=x.device)
@@ -647,9 +644,10 @@ def _expert_combine(name, ys, weights, order):
     dt = _act(name, ys)
     _check_order(name, order)
     tokens, k = order.position.shape
-    _check(ys.dim() == 2 and ys.shape[0] == tokens * k, f"{name} takes rows [tokens * k, hidden]")
-    _check(weights is None or (weights.dtype == torch.float32 and weights.shape == (tokens, k)),
-           f"{name} takes f32 weights [tokens, k]")
+    if ys.dim() != 2 or ys.shape[0] != tokens * k:
+        raise ValueError(f"{name} takes rows [tokens * k, hidden]")
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != (tokens, k)):
+        raise ValueError(f"{name} takes f32 weights [tokens, k]")
     _prepare(ys, weights, *order)
     y = torch.empty(tokens, ys.shape[1], dtype=ys.dtype, device=ys.device)
     L.call("chelis_cuda_expert_combine", dt, ys.data_ptr(), _ptr(weights), order.position.data_ptr(),
@@ -665,7 +663,8 @@ def expert_gather_bwd(dxs: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
 def expert_combine(ys: torch.Tensor, weights: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The way back: y[t] = sum_j weights[t, j] * ys[position[t, j]], f32 sums
     in slot order."""
-    _check(weights is not None, "expert_combine takes weights")
+    if weights is None:
+        raise ValueError("expert_combine takes weights")
     return _expert_combine("expert_combine", ys, weights, order)
 
 
@@ -674,11 +673,11 @@ def expert_combine_bwd(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor
     dt = _act("expert_combine_bwd", dy)
     _check_order("expert_combine_bwd", order)
     tokens, k = order.position.shape
-    _check(ys.dtype == dy.dtype and dy.dim() == 2 and dy.shape[0] == tokens
-           and ys.shape == (tokens * k, dy.shape[1]),
-           "expert_combine_bwd takes dy [tokens, hidden] and rows [tokens * k, hidden] of one dtype")
-    _check(weights.dtype == torch.float32 and weights.shape == (tokens, k),
-           "expert_combine_bwd takes f32 weights [tokens, k]")
+    if not (ys.dtype == dy.dtype and dy.dim() == 2 and dy.shape[0] == tokens
+            and ys.shape == (tokens * k, dy.shape[1])):
+        raise ValueError("expert_combine_bwd takes dy [tokens, hidden] and rows [tokens * k, hidden] of one dtype")
+    if weights.dtype != torch.float32 or weights.shape != (tokens, k):
+        raise ValueError("expert_combine_bwd takes f32 weights [tokens, k]")
     _prepare(dy, ys, weights, *order)
     dys = torch.empty_like(ys)
     dweights = torch.empty_like(weights)
@@ -697,10 +696,12 @@ def quantize8(x: torch.Tensor, format: str = "e4m3", blocks: str = "rows") -> Bl
     128: along its rows ("rows", x [rows, cols]; activations, gradients) or
     128 x 128 ("tiles", x [rows, cols] or [experts, rows, cols]; weights)."""
     dt = _act("quantize8", x)
-    _check(format in _FLOAT8, "8-bit formats are e4m3 and e5m2")
-    _check(blocks in ("rows", "tiles"), "blocks are rows or tiles")
-    _check(x.dim() == 2 or (x.dim() == 3 and blocks == "tiles"),
-           "quantize8 takes a matrix, or a stack of matrices in tiles")
+    if format not in _FLOAT8:
+        raise ValueError("8-bit formats are e4m3 and e5m2")
+    if blocks not in ("rows", "tiles"):
+        raise ValueError("blocks are rows or tiles")
+    if not (x.dim() == 2 or (x.dim() == 3 and blocks == "tiles")):
+        raise ValueError("quantize8 takes a matrix, or a stack of matrices in tiles")
     _prepare(x)
     rows, cols = x.shape[-2:]
     batch = x.shape[0] if x.dim() == 3 else 1
@@ -720,12 +721,15 @@ def quantize8_transposed(x: torch.Tensor, format: str = "e4m3",
     operand of matmul8_wgrad.  With offsets (expert_sort's) each expert's rows
     start on a block of their own."""
     dt = _act("quantize8_transposed", x)
-    _check(format in _FLOAT8, "8-bit formats are e4m3 and e5m2")
-    _check(x.dim() == 2, "quantize8_transposed takes a matrix")
+    if format not in _FLOAT8:
+        raise ValueError("8-bit formats are e4m3 and e5m2")
+    if x.dim() != 2:
+        raise ValueError("quantize8_transposed takes a matrix")
     groups = 0
     if offsets is not None:
         _check_i32("quantize8_transposed", offsets)
-        _check(offsets.dim() == 1 and offsets.numel() >= 2, "offsets are [experts + 1]")
+        if offsets.dim() != 1 or offsets.numel() < 2:
+            raise ValueError("offsets are [experts + 1]")
         groups = offsets.numel() - 1
     _prepare(x, offsets)
     rows, cols = x.shape
@@ -738,12 +742,18 @@ def quantize8_transposed(x: torch.Tensor, format: str = "e4m3",
 
 
 def _check_blocks8(name: str, b: Blocks8, blocks: str) -> None:
-    _check(b.blocks == blocks and b.data.dtype in _FORMAT and b.scales.dtype == torch.float32,
-           f"{name} takes 8-bit {blocks} with f32 scales here")
-    rows, kb = b.data.shape[-2], _ceil(b.cols, 128)
-    shape = (kb, rows) if blocks == "rows" else (*b.data.shape[:-2], _ceil(rows, 128), kb)
-    _check(b.data.shape[-1] == _ceil(b.cols, 16) * 16 and tuple(b.scales.shape) == shape,
-           f"{name}: data and scales do not belong together")
+    data, scales, cols, kind = b
+    if kind != blocks or data.dtype not in _FORMAT or scales.dtype != torch.float32:
+        raise ValueError(f"{name} takes 8-bit {blocks} with f32 scales here")
+    d, s = data.shape, scales.shape
+    if len(d) < 2 or len(s) != (len(d) if blocks == "tiles" else 2):
+        ok = False
+    elif blocks == "tiles":
+        ok = s[-1] == (cols + 127) // 128 and s[-2] == (d[-2] + 127) // 128 and s[:-2] == d[:-2]
+    else:
+        ok = s[0] == (cols + 127) // 128 and s[1] == d[-2]
+    if not ok or d[-1] != (cols + 15) // 16 * 16:
+        raise ValueError(f"{name}: data and scales do not belong together")
 
 
 def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor | None = None,
@@ -755,18 +765,21 @@ def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor 
     e; rows that no expert holds come out as zeros.  Scales are powers of two,
     as quantize8 makes them (others give NaN and raise at the next
     device_status()); any_scales admits every scale, at a lower rate."""
-    _check(dtype in _ACT, "matmul8 gives f32, bf16 or f16")
+    if dtype not in _ACT:
+        raise ValueError("matmul8 gives f32, bf16 or f16")
     _check_blocks8("matmul8", a, "rows")
     _check_blocks8("matmul8", b, "tiles")
-    _check(a.data.dim() == 2 and b.data.dim() == (2 if offsets is None else 3),
-           "matmul8 takes a matrix b, or a stack of them with offsets")
+    if a.data.dim() != 2 or b.data.dim() != (2 if offsets is None else 3):
+        raise ValueError("matmul8 takes a matrix b, or a stack of them with offsets")
     groups = 1
     if offsets is not None:
         _check_i32("matmul8", offsets)
         groups = b.data.shape[0]
-        _check(offsets.shape == (groups + 1,), "offsets are [experts + 1]")
+        if offsets.shape != (groups + 1,):
+            raise ValueError("offsets are [experts + 1]")
     n, k = (b.data.shape[-2], b.cols) if trans_b else (b.cols, b.data.shape[-2])
-    _check(a.cols == k, f"contraction extents differ: {a.cols} vs {k}")
+    if a.cols != k:
+        raise ValueError(f"contraction extents differ: {a.cols} vs {k}")
     _prepare(a.data, a.scales, b.data, b.scales, offsets)
     rows = a.data.shape[0]
     out = torch.empty(rows, n, dtype=dtype, device=a.data.device)
@@ -782,17 +795,21 @@ def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
     dy [rows, n] and x [rows, k] (quantize8_transposed); with offsets one
     matrix an expert, [experts, n, k], zeros for an expert without rows.
     any_scales as in matmul8."""
-    _check(dtype in _ACT, "matmul8_wgrad gives f32, bf16 or f16")
+    if dtype not in _ACT:
+        raise ValueError("matmul8_wgrad gives f32, bf16 or f16")
     _check_blocks8("matmul8_wgrad", dy, "rows")
     _check_blocks8("matmul8_wgrad", x, "rows")
-    _check(dy.cols == x.cols and dy.cols % 128 == 0, "matmul8_wgrad takes operands over the same rows")
+    if dy.cols != x.cols or dy.cols % 128:
+        raise ValueError("matmul8_wgrad takes operands over the same rows")
     n, k = dy.data.shape[0], x.data.shape[0]
     groups = 0
     if offsets is not None:
         _check_i32("matmul8_wgrad", offsets)
-        _check(offsets.dim() == 1 and offsets.numel() >= 2, "offsets are [experts + 1]")
+        if offsets.dim() != 1 or offsets.numel() < 2:
+            raise ValueError("offsets are [experts + 1]")
         groups = offsets.numel() - 1
-        _check(dy.cols >= 128 * groups, "the operands were not turned over with these offsets")
+        if dy.cols < 128 * groups:
+            raise ValueError("the operands were not turned over with these offsets")
     _prepare(dy.data, dy.scales, x.data, x.scales, offsets)
     shape = (n, k) if offsets is None else (groups, n, k)
     out = torch.empty(*shape, dtype=dtype, device=dy.data.device)
