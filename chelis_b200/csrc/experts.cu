@@ -208,9 +208,10 @@ __global__ void route_bwd_kernel(const T *__restrict__ logits, const int32_t *__
 // A stable counting sort of the n = tokens * k pairs.  sort_count_kernel
 // counts each segment's pairs by expert; sort_place_kernel adds up the
 // segments before its own, ranks its pairs in order and writes the places.
-// One segment (n <= SEGMENT) needs the second kernel alone.  Latency bounds
-// both: 16384 x 2 pairs by 8 experts 5.2 us, 16384 x 8 by 64 8.7 us, by 1024
-// 33 us, 8 x 2 2.8 us.  Shorter segments read too many others' counts, longer
+// One segment (n <= SEGMENT) needs that kernel alone; from SCAN_FROM counts on
+// sort_scan_kernel adds them up in between.  Latency bounds them: 8 x 2 pairs
+// by 8 experts 2.8 us, 16384 x 2 by 8 5.3 us, 16384 x 8 by 64 9.3 us, by 1024
+// 10.7 us; 131072 x 8 by 64 20 us.  Shorter segments read too many others' counts, longer
 // ones leave the machine idle (512 / 1024 / 2048 pairs, before the counts were
 // shared out among the threads: 9.1 / 7.5 / 8.9 us for the first of these).
 constexpr int SORT_THREADS = 256;
@@ -243,9 +244,75 @@ __global__ void __launch_bounds__(SORT_THREADS)
         counts[static_cast<int64_t>(blockIdx.x) * experts + e] = hist[e];
 }
 
+// For many segments or experts, where each segment adding up all the others'
+// counts is what costs (with the scan and without: 32 segments of 64 experts
+// 8.5 and 6.7 us, of 256 8.8 and 9.9; 128 of 64 9.3 and 11.0, of 1024 10.7 and
+// 78; 1024 of 64 20 and 72, of 1024 25 and 1050): counts[s][e] becomes the pairs of e in the segments before s, and
+// one more row, counts[segments], each expert's total.  A block has SCAN_WIDTH
+// experts (a 32-byte sector of a row), its threads consecutive shares of the
+// segments.
+constexpr int SCAN_THREADS = 1024;
+constexpr int SCAN_WIDTH = 8;
+constexpr int SCAN_SHARES = SCAN_THREADS / SCAN_WIDTH;
+constexpr int SCAN_DEEP = 8;  // counts in flight a thread
+constexpr int64_t SCAN_FROM = 8192;  // counts from which the scan pays for its launch
+
+__global__ void __launch_bounds__(SCAN_THREADS)
+    sort_scan_kernel(int32_t *__restrict__ counts, int64_t segments, int experts) {
+    __shared__ int part[SCAN_WIDTH][SCAN_SHARES];
+    const int col = threadIdx.x % SCAN_WIDTH, share = threadIdx.x / SCAN_WIDTH;
+    const int e = blockIdx.x * SCAN_WIDTH + col;
+    const int64_t per = (segments + SCAN_SHARES - 1) / SCAN_SHARES;
+    const int64_t first = share * per;
+    int64_t last = first + per < segments ? first + per : segments;
+    if (e >= experts) last = first;  // no expert, nothing to add up
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int sum = 0;
+#pragma unroll SCAN_DEEP
+    for (int64_t s = first; s < last; ++s) sum += counts[s * experts + e];
+    part[col][share] = sum;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < SCAN_WIDTH) {  // an expert's shares, each to the sum of those before it
+        constexpr int EACH = SCAN_SHARES / 32;
+        int own[EACH], all = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            own[i] = part[warp][lane * EACH + i];
+            all += own[i];
+        }
+        int scan = all;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, scan, off);
+            if (lane >= off) scan += o;
+        }
+        const int expert = blockIdx.x * SCAN_WIDTH + warp;
+        if (lane == 31 && expert < experts) counts[segments * experts + expert] = scan;
+        scan -= all;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            part[warp][lane * EACH + i] = scan;
+            scan += own[i];
+        }
+    }
+    __syncthreads();
+    int before = part[col][share];
+    for (int64_t s = first; s < last; s += SCAN_DEEP) {
+        int c[SCAN_DEEP];
+#pragma unroll
+        for (int i = 0; i < SCAN_DEEP; ++i) c[i] = s + i < last ? counts[(s + i) * experts + e] : 0;
+#pragma unroll
+        for (int i = 0; i < SCAN_DEEP; ++i) {
+            if (s + i < last) counts[(s + i) * experts + e] = before;
+            before += c[i];
+        }
+    }
+}
+
 __global__ void __launch_bounds__(SORT_THREADS)
     sort_place_kernel(const int32_t *__restrict__ ids, int64_t n, int experts,
-                      const int32_t *__restrict__ counts, int32_t *__restrict__ offsets,
+                      const int32_t *__restrict__ counts, int scanned, int32_t *__restrict__ offsets,
                       int32_t *__restrict__ position, int32_t *__restrict__ source) {
     extern __shared__ int sort_smem[];
     int *next = sort_smem;                      // [SORT_WARPS][experts]: a warp's next place
@@ -267,7 +334,12 @@ __global__ void __launch_bounds__(SORT_THREADS)
     __syncthreads();
     // before[w] = pairs of earlier segments and earlier warps, once those are counted
     if (segments > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (segments > 1) {
+    if (scanned) {
+        for (int e = threadIdx.x; e < experts; e += SORT_THREADS) {
+            earlier[e] = counts[static_cast<int64_t>(seg) * experts + e];
+            total[e] = counts[static_cast<int64_t>(segments) * experts + e];
+        }
+    } else if (segments > 1) {
         // `shares` threads add up an expert's segments, every shares-th each
         const int shares = experts < SORT_THREADS ? SORT_THREADS / experts : 1;
         for (int i = threadIdx.x; i < shares * experts; i += SORT_THREADS) {
@@ -645,27 +717,45 @@ extern "C" int chelis_cuda_expert_sort(const int32_t *ids, int64_t tokens, int32
     const unsigned segments = static_cast<unsigned>((n + experts::SEGMENT - 1) / experts::SEGMENT);
     void *counts = nullptr;
     if (segments > 1) {
-        CHELIS_TRY(scratch_alloc(&counts, sizeof(int32_t) * segments * n_experts, s));
+        CHELIS_TRY(scratch_alloc(&counts, sizeof(int32_t) * (segments + 1) * n_experts, s));
         experts::sort_count_kernel<<<segments, experts::SORT_THREADS, 0, s>>>(
             ids, n, n_experts, static_cast<int32_t *>(counts));
         g_launches++;
     }
+    cudaLaunchAttribute early{};  // the next kernel's blocks start while the last of this one's run
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    const bool scanned = static_cast<int64_t>(segments) * n_experts >= experts::SCAN_FROM;
+    if (scanned) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((n_experts + experts::SCAN_WIDTH - 1) / experts::SCAN_WIDTH);
+        cfg.blockDim = dim3(experts::SCAN_THREADS);
+        cfg.stream = s;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        const int rc = check_cuda(cudaLaunchKernelEx(&cfg, experts::sort_scan_kernel, static_cast<int32_t *>(counts),
+                                                     static_cast<int64_t>(segments), static_cast<int>(n_experts)),
+                                  "experts::sort_scan_kernel");
+        if (rc != CHELIS_CUDA_OK) {
+            scratch_free(counts, s);
+            return rc;
+        }
+        g_launches++;
+    }
     const size_t smem = sizeof(int) * (experts::SORT_WARPS + 2) * n_experts;
-    // the second kernel counts its own pairs while the first one finishes
+    // the last kernel counts its own pairs while the one before it finishes
     // (16384 x 2 by 8 6.8 us against 7.6; with more segments its waiting blocks
-    // are in the way, 16384 x 8 by 64 12.4 against 11.0)
+    // are in the way, 16384 x 8 by 64 12.4 against 11.0 without the scan)
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(segments);
     cfg.blockDim = dim3(experts::SORT_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
+    cfg.attrs = &early;
     cfg.numAttrs = segments > 1 && segments <= 64 ? 1 : 0;
     const int rc = check_cuda(cudaLaunchKernelEx(&cfg, experts::sort_place_kernel, ids, n, static_cast<int>(n_experts),
-                                                 static_cast<const int32_t *>(counts), offsets, position, source),
+                                                 static_cast<const int32_t *>(counts), static_cast<int>(scanned),
+                                                 offsets, position, source),
                               "experts::sort_place_kernel");
     g_launches++;
     scratch_free(counts, s);

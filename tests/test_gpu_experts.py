@@ -140,6 +140,20 @@ def test_sort(cuda, t, k, experts):
     cuda.device_status()
 
 
+# counts of segments that are added up in their own pass: just from there on, shares of one
+# segment and of many, experts that a block of the pass is too wide for
+@pytest.mark.parametrize("t,k,experts", [(8 * 1024, 1, 1024), (4099, 2, 1021), (8 * 1024 + 1, 8, 127), (300007, 3, 13),
+                                         (131072, 8, 64), (1 << 20, 2, 4), (1 << 20, 8, 1)])
+def test_sort_of_many_segments(cuda, t, k, experts):
+    import torch
+    rng = np.random.default_rng(t + experts)
+    ids = rng.integers(-1, experts, size=(t, k), dtype=np.int32)
+    order = cuda.expert_sort(torch.from_numpy(ids).cuda(), experts)
+    for got, ref in zip(order, _fast_sort(ids, experts)):
+        assert np.array_equal(got.cpu().numpy(), ref)
+    cuda.device_status()
+
+
 def _fast_sort(ids, experts):
     flat = ids.reshape(-1).astype(np.int64)
     key = np.where(flat < 0, experts, flat)
