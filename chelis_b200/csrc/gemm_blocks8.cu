@@ -56,8 +56,9 @@ constexpr int LAUNCH_REGS = 168, FEW_REGS = 56, FOLD_REGS = 224;
 static_assert(128 * FEW_REGS + 32 * FOLD_WARPS * FOLD_REGS <= THREADS * LAUNCH_REGS, "register split");
 constexpr uint32_t ACC_COLS = 256, TMEM_COLS = 512;
 constexpr int MAX_GROUPS = experts::MAX_EXPERTS;
-constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + 512 /*barriers*/ +
-                           SCALE_SLOTS * SLOT_FLOATS * 4 + (MAX_GROUPS + 1) * 4 /*tile starts*/;
+constexpr int OUT_BOX = 2048;  // 32 rows x 64 bytes of a fold warp on the way out
+constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + 512 /*barriers*/ + SCALE_SLOTS * SLOT_FLOATS * 4 +
+                           FOLD_WARPS * OUT_BOX + (MAX_GROUPS + 1) * 4 /*tile starts*/;
 
 struct Params {
     int64_t rows;     // rows of a: tokens (forward, input gradient), outputs (weight gradient)
@@ -251,47 +252,99 @@ __device__ __forceinline__ uint32_t round2(float2 v, bool bf) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// This thread's row, 128 columns of which `left` lie in the result.
-__device__ __forceinline__ void store_row(const Params &p, const f32x2 (&run)[64], int64_t index,
-                                          int64_t left) {
-    if (p.out_dtype == CHELIS_DTYPE_F32) {
-        float *o = static_cast<float *>(p.out) + index;
-        if (left >= 128 && (reinterpret_cast<uintptr_t>(o) & 31) == 0) {
+// 64 bytes of this lane's row into the warp's 32 x 64 byte box, 16-byte pieces
+// in the order of TMA's 64-byte swizzle.
+__device__ __forceinline__ void stage_box(unsigned char *box, int lane, const uint32_t (&w)[16]) {
 #pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                uint32_t w[8];
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4 *>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+// Columns N * 64 bytes on of this thread's row, as they are stored.
+template <int N>
+__device__ __forceinline__ void box_words(const f32x2 (&run)[64], int32_t dtype, uint32_t (&w)[16]) {
+    if (dtype == CHELIS_DTYPE_F32) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 v = unpack2(run[j + i]);
-                    w[2 * i] = __float_as_uint(v.x);
-                    w[2 * i + 1] = __float_as_uint(v.y);
-                }
-                store32(o + 2 * j, w);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                const float2 v = unpack2(run[j]);
-                if (2 * j < left) o[2 * j] = v.x;
-                if (2 * j + 1 < left) o[2 * j + 1] = v.y;
-            }
+        for (int c = 0; c < 8; ++c) {
+            const float2 v = unpack2(run[(N * 8 + c) & 63]);
+            w[2 * c] = __float_as_uint(v.x);
+            w[2 * c + 1] = __float_as_uint(v.y);
         }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) w[c] = round2(unpack2(run[(N * 16 + c) & 63]), dtype == CHELIS_DTYPE_BF16);
+    }
+}
+
+// The rows of a box to global memory, U at a time: two rows (32-bit units) or
+// one (16-bit) by the warp's 32 lanes.
+template <typename U>
+__device__ __forceinline__ void store_box(const unsigned char *box, int lane, U *out, int64_t ld, int rows,
+                                          int64_t cols) {
+    constexpr int WIDE = 64 / static_cast<int>(sizeof(U)), ROWS = 32 / WIDE;
+    const int c = lane % WIDE, byte = c * static_cast<int>(sizeof(U));
+    if (c >= cols) return;
+#pragma unroll 8
+    for (int r = lane / WIDE; r < rows; r += ROWS)
+        out[r * ld + c] = *reinterpret_cast<const U *>(box + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+}
+template <int N>
+__device__ __forceinline__ void store_boxes(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
+                                            int64_t index, int rows, int64_t left) {
+    const bool f32 = p.out_dtype == CHELIS_DTYPE_F32;
+    const int cols = f32 ? 16 : 32;  // of a box
+    if (N * cols >= 128 || N * cols >= left) return;
+    uint32_t w[16];
+    box_words<N>(run, p.out_dtype, w);
+    __syncwarp();
+    stage_box(box, lane, w);
+    __syncwarp();
+    const int64_t at = index + N * cols;
+    if (f32)
+        store_box(box, lane, static_cast<uint32_t *>(p.out) + at, p.n, rows, left - N * cols);
+    else if ((p.n & 1) == 0 && (reinterpret_cast<uintptr_t>(static_cast<uint16_t *>(p.out) + at) & 3) == 0)
+        store_box(box, lane, reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + at), p.n / 2, rows,
+                  (left - N * cols) / 2);
+    else
+        store_box(box, lane, static_cast<uint16_t *>(p.out) + at, p.n, rows, left - N * cols);
+    if constexpr (N < 7) store_boxes<N + 1>(p, run, box, lane, index, rows, left);
+}
+
+// 32 rows x 128 columns of a warp from element `index` on, of which `rows` and
+// `left` lie in the result.  Whole columns of rows that start on 32 bytes go
+// from each thread's registers, a sector at a time; others through the warp's
+// box, so that neighbouring lanes write neighbouring elements.  One element at
+// a time from the registers touched 32 sectors a store: 8941 x 3329 x 144 by
+// 11 experts to f16 336 us, so 55; 20930 x 263 x 135 by 19 112 and 26; up to 2
+// us are lost where a tile has a few rows alone.
+__device__ __forceinline__ void store_rows(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
+                                           int64_t index, int rows, int64_t left) {
+    const int64_t w = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
+    if (left < 128 || p.n * w % 32 != 0 || ((reinterpret_cast<uintptr_t>(p.out) + index * w) & 31) != 0) {
+        store_boxes<0>(p, run, box, lane, index, rows, left);
         return;
     }
-    const bool bf = p.out_dtype == CHELIS_DTYPE_BF16;
-    uint16_t *o = static_cast<uint16_t *>(p.out) + index;
-    const bool vec = left >= 128 && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
+    if (lane >= rows) return;
+    unsigned char *o = static_cast<unsigned char *>(p.out) + (index + lane * p.n) * w;
+    if (p.out_dtype == CHELIS_DTYPE_F32) {
 #pragma unroll
-    for (int j = 0; j < 64; j += 8) {
-        uint32_t w[8];
+        for (int j = 0; j < 64; j += 4) {
+            uint32_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = round2(unpack2(run[j + i]), bf);
-        if (vec) {
-            store32(o + 2 * j, w);
-        } else {
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2(run[j + i]);
+                v[2 * i] = __float_as_uint(f.x);
+                v[2 * i + 1] = __float_as_uint(f.y);
+            }
+            store32(o + 8 * j, v);
+        }
+    } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (2 * j + i < left) o[2 * j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        for (int j = 0; j < 64; j += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = round2(unpack2(run[j + i]), p.out_dtype == CHELIS_DTYPE_BF16);
+            store32(o + 4 * j, v);
         }
     }
 }
@@ -397,7 +450,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     volatile uint32_t *abort_flag = tmem_slot + 1;
     volatile int32_t *consumed = reinterpret_cast<volatile int32_t *>(tmem_slot + 2);
     float *scales = reinterpret_cast<float *>(smem + RING_BYTES + 512);
-    int32_t *start = reinterpret_cast<int32_t *>(scales + SCALE_SLOTS * SLOT_FLOATS);
+    unsigned char *out_stage = reinterpret_cast<unsigned char *>(scales + SCALE_SLOTS * SLOT_FLOATS);
+    int32_t *start = reinterpret_cast<int32_t *>(out_stage + FOLD_WARPS * OUT_BOX);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t tries = *static_cast<volatile uint32_t *>(&g_wait_tries);
@@ -548,8 +602,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true;
         for (int L = first; ok && L < tiles; L += step) {
             const Tile t = tile_at<WG, BM>(p, start, L);
-            const int64_t row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * 128;
-            const bool live = row - lane < t.m_end && col0 < p.n;  // else nothing to read or store
+            const int64_t row0 = t.m0 + quad * 32, col0 = t.n0 + half * 128;
+            const bool live = row0 < t.m_end && col0 < p.n;  // else nothing to read or store
             f32x2 run[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) run[j] = 0ull;
@@ -601,9 +655,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scale_empty[q]);
             }
-            if (ok && live && row < t.m_end) {
+            if (ok && live) {
                 const int64_t base = WG ? t.group * p.rows * p.n : 0;
-                store_row(p, run, base + row * p.n + col0, p.n - col0);
+                const int rows = static_cast<int>(t.m_end - row0 < 32 ? t.m_end - row0 : 32);
+                store_rows(p, run, out_stage + (warp - 4) * OUT_BOX, lane, base + row0 * p.n + col0, rows,
+                           p.n - col0);
             }
         }
         if (!WG && p.offsets) zero_loose_rows(p);

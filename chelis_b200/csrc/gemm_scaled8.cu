@@ -45,8 +45,7 @@ constexpr int SF_BYTES = 512;             // packed scales of 128 rows, four blo
 constexpr int SF_SLOT = 3 * SF_BYTES;     // a's 128 rows, b's 256 columns
 constexpr uint32_t ACC1 = 224;            // first column of the second accumulator
 constexpr uint32_t SF_COL = 480;          // two slots of 12 columns of scales
-constexpr int OUT_BOX = 2048;             // 32 rows x 64 bytes on the way out
-constexpr int OUT_BUFS = 1;               // of them a warp
+constexpr int OUT_BUFS = 1;               // boxes of a warp on the way out
 constexpr int OUT_BYTES = FOLD_WARPS * OUT_BUFS * OUT_BOX;
 
 constexpr int TM = 2 * BM;                // rows of a pair's tile
@@ -251,15 +250,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t sr
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void store_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(OUT_BUFS - 1) : "memory");
-}
-
-// 64 bytes of this lane's row into the warp's 32 x 64 byte box, in the 64-byte
-// swizzle that the map names.
-__device__ __forceinline__ void stage_box(unsigned char *box, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4 *>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
 // 32 rows x 128 columns of a warp, 64 bytes of each row at a time through its
@@ -524,9 +514,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             // group's last rows one by one
             if (q.tma_out && (WG || row0 + 32 <= t.m_end)) {
                 store_tma(p, &map_out, run, stage, lane, col0, row0, WG ? t.group : 0);
-            } else if (row0 + lane < t.m_end) {
+            } else {
                 const int64_t base = WG ? t.group * p.rows * p.n : 0;
-                store_row(p, run, base + (row0 + lane) * p.n + col0, p.n - col0);
+                const int rows = static_cast<int>(t.m_end - row0 < 32 ? t.m_end - row0 : 32);
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is free
+                store_rows(p, run, stage, lane, base + row0 * p.n + col0, rows, p.n - col0);
             }
         }
         if (!WG && p.offsets) zero_loose_rows(p);
