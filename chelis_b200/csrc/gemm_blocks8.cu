@@ -72,6 +72,7 @@ struct Params {
     int64_t sb_group, sb_n, sb_k;  // tiles: strides of expert, column block, contraction block
     void *out;
     int32_t out_dtype;
+    int32_t parts;       // of the contraction, each with a result of its own (part_sums)
     uint32_t idesc;
 };
 
@@ -175,46 +176,66 @@ __device__ __forceinline__ void group_starts(const Params &p, int64_t rows, int 
     if (lane == 0) start[0] = 0;
 }
 
-// One tile of the result.
+// One tile of the result.  Extents are below 2^31 and so are the tiles that
+// fit any memory: 32 bits, as the fold has no register to spare.
 struct Tile {
     int group;
     int m_tile;         // its row tile, counted over all groups (weight gradient: in its matrix)
-    int64_t m0, m_end;  // rows of the result, this tile's first and the group's last + 1
-    int64_t n0;
+    int m0, m_end;      // rows of the result, this tile's first and the group's last + 1
+    int n0;
     int kb0, kbs;       // contraction blocks
+    int in_group;       // of them before kb0 in the group
+    int matrix;         // of the result: a group's (weight gradient), a part's
 };
+
+// Blocks of part `part` of a contraction, in whole units of UNIT.
+template <int UNIT>
+__device__ __forceinline__ void take_part(const Params &p, int part, Tile *t) {
+    const int64_t units = (t->kbs + UNIT - 1) / UNIT;
+    const int lo = static_cast<int>(units * part / p.parts) * UNIT, hi = static_cast<int>(units * (part + 1) / p.parts) * UNIT;
+    t->kbs = min(hi, t->kbs) - lo;
+    t->kb0 += lo;
+    t->in_group = lo;
+}
 
 // Tiles of one group's matrix (mt x nt) in bands of BAND row tiles, column by
 // column within a band: the tiles in flight then share a few panels of a and
 // b in L2 however tall the matrix is (8192^3 by pairs: bands of 4, 8 and 16
 // tiles 425, 435 and 458 us, whole columns 440).
 constexpr int BAND = 8;
-__device__ __forceinline__ void band_order(int64_t in, int64_t mt, int64_t nt, int64_t *m, int64_t *n) {
-    const int64_t band = in / (BAND * nt), first = band * BAND;
-    const int64_t high = mt - first < BAND ? mt - first : BAND, r = in - band * (BAND * nt);
+__device__ __forceinline__ void band_order(int in, int mt, int nt, int *m, int *n) {
+    const int band = in / (BAND * nt), first = band * BAND;
+    const int high = min(mt - first, BAND), r = in - band * (BAND * nt);
     *n = r / high;
     *m = first + (r - *n * high);
 }
 
 // `start` is, by group, the prefix of row tiles of TM rows (forward, input
 // gradient) or of contraction blocks (weight gradient).
-template <bool WG, int TM>
-__device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, int64_t L) {
-    const int64_t nt = (p.n + BN - 1) / BN;
+template <bool WG, int TM, int UNIT>
+__device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, int L) {
+    const int nt = static_cast<int>((p.n + BN - 1) / BN);
     Tile t;
+    t.in_group = 0;
+    int m, n;
     if (WG) {
-        const int64_t mt = (p.rows + TM - 1) / TM;
-        t.group = static_cast<int>(L / (mt * nt));
-        const int64_t in = L - t.group * mt * nt;
-        int64_t m, n;
-        band_order(in, mt, nt, &m, &n);
-        t.m_tile = static_cast<int>(m);
+        const int mt = static_cast<int>((p.rows + TM - 1) / TM);
+        t.matrix = L / (mt * nt);
+        band_order(L - t.matrix * (mt * nt), mt, nt, &m, &n);
+        t.group = p.parts > 1 ? t.matrix / p.parts : t.matrix;
+        t.m_tile = m;
         t.m0 = m * TM;
-        t.n0 = n * BN;
-        t.m_end = p.rows;
+        t.m_end = static_cast<int>(p.rows);
         t.kb0 = start[t.group];
         t.kbs = start[t.group + 1] - t.kb0;
+        if (p.parts > 1) take_part<UNIT>(p, t.matrix - t.group * p.parts, &t);
     } else {
+        t.matrix = 0;
+        if (p.parts > 1) {
+            const int tiles = start[p.groups] * nt;
+            t.matrix = L / tiles;
+            L -= t.matrix * tiles;
+        }
         int lo = 0, hi = p.groups;  // the last group whose first tile is at or before L
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -222,18 +243,17 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *start, i
             else hi = mid;
         }
         t.group = lo;
-        const int64_t in = L - start[lo] * nt, mt = start[lo + 1] - start[lo];
+        band_order(L - start[lo] * nt, start[lo + 1] - start[lo], nt, &m, &n);
         int64_t a, b;
         group_span(p, p.rows, lo, &a, &b);
-        int64_t m, n;
-        band_order(in, mt, nt, &m, &n);
-        t.m_tile = start[lo] + static_cast<int>(m);
-        t.m0 = a + m * TM;
-        t.n0 = n * BN;
-        t.m_end = b;
+        t.m_tile = start[lo] + m;
+        t.m0 = static_cast<int>(a) + m * TM;
+        t.m_end = static_cast<int>(b);
         t.kb0 = 0;
         t.kbs = p.kblocks;
+        if (p.parts > 1) take_part<UNIT>(p, t.matrix, &t);
     }
+    t.n0 = n * BN;
     return t;
 }
 
@@ -263,7 +283,7 @@ __device__ __forceinline__ void stage_box(unsigned char *box, int lane, const ui
 // Columns N * 64 bytes on of this thread's row, as they are stored.
 template <int N>
 __device__ __forceinline__ void box_words(const f32x2 (&run)[64], int32_t dtype, uint32_t (&w)[16]) {
-    if (dtype == CHELIS_DTYPE_F32) {
+    if (N >= 4 || dtype == CHELIS_DTYPE_F32) {  // 16 bits fill four boxes
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const float2 v = unpack2(run[(N * 8 + c) & 63]);
@@ -276,56 +296,88 @@ __device__ __forceinline__ void box_words(const f32x2 (&run)[64], int32_t dtype,
     }
 }
 
-// The rows of a box to global memory, U at a time: two rows (32-bit units) or
-// one (16-bit) by the warp's 32 lanes.
+__device__ __forceinline__ uint32_t load_shared(uint32_t at, uint32_t) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint16_t load_shared(uint32_t at, uint16_t) {
+    uint16_t v;
+    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_if(bool ok, void *p, uint32_t v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}" ::"l"(p), "r"(v),
+                 "r"(static_cast<int>(ok))
+                 : "memory");
+}
+__device__ __forceinline__ void store_if(bool ok, void *p, uint16_t v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}" ::"l"(p), "h"(v),
+                 "r"(static_cast<int>(ok))
+                 : "memory");
+}
+// The rows of a box to global memory from `out`, U at a time: two rows (32-bit
+// units) or one (16-bit) by the warp's 32 lanes, sixteen loads before their
+// stores.  The loads are asm because the compiler, depending on what else is in
+// the file, moved each one under its store's condition, which made the stores
+// wait for one load after another (6718 x 2335 x 656 by 26 experts 54 against
+// 47 us).
 template <typename U>
-__device__ __forceinline__ void store_box(const unsigned char *box, int lane, U *out, int64_t ld, int rows,
-                                          int64_t cols) {
-    constexpr int WIDE = 64 / static_cast<int>(sizeof(U)), ROWS = 32 / WIDE;
-    const int c = lane % WIDE, byte = c * static_cast<int>(sizeof(U));
-    if (c >= cols) return;
-#pragma unroll 8
-    for (int r = lane / WIDE; r < rows; r += ROWS)
-        out[r * ld + c] = *reinterpret_cast<const U *>(box + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+__device__ __forceinline__ void store_box(const unsigned char *box, int lane, unsigned char *out, int64_t ld, int rows,
+                                          int bytes) {
+    constexpr int WIDE = 64 / static_cast<int>(sizeof(U)), ROWS = 32 / WIDE, DEEP = 16;
+    const int byte = lane % WIDE * static_cast<int>(sizeof(U)), row = lane / WIDE;
+    rows = byte < bytes ? rows - row : 0;
+    out += row * ld + byte;
+    const uint32_t at = smem_u32(box) + row * 64 + (byte & 15), piece = byte >> 4;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += DEEP * ROWS) {
+        U v[DEEP];
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+            const int r = r0 + i * ROWS;  // its bits 1 and 2 alone turn the pieces round
+            v[i] = load_shared(at + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4), U{});
+        }
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+            store_if(r0 + i * ROWS < rows, out, v[i]);
+            out += ROWS * ld;
+        }
+    }
 }
 template <int N>
-__device__ __forceinline__ void store_boxes(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
-                                            int64_t index, int rows, int64_t left) {
-    const bool f32 = p.out_dtype == CHELIS_DTYPE_F32;
-    const int cols = f32 ? 16 : 32;  // of a box
-    if (N * cols >= 128 || N * cols >= left) return;
+__device__ __forceinline__ void store_boxes(const f32x2 (&run)[64], int32_t dtype, unsigned char *box, int lane,
+                                            unsigned char *out, int64_t ld, int rows, int bytes) {
+    if (N * 64 >= bytes) return;
     uint32_t w[16];
-    box_words<N>(run, p.out_dtype, w);
+    box_words<N>(run, dtype, w);
     __syncwarp();
     stage_box(box, lane, w);
     __syncwarp();
-    const int64_t at = index + N * cols;
-    if (f32)
-        store_box(box, lane, static_cast<uint32_t *>(p.out) + at, p.n, rows, left - N * cols);
-    else if ((p.n & 1) == 0 && (reinterpret_cast<uintptr_t>(static_cast<uint16_t *>(p.out) + at) & 3) == 0)
-        store_box(box, lane, reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + at), p.n / 2, rows,
-                  (left - N * cols) / 2);
+    if (((reinterpret_cast<uintptr_t>(out) | ld) & 3) == 0)
+        store_box<uint32_t>(box, lane, out + N * 64, ld, rows, bytes - N * 64);
     else
-        store_box(box, lane, static_cast<uint16_t *>(p.out) + at, p.n, rows, left - N * cols);
-    if constexpr (N < 7) store_boxes<N + 1>(p, run, box, lane, index, rows, left);
+        store_box<uint16_t>(box, lane, out + N * 64, ld, rows, bytes - N * 64);
+    if constexpr (N < 7) store_boxes<N + 1>(run, dtype, box, lane, out, ld, rows, bytes);
 }
 
 // 32 rows x 128 columns of a warp from element `index` on, of which `rows` and
 // `left` lie in the result.  Whole columns of rows that start on 32 bytes go
 // from each thread's registers, a sector at a time; others through the warp's
-// box, so that neighbouring lanes write neighbouring elements.  One element at
+// box, so that neighbouring lanes write neighbouring units.  One element at
 // a time from the registers touched 32 sectors a store: 8941 x 3329 x 144 by
 // 11 experts to f16 336 us, so 55; 20930 x 263 x 135 by 19 112 and 26; up to 2
 // us are lost where a tile has a few rows alone.
 __device__ __forceinline__ void store_rows(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
                                            int64_t index, int rows, int64_t left) {
-    const int64_t w = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
-    if (left < 128 || p.n * w % 32 != 0 || ((reinterpret_cast<uintptr_t>(p.out) + index * w) & 31) != 0) {
-        store_boxes<0>(p, run, box, lane, index, rows, left);
+    const int w = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
+    unsigned char *first = static_cast<unsigned char *>(p.out) + index * w;
+    if (left < 128 || p.n * w % 32 != 0 || (reinterpret_cast<uintptr_t>(first) & 31) != 0) {
+        store_boxes<0>(run, p.out_dtype, box, lane, first, p.n * w, rows, static_cast<int>(left < 128 ? left : 128) * w);
         return;
     }
     if (lane >= rows) return;
-    unsigned char *o = static_cast<unsigned char *>(p.out) + (index + lane * p.n) * w;
+    unsigned char *o = first + lane * p.n * w;
     if (p.out_dtype == CHELIS_DTYPE_F32) {
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
@@ -419,8 +471,9 @@ __device__ __forceinline__ void zero_loose_rows(const Params &p) {
     const int64_t who = static_cast<int64_t>(blockIdx.x) * (FOLD_WARPS * 32) + threadIdx.x - (THREADS - FOLD_WARPS * 32);
     const int64_t step = static_cast<int64_t>(gridDim.x) * (FOLD_WARPS * 32);
     const int64_t loose = (first + p.rows - last) * p.n;
-    for (int64_t i = who; i < loose; i += step) {
-        const int64_t e = i < first * p.n ? i : last * p.n + (i - first * p.n);
+    for (int64_t i = who; i < loose * p.parts; i += step) {
+        const int64_t part = p.parts > 1 ? i / loose : 0, j = i - part * loose;
+        const int64_t e = part * p.rows * p.n + (j < first * p.n ? j : last * p.n + (j - first * p.n));
         if (p.out_dtype == CHELIS_DTYPE_F32) static_cast<float *>(p.out)[e] = 0.0f;
         else static_cast<uint16_t *>(p.out)[e] = 0;
     }
@@ -484,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int64_t nt = (p.n + BN - 1) / BN;
-    const int tiles = uniform(static_cast<int>(WG ? p.groups * nt * ((p.rows + BM - 1) / BM) : start[p.groups] * nt));
+    const int tiles = uniform(static_cast<int>(p.parts * (WG ? p.groups * nt * ((p.rows + BM - 1) / BM) : start[p.groups] * nt)));
     const int first = static_cast<int>(blockIdx.x), step = static_cast<int>(gridDim.x);
     int32_t issued = 0;
 
@@ -496,9 +549,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t phase = 1;
             bool ok = true;
             for (int L = first; ok && L < tiles; L += step) {
-                const Tile t = tile_at<WG, BM>(p, start, L);
+                const Tile t = tile_at<WG, BM, 1>(p, start, L);
                 const int group = uniform(t.group), kbs = uniform(t.kbs);
-                const int32_t m0 = uniform(static_cast<int32_t>(t.m0)), n0 = uniform(static_cast<int32_t>(t.n0));
+                const int32_t m0 = uniform(t.m0), n0 = uniform(t.n0);
                 int32_t k0 = uniform(t.kb0) * BK;
                 for (int i = 0; i < kbs; ++i, k0 += BK) {
                     ok = all(wait(&empty[stage], phase, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER));
@@ -531,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t phase = 0;
             bool ok = true;
             for (int L = first; ok && L < tiles; L += step) {
-                const int kbs = WG ? uniform(tile_at<WG, BM>(p, start, L).kbs) : p.kblocks;
+                const int kbs = WG || p.parts > 1 ? uniform(tile_at<WG, BM, 1>(p, start, L).kbs) : p.kblocks;
                 for (int i = 0; i < kbs; ++i, ++it) {
                     const int cur = it & 1;
                     if (it >= 2)
@@ -563,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             int32_t it = 0;
             bool ok = true;
             for (int L = first; ok && L < tiles; L += step) {
-                const Tile t = tile_at<WG, BM>(p, start, L);
+                const Tile t = tile_at<WG, BM, 1>(p, start, L);
                 const float *tile_sb = p.sb + t.group * p.sb_group + (t.n0 / 128) * p.sb_n;
                 for (int i = 0; i < t.kbs; ++i, ++it) {
                     const int q = it % SCALE_SLOTS;
@@ -601,8 +654,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         int32_t it = 0;
         bool ok = true;
         for (int L = first; ok && L < tiles; L += step) {
-            const Tile t = tile_at<WG, BM>(p, start, L);
-            const int64_t row0 = t.m0 + quad * 32, col0 = t.n0 + half * 128;
+            const Tile t = tile_at<WG, BM, 1>(p, start, L);
+            const int row0 = t.m0 + quad * 32, col0 = t.n0 + half * 128;
             const bool live = row0 < t.m_end && col0 < p.n;  // else nothing to read or store
             f32x2 run[64];
 #pragma unroll
@@ -655,12 +708,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scale_empty[q]);
             }
-            if (ok && live) {
-                const int64_t base = WG ? t.group * p.rows * p.n : 0;
-                const int rows = static_cast<int>(t.m_end - row0 < 32 ? t.m_end - row0 : 32);
-                store_rows(p, run, out_stage + (warp - 4) * OUT_BOX, lane, base + row0 * p.n + col0, rows,
-                           p.n - col0);
-            }
+            if (ok && live)
+                store_rows(p, run, out_stage + (warp - 4) * OUT_BOX, lane,
+                           (t.matrix * p.rows + row0) * p.n + col0, min(t.m_end - row0, 32), p.n - col0);
         }
         if (!WG && p.offsets) zero_loose_rows(p);
     }
@@ -700,6 +750,75 @@ int64_t row_tiles(int64_t rows, int32_t groups, bool offsets, int64_t high) {
     return (rows + high - 1) / high + (offsets ? groups : 0);
 }
 
+// ---- parts ----------------------------------------------------------------
+// Fewer tiles than half the machine: the contraction is cut into parts, each
+// tile of each part its own piece of work with its own f32 result, which
+// part_sums_kernel adds up in order (us, whole and in parts): weight gradients
+// 256 x 256 from 8192 rows 77 and 17, 1024 x 256 from 131072 rows 339 and 48,
+// products 512 x 1024 x 16384 47 and 22, input gradient 16 x 1024 x 4096 30 and
+// 11.  Each part costs a result written and read and the join its launch: with
+// 6 blocks saved of 12, 1369 x 1013 x 1507 by 4 experts took 21 us and whole 17.
+constexpr int PART_BLOCKS = 2;   // that a part has at least (2, 4, 8: 169 x 133 from 3332 rows by 2 22, 27, 45 us)
+constexpr int SAVED_BLOCKS = 8;  // one after another, from which the second launch pays
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+    part_sums_kernel(const float *__restrict__ parts, int32_t count, int64_t matrix, int64_t all, T *__restrict__ out) {
+    constexpr int N = VEC ? 4 : 1;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * N;
+    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N; i < all; i += step) {
+        const int64_t g = i / matrix;
+        const float *src = parts + g * count * matrix + (i - g * matrix);
+        float sum[N] = {};
+#pragma unroll 4
+        for (int s = 0; s < count; ++s) {
+            if constexpr (VEC) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(src + s * matrix));
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            } else {
+                sum[0] += __ldg(src + s * matrix);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < N; ++c) out[i + c] = experts::from_f32<T>(sum[c]);
+    }
+}
+
+int32_t part_count(int64_t tiles, int64_t blocks, int64_t workers, int64_t least, int64_t saved) {
+    if (2 * tiles > workers) return 1;
+    const int64_t most = workers / tiles, parts = blocks / least < most ? blocks / least : most;
+    return parts < 2 || blocks - (blocks + parts - 1) / parts < saved ? 1 : static_cast<int32_t>(parts);
+}
+
+// f(p) with p.parts results in scratch and their sums into p.out; f(p) itself
+// for one part.
+template <typename F>
+int in_parts(Params p, int32_t parts, int64_t matrices, F f) {
+    p.parts = parts;
+    if (parts == 1) return f(p);
+    cudaStream_t s = current_stream();
+    const int64_t matrix = p.rows * p.n, all = matrices * matrix;
+    void *out = p.out, *sums = nullptr;
+    const int32_t dtype = p.out_dtype;
+    CHELIS_TRY(scratch_alloc(&sums, static_cast<size_t>(parts) * all * sizeof(float), s));
+    p.out = sums;
+    p.out_dtype = CHELIS_DTYPE_F32;
+    int rc = f(p);
+    if (rc == CHELIS_CUDA_OK) {
+        const bool vec = matrix % 4 == 0;
+        experts::by_type(dtype, vec, [&](auto t, auto v) {
+            using T = decltype(t);
+            constexpr bool VEC = decltype(v)::value;
+            part_sums_kernel<T, VEC><<<blocks8::grid_for((all / (VEC ? 4 : 1) + 255) / 256, 8), 256, 0, s>>>(
+                static_cast<const float *>(sums), parts, matrix, all, static_cast<T *>(out));
+        });
+        g_launches++;
+        rc = check_cuda(cudaGetLastError(), "gemm8::part_sums_kernel");
+    }
+    scratch_free(sums, s);
+    return rc;
+}
+
 template <bool BMN, bool WG>
 int run(const CUtensorMap &ma, const CUtensorMap &mb, Params p, int32_t fa, int32_t fb) {
     p.idesc = (1u << 4) |                                    // f32 sums
@@ -714,11 +833,15 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, Params p, int32_t fa, int3
     CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
                           "cudaFuncSetAttribute"));
     const int64_t sms = sm_count();
-    kernel<<<static_cast<unsigned>(most < sms ? (most < 1 ? 1 : most) : sms), THREADS, SMEM_BYTES, current_stream()>>>(
-        ma, mb, p);
-    g_launches++;
-    CHELIS_LAUNCH_CHECK("gemm8::gemm8_kernel");
-    return CHELIS_CUDA_OK;
+    const int32_t parts = part_count(most, WG ? p.kblocks / p.groups : p.kblocks, sms, PART_BLOCKS,
+                                     SAVED_BLOCKS);
+    return in_parts(p, parts, WG ? p.groups : 1, [&](const Params &q) -> int {
+        const int64_t grid = parts * most < sms ? parts * most : sms;
+        kernel<<<static_cast<unsigned>(grid), THREADS, SMEM_BYTES, current_stream()>>>(ma, mb, q);
+        g_launches++;
+        CHELIS_LAUNCH_CHECK("gemm8::gemm8_kernel");
+        return CHELIS_CUDA_OK;
+    });
 }
 
 int check_common(const char *op, int32_t fa, int32_t fb, int32_t out_dtype, int64_t rows, int64_t n,

@@ -212,31 +212,25 @@ __device__ __forceinline__ void mma_scaled(uint32_t tmem_d, uint64_t adesc, uint
 }
 
 // ---- fold -----------------------------------------------------------------
-template <int J>
-__device__ __forceinline__ void add32(f32x2 (&run)[64], const uint32_t (&r)[32]) {
-#pragma unroll
-    for (int c = 0; c < 16; ++c)
-        run[J * 16 + c] = add2(run[J * 16 + c], pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])));
-}
-// This warp's 128 columns in the order J0 .. J3 of 32, the next loading while
-// one is added; `first` runs once the first 32 have been read, `last` once all.
-template <int J0, int J1, int J2, int J3, typename F, typename G>
+// This warp's 128 columns 16 at a time, from the FIRST of the eight pieces on,
+// the next loading while one is added; `first` runs once two pieces have been
+// read, `last` once all.  (32 at a time need 32 registers more and spilled.)
+template <int FIRST, typename F, typename G>
 __device__ __forceinline__ void fold128(f32x2 (&run)[64], uint32_t acc, F first, G last) {
-    uint32_t r0[32], r1[32];
-    tmem_ld_32x32b_x32(acc + J0 * 32, r0);
-    tmem_wait_ld();
-    first();
-    tmem_ld_32x32b_x32(acc + J1 * 32, r1);
-    add32<J0>(run, r0);
-    tmem_wait_ld();
-    tmem_ld_32x32b_x32(acc + J2 * 32, r0);
-    add32<J1>(run, r1);
-    tmem_wait_ld();
-    tmem_ld_32x32b_x32(acc + J3 * 32, r1);
-    add32<J2>(run, r0);
-    tmem_wait_ld();
-    last();
-    add32<J3>(run, r1);
+    uint32_t r[2][16];
+    tmem_ld_32x32b_x16(acc + FIRST * 16, r[0]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int piece = (FIRST + j) % 8, next = (FIRST + j + 1) % 8;
+        tmem_wait_ld();
+        if (j == 1) first();
+        if (j == 7) last();
+        else tmem_ld_32x32b_x16(acc + next * 16, r[(j + 1) & 1]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            run[piece * 8 + c] = add2(run[piece * 8 + c], pack2(__uint_as_float(r[j & 1][2 * c]),
+                                                                __uint_as_float(r[j & 1][2 * c + 1])));
+    }
 }
 
 // ---- the way out ----------------------------------------------------------
@@ -352,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int64_t nt = (p.n + BN - 1) / BN;
-    const int64_t tiles = WG ? p.groups * nt * ((p.rows + TM - 1) / TM) : start[p.groups] * nt;
+    const int64_t tiles = p.parts * (WG ? p.groups * nt * ((p.rows + TM - 1) / TM) : start[p.groups] * nt);
     const int all_tiles = uniform(static_cast<int>(tiles));
     int32_t issued = 0;
 
@@ -365,12 +359,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");  // the packed scales are written
             for (int L = worker; ok && L < all_tiles; L += workers) {
-                const Tile t = tile_at<WG, TM>(p, start, L);
+                const Tile t = tile_at<WG, TM, QUAD>(p, start, L);
                 const int group = uniform(t.group), kbs = uniform(t.kbs), kb0 = uniform(t.kb0);
-                const int32_t m0 = uniform(static_cast<int32_t>(t.m0)) + static_cast<int32_t>(rank) * BM;
-                const int32_t n_tile = uniform(static_cast<int32_t>(t.n0));
+                const int32_t m0 = uniform(t.m0) + static_cast<int32_t>(rank) * BM;
+                const int32_t n_tile = uniform(t.n0);
                 const int32_t n0 = n_tile + static_cast<int32_t>(rank) * 128;
-                const int quad0 = WG ? uniform(quad_start[group]) : 0;
+                const int quad0 = uniform((WG ? quad_start[group] : 0) + t.in_group / QUAD);
                 int32_t sfa = uniform(t.m_tile) * (TM / 128) + static_cast<int32_t>(rank) + quad0 * q.m_atoms;
                 int32_t sfb = (WG ? 0 : group * q.sfb_group) + n_tile / 128 + quad0 * q.sfb_k;
                 int32_t k0 = kb0 * BK;
@@ -413,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t phase = 0;
             bool ok = true, ready = false;
             for (int L = worker; ok && L < all_tiles; L += workers) {
-                const int kbs = WG ? uniform(tile_at<WG, TM>(p, start, L).kbs) : p.kblocks;
+                const int kbs = WG || p.parts > 1 ? uniform(tile_at<WG, TM, QUAD>(p, start, L).kbs) : p.kblocks;
                 uint32_t d = 0;
                 int cur = 0;
                 for (int i = 0; i < kbs; ++i, ++it) {
@@ -480,8 +474,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         int32_t chunk = 0;
         bool ok = true;
         for (int L = worker; ok && L < all_tiles; L += workers) {
-            const Tile t = tile_at<WG, TM>(p, start, L);
-            const int64_t row0 = t.m0 + rank * BM + quad * 32, col0 = t.n0 + half * 128;
+            const Tile t = tile_at<WG, TM, QUAD>(p, start, L);
+            const int row0 = t.m0 + static_cast<int>(rank) * BM + quad * 32, col0 = t.n0 + half * 128;
             const bool live = row0 < t.m_end && col0 < p.n;  // else nothing to read or store
             f32x2 run[64];
 #pragma unroll
@@ -505,20 +499,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!live) {
                     if (half != b) arrive(shared_cols);
                     arrive(&acc_empty[b]);
-                } else if (b == 0 && half == 1) fold128<3, 0, 1, 2>(run, acc, shared, done);
-                else if (b == 1 && half == 0) fold128<0, 1, 2, 3>(run, acc, shared, done);
-                else fold128<0, 1, 2, 3>(run, acc, none, done);
+                } else if (b == 0 && half == 1) fold128<6>(run, acc, shared, done);
+                else if (b == 1 && half == 0) fold128<0>(run, acc, shared, done);
+                else fold128<0>(run, acc, none, done);
             }
             if (!ok || !live) continue;
             // whole rows of 32 by TMA (which cuts at the result's own edge); a
             // group's last rows one by one
             if (q.tma_out && (WG || row0 + 32 <= t.m_end)) {
-                store_tma(p, &map_out, run, stage, lane, col0, row0, WG ? t.group : 0);
+                store_tma(p, &map_out, run, stage, lane, col0, row0, t.matrix);
             } else {
-                const int64_t base = WG ? t.group * p.rows * p.n : 0;
-                const int rows = static_cast<int>(t.m_end - row0 < 32 ? t.m_end - row0 : 32);
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is free
-                store_rows(p, run, stage, lane, base + row0 * p.n + col0, rows, p.n - col0);
+                store_rows(p, run, stage, lane, (t.matrix * p.rows + row0) * p.n + col0, min(t.m_end - row0, 32),
+                           p.n - col0);
             }
         }
         if (!WG && p.offsets) zero_loose_rows(p);
@@ -588,7 +581,7 @@ uint32_t instruction(int32_t format_a, int32_t format_b, bool bmn) {
 }
 
 template <bool BMN, bool WG>
-int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
+int run_parts(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
     cudaStream_t s = current_stream();
     const int64_t nt = (p.n + BN - 1) / BN, nb = (p.n + 127) / 128;
     const int64_t mt = WG ? (p.rows + TM - 1) / TM : row_tiles(p.rows, p.groups, p.offsets != nullptr, TM);
@@ -612,7 +605,7 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t f
         CHELIS_TRY(make_scale_map(&msa, scratch, a_atoms, 1));
         CHELIS_TRY(make_scale_map(&msb, sfb, b_atoms, 2));
         q.tma_out = p.n * experts::width(p.out_dtype) % 16 == 0 && experts::aligned16(p.out);
-        if (q.tma_out) CHELIS_TRY(make_out_map(&mo, p.out, p.out_dtype, p.n, p.rows, WG ? p.groups : 1));
+        if (q.tma_out) CHELIS_TRY(make_out_map(&mo, p.out, p.out_dtype, p.n, p.rows, (WG ? p.groups : 1) * p.parts));
         pack_scales_kernel<WG><<<blocks8::grid_for((a_atoms + b_atoms + 7) / 8, 8), PACK_THREADS, 0, s>>>(
             q.p, q.quads, q.m_atoms, static_cast<uint4 *>(scratch), reinterpret_cast<uint4 *>(sfb));
         g_launches++;
@@ -620,7 +613,7 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t f
         auto kernel = scaled8_kernel<BMN, WG>;
         CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    PAIR_SMEM), "cudaFuncSetAttribute"));
-        const int64_t most = (WG ? p.groups : 1) * mt * nt;
+        const int64_t most = (WG ? p.groups : 1) * mt * nt * p.parts;
         const int64_t workers = sm_count() / 2;
         const int64_t used = most < workers ? (most < 1 ? 1 : most) : workers;
         cudaLaunchConfig_t cfg{};
@@ -645,6 +638,15 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t f
     const int rc = body();
     scratch_free(scratch, s);
     return rc;
+}
+template <bool BMN, bool WG>
+int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
+    const int64_t tiles = (WG ? p.groups * row_tiles(p.rows, 0, false, TM)
+                              : row_tiles(p.rows, p.groups, p.offsets != nullptr, TM)) * ((p.n + BN - 1) / BN);
+    const int32_t parts = part_count(tiles, WG ? p.kblocks / p.groups : p.kblocks, sm_count() / 2, QUAD,
+                                     2 * SAVED_BLOCKS);  // a block takes half as long here
+    return in_parts(p, parts, WG ? p.groups : 1,
+                    [&](const Params &q) { return run_parts<BMN, WG>(ma, mb, q, fa, fb); });
 }
 
 }  // namespace scaled8

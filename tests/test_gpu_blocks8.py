@@ -300,6 +300,53 @@ def test_matmul8_wgrad_large(cuda, counts, n, k, dtype):
     cuda.device_status()
 
 
+# Few tiles and long contractions, which are cut into parts: both kernels, last parts that are
+# short, experts without rows, rows that no expert holds, results off 16 bytes.
+@pytest.mark.parametrize("trans_b", [True, False])
+@pytest.mark.parametrize("rows,n,k,counts,any_scales,dtype", [
+    (100, 300, 2600, None, False, "bf16"), (129, 40, 1400, None, True, "f32"), (70, 517, 4000, None, False, "f16"),
+    (95, 129, 2100, [50, 0, 40], False, "f16"), (300, 1000, 19200, None, False, "f32"),
+    (287, 1001, 9500, [100, 0, 180], False, "bf16")])
+def test_matmul8_in_parts(cuda, rows, n, k, counts, any_scales, dtype, trans_b):
+    import torch
+    rng = np.random.default_rng(rows + n + k)
+    a8, b8, va, vb = _operands(cuda, rng, rows, n, k, None if counts is None else len(counts), trans_b, "e4m3", "e5m2")
+    off = None if counts is None else _offsets(counts)
+    y = cuda.matmul8(a8, b8, trans_b, off, _dtype(dtype), any_scales=any_scales)
+    at = 0
+    for e, c in enumerate([rows] if counts is None else counts):
+        w = vb if counts is None else vb[e]
+        _near(y[at:at + c], va[at:at + c] @ w, np.abs(va[at:at + c]) @ np.abs(w), k, dtype)
+        at += c
+    assert not y[at:].any()
+    assert torch.equal(y, cuda.matmul8(a8, b8, trans_b, off, _dtype(dtype), any_scales=any_scales))
+    cuda.device_status()
+
+
+@pytest.mark.parametrize("counts,n,k,any_scales,dtype", [
+    ([9001], 77, 263, False, "f32"), ([3000, 0, 130, 5000, 1], 100, 300, False, "bf16"), ([2600], 128, 256, True, "f16"),
+    ([60000], 520, 600, False, "f32"), ([40000, 0, 15000, 1], 301, 520, False, "f16")])
+def test_matmul8_wgrad_in_parts(cuda, counts, n, k, any_scales, dtype):
+    import torch
+    rng = np.random.default_rng(n + k)
+    rows = sum(counts)
+    dy, _ = _input(rng, (rows, n), "f32")
+    x, _ = _input(rng, (rows, k), "f32")
+    off = _offsets(counts) if len(counts) > 1 else None
+    a8, b8 = cuda.quantize8_transposed(dy, "e5m2", off), cuda.quantize8_transposed(x, "e4m3", off)
+    va = R.values(_values(a8.data), a8.scales.cpu().double().numpy().T, 1)
+    vb = R.values(_values(b8.data), b8.scales.cpu().double().numpy().T, 1)
+    got = cuda.matmul8_wgrad(a8, b8, off, _dtype(dtype), any_scales=any_scales)
+    at = 0
+    for e, c in enumerate(counts):
+        end = at + -(-c // 128) * 128
+        _near(got[e] if off is not None else got, va[:, at:end] @ vb[:, at:end].T,
+              np.abs(va[:, at:end]) @ np.abs(vb[:, at:end]).T, c, dtype)
+        at = end
+    assert torch.equal(got, cuda.matmul8_wgrad(a8, b8, off, _dtype(dtype), any_scales=any_scales))
+    cuda.device_status()
+
+
 def test_matmul8_reports_scales_that_are_no_powers_of_two(cuda):
     """Where the tensor core applies the scales it takes powers of two; another
     one makes the numbers under it NaN, is reported, and any_scales admits it."""
