@@ -51,7 +51,7 @@ constexpr int FOLD_WARPS = 8;
 constexpr int THREADS = 128 + 32 * FOLD_WARPS;
 // Registers: a launch of 384 threads at 168 gives the first warpgroup's share
 // to the fold (128 x 56 + 256 x 224 = 384 x 168), which keeps 128 sums and
-// two 32-column loads of tensor memory in flight.
+// two 16-column loads of tensor memory in flight.
 constexpr int LAUNCH_REGS = 168, FEW_REGS = 56, FOLD_REGS = 224;
 static_assert(128 * FEW_REGS + 32 * FOLD_WARPS * FOLD_REGS <= THREADS * LAUNCH_REGS, "register split");
 constexpr uint32_t ACC_COLS = 256, TMEM_COLS = 512;
@@ -683,24 +683,24 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const f32x2 s2 = pack2(s, s);
                 const float4 *cs = reinterpret_cast<const float4 *>(slot + BM + half * 128);
                 const uint32_t acc = tmem_base + lanes + static_cast<uint32_t>(b) * ACC_COLS + half * 128;
-                // 32 columns are added while the next 32 load
-                uint32_t r[2][32];
-                tmem_ld_32x32b_x32(acc, r[0]);
+                // 16 columns are added while the next 16 load
+                uint32_t r[2][16];
+                tmem_ld_32x32b_x16(acc, r[0]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 8; ++j) {
                     tmem_wait_ld();
-                    if (j < 3) tmem_ld_32x32b_x32(acc + (j + 1) * 32, r[(j + 1) & 1]);
+                    if (j < 7) tmem_ld_32x32b_x16(acc + (j + 1) * 16, r[(j + 1) & 1]);
                     else release();  // the accumulator has been read: the next block may have it
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
+                    for (int c = 0; c < 16; c += 4) {
                         f32x2 v0 = pack2(__uint_as_float(r[j & 1][c]), __uint_as_float(r[j & 1][c + 1]));
                         f32x2 v1 = pack2(__uint_as_float(r[j & 1][c + 2]), __uint_as_float(r[j & 1][c + 3]));
                         if (WG) {
-                            const float4 w = cs[j * 8 + c / 4];
+                            const float4 w = cs[j * 4 + c / 4];
                             v0 = mul2(v0, pack2(w.x, w.y));
                             v1 = mul2(v1, pack2(w.z, w.w));
                         }
-                        const int o = j * 16 + c / 2;
+                        const int o = j * 8 + c / 2;
                         run[o] = fma2(v0, s2, run[o]);
                         run[o + 1] = fma2(v1, s2, run[o + 1]);
                     }
