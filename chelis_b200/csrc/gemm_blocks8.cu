@@ -366,8 +366,8 @@ __device__ __forceinline__ void store_boxes(const f32x2 (&run)[64], int32_t dtyp
 // from each thread's registers, a sector at a time; others through the warp's
 // box, so that neighbouring lanes write neighbouring units.  One element at
 // a time from the registers touched 32 sectors a store: 8941 x 3329 x 144 by
-// 11 experts to f16 336 us, so 55; 20930 x 263 x 135 by 19 112 and 26; up to 2
-// us are lost where a tile has a few rows alone.
+// 11 experts to f16 334 us, so 46; 20930 x 263 x 135 by 19 115 and 20; up to
+// 1.2 us are lost where a tile has a few rows alone.
 __device__ __forceinline__ void store_rows(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
                                            int64_t index, int rows, int64_t left) {
     const int w = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
