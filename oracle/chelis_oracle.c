@@ -27,7 +27,8 @@
 #include <string.h>
 
 /* Correctly rounded kernels from the reference's vendored CORE-MATH
- * (crates/chelis-crmath/csrc/crmath_ffi.c:15-45), linked from oracle/_ref. */
+ * (crates/chelis-crmath/csrc/crmath_ffi.c:15-45), linked from oracle/_ref, or
+ * from rounded_math.c where the reference tree is not here. */
 float chelis_crmath_ffi_expf(float);
 float chelis_crmath_ffi_logf(float);
 float chelis_crmath_ffi_erfcf(float);

@@ -29,8 +29,8 @@ _u64 = ctypes.c_uint64
 
 
 def build() -> None:
-    """Compile liborc.so (and the reference CORE-MATH shim when the reference
-    tree is present) with oracle/Makefile."""
+    """Compile liborc.so and the correctly rounded functions that it links
+    (the reference's CORE-MATH when it is present) with oracle/Makefile."""
     subprocess.run(["make", "-s", "-C", _HERE], check=True)
 
 
