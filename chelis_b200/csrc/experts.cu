@@ -310,9 +310,12 @@ __global__ void __launch_bounds__(SCAN_THREADS)
     }
 }
 
+// `counts` is still being written while this kernel's first part runs, so it is
+// neither const nor __restrict__: as such its loads could take the read-only
+// path or be moved above the wait.
 __global__ void __launch_bounds__(SORT_THREADS)
     sort_place_kernel(const int32_t *__restrict__ ids, int64_t n, int experts,
-                      const int32_t *__restrict__ counts, int scanned, int32_t *__restrict__ offsets,
+                      int32_t *counts, int scanned, int32_t *__restrict__ offsets,
                       int32_t *__restrict__ position, int32_t *__restrict__ source) {
     extern __shared__ int sort_smem[];
     int *next = sort_smem;                      // [SORT_WARPS][experts]: a warp's next place
@@ -754,7 +757,7 @@ extern "C" int chelis_cuda_expert_sort(const int32_t *ids, int64_t tokens, int32
     cfg.attrs = &early;
     cfg.numAttrs = segments > 1 && segments <= 64 ? 1 : 0;
     const int rc = check_cuda(cudaLaunchKernelEx(&cfg, experts::sort_place_kernel, ids, n, static_cast<int>(n_experts),
-                                                 static_cast<const int32_t *>(counts), static_cast<int>(scanned),
+                                                 static_cast<int32_t *>(counts), static_cast<int>(scanned),
                                                  offsets, position, source),
                               "experts::sort_place_kernel");
     g_launches++;
