@@ -17,6 +17,7 @@
 //   warp 0      TMA producer
 //   warp 1      TMEM allocator + tcgen05.mma kind::f8f6f4 issuer
 //   warp 2      the blocks' scales into a ring of their own (cp.async)
+//   warp 3      looks at them: not admitted or far from 1?
 //   warps 4-11  fold: a block's sum in tensor memory times its scales into
 //               f32 registers, then the store
 // The scales differ from block to block, so the tensor core sums one block
@@ -25,7 +26,11 @@
 // block runs.  The round trip between the two, about twice a block's 512
 // clocks of MMAs, is what bounds it; gemm_scaled8.cu has none.
 // Scales that are powers of two come here too where the product is too small
-// for that kernel's second launch (see gemm_scaled8.cu's entries).
+// for that kernel's second launch (see gemm_scaled8.cu's entries).  Without
+// any_scales another scale is made NaN and reported.  The fold multiplies the
+// two scales, or one of them and the sum, first; where a block has one so far
+// from 1 that this may leave f32 although the result does not, it takes them by
+// halves of their exponents.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,9 +55,10 @@ constexpr int SLOT_FLOATS = BM + BN;  // row scales, then column scales (or one 
 constexpr int FOLD_WARPS = 8;
 constexpr int THREADS = 128 + 32 * FOLD_WARPS;
 // Registers: a launch of 384 threads at 168 gives the first warpgroup's share
-// to the fold (128 x 56 + 256 x 224 = 384 x 168), which keeps 128 sums and
-// two 16-column loads of tensor memory in flight.
-constexpr int LAUNCH_REGS = 168, FEW_REGS = 56, FOLD_REGS = 224;
+// to the fold (128 x 40 + 256 x 232 = 384 x 168), which keeps 128 sums and
+// two 16-column loads of tensor memory in flight.  With 56 and 224 the fold
+// spilled in its loop (8192 x 4096 x 1024 with any scales 71 us against 60).
+constexpr int LAUNCH_REGS = 168, FEW_REGS = 40, FOLD_REGS = 232;
 static_assert(128 * FEW_REGS + 32 * FOLD_WARPS * FOLD_REGS <= THREADS * LAUNCH_REGS, "register split");
 constexpr uint32_t ACC_COLS = 256, TMEM_COLS = 512;
 constexpr int MAX_GROUPS = experts::MAX_EXPERTS;
@@ -73,8 +79,45 @@ struct Params {
     void *out;
     int32_t out_dtype;
     int32_t parts;       // of the contraction, each with a result of its own (part_sums)
+    int32_t any_scales;  // admit scales that are no powers of two
     uint32_t idesc;
 };
+
+// ---- scales ---------------------------------------------------------------
+// A normal power of two, what a product takes without any_scales.
+__device__ __forceinline__ bool power_of_two(uint32_t bits) {
+    return (bits & 0x7fffffu) == 0 && bits - (1u << 23) < (254u << 23);
+}
+// Magnitude from 2^-60 to 2^60: a block's sum (below 2^39) times two of them
+// leaves f32 only where the result does, in any order.  look() gathers scales,
+// odd() says whether one of them is further off or not admitted.
+constexpr uint32_t NEAR_LOW = 67u << 23, NEAR_SPAN = 120u << 23;
+__device__ __forceinline__ void look(float scale, uint32_t *span, uint32_t *bits) {
+    const uint32_t b = __float_as_uint(scale);
+    *span = max(*span, 2 * b - 2 * NEAR_LOW);  // without the sign
+    *bits |= b;
+}
+__device__ __forceinline__ bool odd(uint32_t span, uint32_t bits, bool any) {
+    return span > 2 * NEAR_SPAN || (!any && (bits & 0x807fffffu) != 0);
+}
+// NaN for a scale that is not admitted.
+__device__ __forceinline__ float admitted(float scale, bool any) {
+    return any || power_of_two(__float_as_uint(scale)) ? scale : __int_as_float(0x7fc00000);
+}
+// v s w where a scale is far from 1: each as two factors of half its exponent
+// (exact, the first a power of two), multiplied in an order in which nothing
+// leaves f32 that is not on its way out: no factor is infinite, and the
+// magnitude moves one way once s1 w1 is in.
+struct Halves {
+    float one, two;
+};
+__device__ __forceinline__ Halves halves(float scale) {
+    const uint32_t h = (__float_as_uint(scale) >> 24 & 0x7fu) + 63u;  // half the exponent, in [2^-64, 2^63]
+    return {__uint_as_float(h << 23), scale * __uint_as_float((254u - h) << 23)};
+}
+__device__ __forceinline__ float scaled(float v, const Halves &s, const Halves &w) {
+    return v * (s.one * w.one) * s.two * w.two;
+}
 
 __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -85,11 +128,9 @@ __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 4 bytes from global to shared memory, zero when !ok.
-__device__ __forceinline__ void cp_async4(float *dst, const float *src, bool ok) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
-                 "r"(ok ? 4 : 0)
-                 : "memory");
+// 4 bytes from global to shared memory.
+__device__ __forceinline__ void cp_async4(float *dst, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 // Arrive once this thread's cp.async so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
@@ -484,6 +525,45 @@ __device__ __forceinline__ void landed(uint64_t *bar, uint32_t parity, uint32_t 
         if (mbar_try_wait(bar, parity)) return;
 }
 
+// One block's scales, by one warp, before the fold sees them: true where one is
+// far from 1.  Those that are not admitted become NaN and are reported, where
+// `rows` and `cols` have them in the result (what lies past its end repeats the
+// last).  The usual block takes few instructions, as the fold needs the issue
+// slots: the weight gradient of 2048 rows by 8 experts of 1024 x 1024 takes 23.4
+// us with this and the fold's branch, 20.9 without.
+template <bool WG>
+__device__ __forceinline__ bool check_scales(float *slot, int lane, int rows, int cols, bool any) {
+    uint32_t span = 0, bits = 0;
+    auto look4 = [&](int at) {
+        const float4 v = *reinterpret_cast<const float4 *>(slot + at + 4 * lane);
+        look(v.x, &span, &bits);
+        look(v.y, &span, &bits);
+        look(v.z, &span, &bits);
+        look(v.w, &span, &bits);
+    };
+    look4(0);
+    if (WG) {
+        look4(BM);
+        look4(BM + 128);
+    } else {
+        look(slot[BM + (cols > 128 ? lane & 1 : 0)], &span, &bits);
+    }
+    if (!__any_sync(0xffffffffu, odd(span, bits, any))) return false;
+    if (!any) {
+        bool bad = false;
+        auto look_again = [&](float *at) {
+            if (!power_of_two(__float_as_uint(*at))) {
+                bad = true;
+                *at = __int_as_float(0x7fc00000);
+            }
+        };
+        for (int i = lane; i < min(rows, BM); i += 32) look_again(slot + i);
+        for (int i = lane; i < (WG ? min(cols, BN) : (cols > 128 ? 2 : 1)); i += 32) look_again(slot + BM + i);
+        if (bad) report_device_error(DEVERR_SCALE);
+    }
+    return true;
+}
+
 // BMN: b is read with its rows along the contraction (the input gradient).
 // WG: the weight gradient (groups along the contraction, scales on both sides).
 template <bool BMN, bool WG>
@@ -499,9 +579,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *acc_empty = acc_full + 2;   // [2]
     uint64_t *scale_full = acc_empty + 2;
     uint64_t *scale_empty = scale_full + SCALE_SLOTS;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_empty + SCALE_SLOTS);
+    uint64_t *scale_landed = scale_empty + SCALE_SLOTS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_landed + SCALE_SLOTS);
     volatile uint32_t *abort_flag = tmem_slot + 1;
     volatile int32_t *consumed = reinterpret_cast<volatile int32_t *>(tmem_slot + 2);
+    uint32_t *far = tmem_slot + 3;  // [SCALE_SLOTS]: a scale of the block is far from 1 or not admitted
     float *scales = reinterpret_cast<float *>(smem + RING_BYTES + 512);
     unsigned char *out_stage = reinterpret_cast<unsigned char *>(scales + SCALE_SLOTS * SLOT_FLOATS);
     int32_t *start = reinterpret_cast<int32_t *>(out_stage + FOLD_WARPS * OUT_BOX);
@@ -518,7 +600,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&acc_empty[b], FOLD_WARPS);
         }
         for (int q = 0; q < SCALE_SLOTS; ++q) {
-            mbar_init(&scale_full[q], 32);
+            mbar_init(&scale_landed[q], 32);
+            mbar_init(&scale_full[q], 1);
             mbar_init(&scale_empty[q], FOLD_WARPS);
         }
         *abort_flag = 0;
@@ -628,23 +711,38 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int u = 0; u < BM / 32; ++u) {
                         const int64_t row = t.m0 + u * 32 + lane;
-                        cp_async4(slot + u * 32 + lane, p.sa + kb * p.rows + (row < p.rows ? row : 0),
-                                  row < p.rows);
+                        cp_async4(slot + u * 32 + lane, p.sa + kb * p.rows + (row < p.rows ? row : p.rows - 1));
                     }
                     if (WG) {
 #pragma unroll
                         for (int u = 0; u < BN / 32; ++u) {
                             const int64_t c = t.n0 + u * 32 + lane;
-                            cp_async4(slot + BM + u * 32 + lane, p.sb + kb * p.n + (c < p.n ? c : 0), c < p.n);
+                            cp_async4(slot + BM + u * 32 + lane, p.sb + kb * p.n + (c < p.n ? c : p.n - 1));
                         }
-                    } else if (lane < 2) {
-                        const bool in = t.n0 + lane * 128 < p.n;
-                        cp_async4(slot + BM + lane, in ? tile_sb + lane * p.sb_n + kb * p.sb_k : p.sb, in);
+                    } else if (lane < 2 && t.n0 + lane * 128 < p.n) {
+                        cp_async4(slot + BM + lane, tile_sb + lane * p.sb_n + kb * p.sb_k);
                     }
-                    cp_async_arrive(&scale_full[q]);
+                    cp_async_arrive(&scale_landed[q]);
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            // ---------------- check of the scales ----------------
+            int32_t it = 0;
+            bool ok = true;
+            for (int L = first; ok && L < tiles; L += step) {
+                const Tile t = tile_at<WG, BM, 1>(p, start, L);
+                const int rows = t.m_end - t.m0, cols = static_cast<int>(p.n) - t.n0;
+                for (int i = 0; i < t.kbs; ++i, ++it) {
+                    const int q = it % SCALE_SLOTS;
+                    ok = all(wait(&scale_landed[q], (it / SCALE_SLOTS) & 1, tries, abort_flag, DEVERR_TIMEOUT_PRODUCER));
+                    if (!ok) break;
+                    const bool distant = check_scales<WG>(scales + q * SLOT_FLOATS, lane, rows, cols, p.any_scales != 0);
+                    if (lane == 0) far[q] = distant;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&scale_full[q]);
+                }
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FOLD_REGS));
@@ -679,10 +777,31 @@ __global__ void __launch_bounds__(THREADS, 1)
                     continue;
                 }
                 float s = slot[quad * 32 + lane];
-                if (!WG) s *= slot[BM + half];
-                const f32x2 s2 = pack2(s, s);
                 const float4 *cs = reinterpret_cast<const float4 *>(slot + BM + half * 128);
                 const uint32_t acc = tmem_base + lanes + static_cast<uint32_t>(b) * ACC_COLS + half * 128;
+                if (far[q]) {  // unrolled like the usual fold: it must leave the sums in their registers
+                    const Halves hs = halves(s), hw = halves(WG ? 1.0f : slot[BM + half]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t r[16];
+                        tmem_ld_32x32b_x16(acc + j * 16, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 16; c += 4) {
+                            const float4 w = WG ? cs[j * 4 + c / 4] : float4{};
+                            const int o = j * 8 + c / 2;
+                            run[o] = add2(run[o], pack2(scaled(__uint_as_float(r[c]), hs, WG ? halves(w.x) : hw),
+                                                        scaled(__uint_as_float(r[c + 1]), hs, WG ? halves(w.y) : hw)));
+                            run[o + 1] = add2(run[o + 1], pack2(scaled(__uint_as_float(r[c + 2]), hs, WG ? halves(w.z) : hw),
+                                                                scaled(__uint_as_float(r[c + 3]), hs, WG ? halves(w.w) : hw)));
+                        }
+                    }
+                    release();
+                    if (lane == 0) mbar_arrive(&scale_empty[q]);
+                    continue;
+                }
+                if (!WG) s *= slot[BM + half];
+                const f32x2 s2 = pack2(s, s);
                 // 16 columns are added while the next 16 load
                 uint32_t r[2][16];
                 tmem_ld_32x32b_x16(acc, r[0]);

@@ -39,6 +39,8 @@ namespace scaled8 {
 using namespace gemm8;
 
 constexpr uint64_t DRAIN_NS = 200000;     // bounded drain of an aborted pair's second block
+constexpr int PAIR_FEW_REGS = 56, PAIR_FOLD_REGS = 224;  // 128 x 56 + 256 x 224 = 384 x 168
+static_assert(128 * PAIR_FEW_REGS + 32 * FOLD_WARPS * PAIR_FOLD_REGS <= THREADS * LAUNCH_REGS, "register split");
 constexpr int CHUNK = 32;
 constexpr int QUAD = 4;                   // blocks of K in one packed scale word
 constexpr int SF_BYTES = 512;             // packed scales of 128 rows, four blocks
@@ -66,10 +68,7 @@ struct Params8 {
 
 // ---- scales ---------------------------------------------------------------
 // The exponent byte of a power of two, NaN (0xff) for anything else.
-__device__ __forceinline__ uint32_t exponent_byte(uint32_t bits) {
-    const uint32_t e = bits >> 23;
-    return (bits & 0x7fffffu) != 0 || e == 0 || e >= 255 ? 0xffu : e;
-}
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t bits) { return power_of_two(bits) ? bits >> 23 : 0xffu; }
 
 constexpr int PACK_THREADS = 256;
 
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     int32_t issued = 0;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PAIR_FEW_REGS));
         if (warp == 0) {
             // ---------------- TMA producer ----------------
             int stage = 0;
@@ -466,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) *consumed = it;
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FOLD_REGS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PAIR_FOLD_REGS));
         // ---------------- fold and store ----------------
         const int quad = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
@@ -689,6 +688,7 @@ extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans
     p.sb_k = trans_b ? 1 : nblocks;
     p.out = out;
     p.out_dtype = out_dtype;
+    p.any_scales = any_scales != 0;
     // Few rows for each matrix (measured at 1024 x 4096 weights, rotated through
     // memory; few8 against gemm8, us): one matrix, 1 row 3.1 and 10.1, 64 rows
     // 9.0 and 10.7, 128 rows 15 and 11; 64 matrices, 8 rows 7.4 and 11; 8
@@ -736,6 +736,7 @@ extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int
     p.sb = scales_b;
     p.out = out;
     p.out_dtype = out_dtype;
+    p.any_scales = any_scales != 0;
     const int64_t each = (p.kblocks + groups - 1) / groups;  // blocks of a group, about
     if (any_scales || small(groups * ((n + 127) / 128) * ((k + 255) / 256) * each))
         return gemm8::run<false, true>(ma, mb, p, format_a, format_b);

@@ -764,7 +764,8 @@ def matmul8(a: Blocks8, b: Blocks8, trans_b: bool = True, offsets: torch.Tensor 
     b is a stack of matrices and rows [offsets[e], offsets[e + 1]) meet matrix
     e; rows that no expert holds come out as zeros.  Scales are powers of two,
     as quantize8 makes them (others give NaN and raise at the next
-    device_status()); any_scales admits every scale, at a lower rate."""
+    device_status(), whatever the size); any_scales admits every scale, at a
+    lower rate."""
     if dtype not in _ACT:
         raise ValueError("matmul8 gives f32, bf16 or f16")
     _check_blocks8("matmul8", a, "rows")

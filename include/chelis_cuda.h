@@ -665,10 +665,12 @@ int chelis_cuda_quantize8_transposed(int32_t dtype, int32_t format, const void *
  * [groups][k][n]): a in rows layout, b in tiles layout, f32 sums rounded once
  * to out_dtype.  Row r meets the matrix of the group that holds it; offsets
  * == NULL: one matrix.  Rows that no group holds are written as zeros.
- * any_scales == 0: the scales are powers of two, as quantize8 makes them, and
- * the tensor core applies them; another scale makes the numbers under it NaN
- * and is reported by chelis_cuda_device_status.  any_scales != 0 admits every
- * f32 scale, at a lower rate. */
+ * any_scales == 0: the scales are powers of two (2^-126 .. 2^127), as quantize8
+ * makes them, and in large products the tensor core applies them; whatever the
+ * size, another scale makes the numbers under it NaN and is reported by
+ * chelis_cuda_device_status.  any_scales != 0 admits every f32 scale, at a lower
+ * rate.  Scales far from 1 lose nothing either way: a result is off only where
+ * it leaves f32 itself. */
 int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows, int64_t n,
                         int64_t k, const uint8_t *a, const float *scales_a, const uint8_t *b,
                         const float *scales_b, const int32_t *offsets, int32_t groups,
