@@ -29,6 +29,7 @@ class Saved(NamedTuple):
     order: ops.ExpertOrder
     h: torch.Tensor   # before gelu
     ys: torch.Tensor  # the experts' rows
+    renormalize: bool = True
 
 
 def feed_forward(x: torch.Tensor, router: torch.Tensor, w1: ops.Blocks8, w2: ops.Blocks8, k: int,
@@ -41,12 +42,15 @@ def feed_forward(x: torch.Tensor, router: torch.Tensor, w1: ops.Blocks8, w2: ops
     h = ops.matmul8(x8, w1, offsets=order.offsets, dtype=torch.float32)
     ys = ops.matmul8(ops.quantize8(ops.gelu(h)), w2, offsets=order.offsets, dtype=torch.float32)
     y = ops.expert_combine(ys, weights, order)
-    return y, Saved(x, logits, weights, chosen, order, h, ys)
+    return y, Saved(x, logits, weights, chosen, order, h, ys, bool(renormalize))
 
 
 def feed_forward_bwd(dy: torch.Tensor, s: Saved, router: torch.Tensor, w1: ops.Blocks8,
-                     w2: ops.Blocks8, renormalize: bool = True) -> dict:
-    """The gradients of feed_forward: dx, drouter, dw1, dw2 (all f32)."""
+                     w2: ops.Blocks8, renormalize: bool | None = None) -> dict:
+    """The gradients of feed_forward: dx, drouter, dw1, dw2 (all f32).
+    renormalize is the forward pass's, which s keeps; another one is refused."""
+    if renormalize is not None and bool(renormalize) != s.renormalize:
+        raise ValueError("feed_forward_bwd: renormalize is not the forward pass's")
     off = s.order.offsets
     dys, dweights = ops.expert_combine_bwd(dy, s.ys, s.weights, s.order)
     da = ops.matmul8(ops.quantize8(dys, "e5m2"), w2, trans_b=False, offsets=off, dtype=torch.float32)
@@ -56,7 +60,7 @@ def feed_forward_bwd(dy: torch.Tensor, s: Saved, router: torch.Tensor, w1: ops.B
     dxs = ops.matmul8(ops.quantize8(dh, "e5m2"), w1, trans_b=False, offsets=off, dtype=torch.float32)
     dw1 = ops.matmul8_wgrad(ops.quantize8_transposed(dh, "e5m2", off),
                             ops.quantize8_transposed(ops.expert_gather(s.x, s.order), "e4m3", off), off)
-    dlogits = ops.expert_route_bwd(s.logits, s.experts, dweights, renormalize)
+    dlogits = ops.expert_route_bwd(s.logits, s.experts, dweights, s.renormalize)
     dx = ops.fused_elementwise(_ADD, [ops.expert_gather_bwd(dxs, s.order),
                                       ops.matmul(dlogits, router, trans_b=True)])
     return {"dx": dx, "drouter": ops.matmul(s.x, dlogits, trans_a=True), "dw1": dw1, "dw2": dw2}
