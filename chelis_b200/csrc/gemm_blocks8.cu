@@ -26,7 +26,7 @@
 // block runs.  The round trip between the two, about twice a block's 512
 // clocks of MMAs, is what bounds it; gemm_scaled8.cu has none.
 // Scales that are powers of two come here too where the product is too small
-// for that kernel's second launch (see gemm_scaled8.cu's entries).  Without
+// for that kernel's second launch (see gemm_scaled8.cu's one_by_one).  Without
 // any_scales another scale is made NaN and reported.  The fold multiplies the
 // two scales, or one of them and the sum, first; where a block has one so far
 // from 1 that this may leave f32 although the result does not, it takes them by
@@ -37,6 +37,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -938,6 +939,36 @@ int in_parts(Params p, int32_t parts, int64_t matrices, F f) {
     return rc;
 }
 
+// Tiles at most, and the parts that they are cut into.
+template <bool WG>
+int64_t tiles_of(const Params &p) {
+    return (WG ? p.groups * row_tiles(p.rows, 0, false, BM) : row_tiles(p.rows, p.groups, p.offsets != nullptr, BM)) *
+           ((p.n + BN - 1) / BN);
+}
+template <bool WG>
+int32_t parts_of(const Params &p) {
+    return part_count(tiles_of<WG>(p), WG ? p.kblocks / p.groups : p.kblocks, sm_count(), PART_BLOCKS, SAVED_BLOCKS);
+}
+// Experts that have rows, about: as many as rows dealt out at random reach.
+inline double used_groups(const Params &p) {
+    return p.offsets ? -p.groups * std::expm1(-static_cast<double>(p.rows) / p.groups) : 1.0;
+}
+// The tiles of `high` rows that each of `workers` goes through one after another,
+// about: an expert's rows end half a tile early on average, but each has a tile.
+template <bool WG>
+int64_t rounds(const Params &p, int64_t high, int64_t workers) {
+    double tiles = static_cast<double>((p.rows + high - 1) / high);
+    if (WG) tiles *= p.groups;
+    else if (p.offsets) tiles = std::fmax(static_cast<double>(p.rows) / high + 0.5 * used_groups(p), std::ceil(used_groups(p)));
+    return static_cast<int64_t>(std::ceil(tiles * static_cast<double>((p.n + BN - 1) / BN) / workers));
+}
+// gemm8_kernel's time for a layer product or an input gradient, about (us).
+inline double forward_us(const Params &p, int64_t *serial) {
+    const int64_t parts = parts_of<false>(p);
+    *serial = rounds<false>(p, BM, sm_count()) * ((p.kblocks + parts - 1) / parts);
+    return 6.0 + 0.62 * *serial + (parts > 1 ? 3.5 : 0.0);
+}
+
 template <bool BMN, bool WG>
 int run(const CUtensorMap &ma, const CUtensorMap &mb, Params p, int32_t fa, int32_t fb) {
     p.idesc = (1u << 4) |                                    // f32 sums
@@ -945,15 +976,12 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, Params p, int32_t fa, int3
               (fb == CHELIS_FORMAT_E5M2 ? 1u << 10 : 0u) |
               (BMN ? 1u << 16 : 0u) |                        // b MN-major
               (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);
-    const int64_t nt = (p.n + BN - 1) / BN;
-    const int64_t most = (WG ? p.groups * row_tiles(p.rows, 0, false, BM)
-                             : row_tiles(p.rows, p.groups, p.offsets != nullptr, BM)) * nt;
+    const int64_t most = tiles_of<WG>(p);
     auto kernel = gemm8_kernel<BMN, WG>;
     CHELIS_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
                           "cudaFuncSetAttribute"));
     const int64_t sms = sm_count();
-    const int32_t parts = part_count(most, WG ? p.kblocks / p.groups : p.kblocks, sms, PART_BLOCKS,
-                                     SAVED_BLOCKS);
+    const int32_t parts = parts_of<WG>(p);
     return in_parts(p, parts, WG ? p.groups : 1, [&](const Params &q) -> int {
         const int64_t grid = parts * most < sms ? parts * most : sms;
         kernel<<<static_cast<unsigned>(grid), THREADS, SMEM_BYTES, current_stream()>>>(ma, mb, q);

@@ -638,13 +638,16 @@ int run_parts(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int
     scratch_free(scratch, s);
     return rc;
 }
-template <bool BMN, bool WG>
-int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
+template <bool WG>
+int32_t pair_parts_of(const Params &p) {
     const int64_t tiles = (WG ? p.groups * row_tiles(p.rows, 0, false, TM)
                               : row_tiles(p.rows, p.groups, p.offsets != nullptr, TM)) * ((p.n + BN - 1) / BN);
-    const int32_t parts = part_count(tiles, WG ? p.kblocks / p.groups : p.kblocks, sm_count() / 2, QUAD,
-                                     2 * SAVED_BLOCKS);  // a block takes half as long here
-    return in_parts(p, parts, WG ? p.groups : 1,
+    return part_count(tiles, WG ? p.kblocks / p.groups : p.kblocks, sm_count() / 2, QUAD,
+                      2 * SAVED_BLOCKS);  // a block takes half as long here
+}
+template <bool BMN, bool WG>
+int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t fa, int32_t fb) {
+    return in_parts(p, pair_parts_of<WG>(p), WG ? p.groups : 1,
                     [&](const Params &q) { return run_parts<BMN, WG>(ma, mb, q, fa, fb); });
 }
 
@@ -654,12 +657,57 @@ int run(const CUtensorMap &ma, const CUtensorMap &mb, const Params &p, int32_t f
 using namespace chelis;
 
 namespace {
-// Too little work (blocks of 128 x 256 x 128) for the launch that packs the
-// scales: gemm8 then takes powers of two as well.  Measured, gemm8 against
-// scaled8, us (blocks a multiprocessor): 4096 x 1024 x 1024 (7) 14.5 and 19.5,
-// 1024 x 4096 x 1024 by 8 experts (14) 23 and 25, 2048 (20) 33 and 28, 16384 x
-// 1024 x 1024 by 64 (41) 55 and 48.
-bool small(int64_t blocks) { return blocks < 12 * static_cast<int64_t>(sm_count()); }
+// The kernel for a product, by what each is estimated to take: few8's time goes
+// with the weights that it reads, once for 8 or 32 rows, gemm8's with the blocks
+// of 128 x 256 x 128 that a multiprocessor goes through one after another, and
+// scaled8's too, at about half as much for a block after a launch more.  The
+// estimates' constants are from runs of all three over sizes and experts, of
+// which (us in a graph, the weights rotated through memory):
+//   few8 and gemm8: 8 rows 1024 x 1024 2.8 and 9.6, 4096 x 4096 8.1 and 13.3,
+//   16384 x 4096 22.8 and 22.5; 32 rows 2048 x 4096 8.7 and 12.4, 8192 x 1024 12.6
+//   and 10.8; 64 rows 1024 x 4096 11.4 and 11.9, 8192 x 512 11.6 and 8.1; 16 rows by
+//   8 experts of 4096 x 1024 12.8 and 13.5, by 64 26.8 and 20.1, of 1024 x 4096 20.1
+//   and 28.8.
+//   gemm8 and scaled8, and called among others, host included: 512 x 1024 x 512
+//   (4 blocks) 8.4, 8.8 and 11.3, 15.2; 2048 x 1024 x 1024 (8) 11.5, 10.2 and 13.5,
+//   15.3; 1024 x 1024 x 2048 (16) 14.8, 12.3 and 20.7, 16.4; 6144 x 1024 x 1024 by 8
+//   experts (16) 21, 15; 4096 x 1024 x 1024 by 64 21.0, 24.2 and 22.7, 27.9.  Weight
+//   gradients: 256 x 256 from 256 rows 10.3, 9.2 and 11.3, 14.7; 1024 x 1024 from
+//   512 13.0, 10.1 and 14.5, 15.0, from 2048 17.5, 13.6 and 23.6, 16.7; 1111 x 179
+//   from 250 by 64 experts 25.5 and 31.3.
+// 128 rows at most for few8, as one expert may hold them all (of 64 of 1024 x
+// 1024: 30 and 12.5).
+bool few_rows(const gemm8::Params &p) {
+    if (p.rows > 128 || p.kblocks > 64) return false;
+    const bool wide = p.rows > 8 * static_cast<int64_t>(p.groups);  // as few8::run takes them
+    const double each = static_cast<double>(p.rows) / p.groups / (wide ? 32 : 8);
+    const double passes = p.offsets ? std::fmax(1.0, each + 0.5) : std::ceil(each);
+    if (passes > 2.0) return false;
+    const double mb = static_cast<double>(p.n) * p.kblocks * 128 / (1 << 20) * gemm8::used_groups(p);
+    const double rate = !wide ? (p.offsets ? 0.26 : 0.33) : (p.kblocks <= 8 ? 1.2 : 0.75);  // us a MB and pass
+    int64_t serial;
+    return passes * (2.0 + rate * mb) < gemm8::forward_us(p, &serial);
+}
+
+// gemm8 for powers of two too: few blocks one after another, or experts with so
+// few rows that a pair's tiles of 256 are mostly empty and its blocks no fewer.
+bool one_by_one(const gemm8::Params &p) {
+    int64_t serial;
+    gemm8::forward_us(p, &serial);
+    return serial <= 8 || (p.offsets && p.rows <= 64 * static_cast<int64_t>(p.groups) &&
+                           2 * gemm8::rounds<false>(p, scaled8::TM, sm_count() / 2) * p.kblocks >= 3 * serial);
+}
+// The same for a weight gradient, whose f32 result costs gemm8 as much as three
+// blocks more a tile and scaled8 a little less, the most where TMA cannot store it.
+bool one_by_one_wgrad(const gemm8::Params &p) {
+    const double blocks = static_cast<double>((p.kblocks + p.groups - 1) / p.groups);
+    const int64_t parts = gemm8::parts_of<true>(p), pair_parts = scaled8::pair_parts_of<true>(p);
+    const double one = parts > 1 ? 7.1 + blocks / parts : gemm8::rounds<true>(p, gemm8::BM, sm_count()) * (blocks + 3.4);
+    const double store = p.n * experts::width(p.out_dtype) % 16 == 0 ? 2.9 : 4.0;
+    const int64_t rounds = gemm8::rounds<true>(p, scaled8::TM, sm_count() / 2);
+    const double pairs = pair_parts > 1 ? 9.3 + 0.25 * blocks / pair_parts : 2.7 + rounds * (0.25 * blocks + store);
+    return one <= pairs;
+}
 }  // namespace
 
 extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans_b, int64_t rows,
@@ -689,19 +737,12 @@ extern "C" int chelis_cuda_matmul8(int32_t format_a, int32_t format_b, int trans
     p.out = out;
     p.out_dtype = out_dtype;
     p.any_scales = any_scales != 0;
-    // Few rows for each matrix (measured at 1024 x 4096 weights, rotated through
-    // memory; few8 against gemm8, us): one matrix, 1 row 3.1 and 10.1, 64 rows
-    // 9.0 and 10.7, 128 rows 15 and 11; 64 matrices, 8 rows 7.4 and 11; 8
-    // matrices, 16 rows 10.4 and 11.6, 64 rows 18 and 13; 32 of 4096 x 1024, 64
-    // rows 32 and 26.
-    if (trans_b && (offsets ? rows <= 2 * static_cast<int64_t>(groups) && kblocks < 32 : rows <= 64))
-        return few8::run(a, b, p, blocks8::round16(k), format_a, format_b);
+    if (trans_b && few_rows(p)) return few8::run(a, b, p, blocks8::round16(k), format_a, format_b);
     CUtensorMap ma, mb;
     CHELIS_TRY(gemm8::make_map(&ma, a, k, blocks8::round16(k), rows, 1, false));
     if (trans_b) CHELIS_TRY(gemm8::make_map(&mb, b, k, blocks8::round16(k), n, groups, true));
     else CHELIS_TRY(gemm8::make_map(&mb, b, n, blocks8::round16(n), k, groups, true));
-    const int64_t tiles = gemm8::row_tiles(rows, groups, offsets != nullptr, 128) * ((n + 255) / 256);
-    if (any_scales || small(tiles * kblocks))
+    if (any_scales || one_by_one(p))
         return trans_b ? gemm8::run<false, false>(ma, mb, p, format_a, format_b)
                        : gemm8::run<true, false>(ma, mb, p, format_a, format_b);
     return trans_b ? scaled8::run<false, false>(ma, mb, p, format_a, format_b)
@@ -737,8 +778,7 @@ extern "C" int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int
     p.out = out;
     p.out_dtype = out_dtype;
     p.any_scales = any_scales != 0;
-    const int64_t each = (p.kblocks + groups - 1) / groups;  // blocks of a group, about
-    if (any_scales || small(groups * ((n + 127) / 128) * ((k + 255) / 256) * each))
+    if (any_scales || one_by_one_wgrad(p))
         return gemm8::run<false, true>(ma, mb, p, format_a, format_b);
     return scaled8::run<false, true>(ma, mb, p, format_a, format_b);
 }

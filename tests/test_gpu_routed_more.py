@@ -254,7 +254,7 @@ def test_weight_gradient_of_integers(cuda, counts, n, k, dtype, launches):
 
 @pytest.mark.parametrize("trans_b", [True, False])
 @pytest.mark.parametrize("rows,n,k,counts,launches", [
-    (129, 40, 1400, None, 2), (70, 517, 4000, None, 2), (95, 129, 2100, [50, 0, 40], 2),
+    (129, 40, 1400, None, 2), (70, 517, 4000, None, 2), (195, 129, 2100, [50, 0, 140], 2),
     (300, 1000, 19200, None, PARTS), (287, 1001, 9500, [100, 0, 180], PARTS)])
 def test_products_of_integers_in_parts(cuda, rows, n, k, counts, launches, trans_b):
     import torch
