@@ -156,6 +156,29 @@ def test_quantise_transposed_by_many_experts(cuda, groups):
     _same(b.scales.cpu().double().numpy(), s.T)
 
 
+def test_quantise_transposed_looks_its_rows_up_at_once(cuda):
+    """1024 experts of 16 rows and one matrix of as many blocks of 128 take the
+    same tiles, and the experts' read an eighth of the data: finding a tile's
+    rows may not cost more than the tile itself."""
+    import torch
+
+    def us(rows, off):
+        x = torch.randn((rows, 1024), device="cuda").bfloat16()
+        cuda.quantize8_transposed(x, "e4m3", off)
+        best = float("inf")
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                cuda.quantize8_transposed(x, "e4m3", off)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 100)
+        return best
+    off = (torch.arange(1025, device="cuda") * 16).int()
+    assert us(16384, off) <= 2 * us((128 + 1024) * 128, None)
+
+
 # --------------------------------------------------- rows there and back
 
 @pytest.mark.parametrize("dtype,hidden", [("f32", 64), ("bf16", 65)])
