@@ -243,7 +243,8 @@ __device__ __forceinline__ void take_part(const Params &p, int part, Tile *t) {
 // Tiles of one group's matrix (mt x nt) in bands of BAND row tiles, column by
 // column within a band: the tiles in flight then share a few panels of a and
 // b in L2 however tall the matrix is (8192^3 by pairs: bands of 4, 8 and 16
-// tiles 425, 435 and 458 us, whole columns 440).
+// tiles 390, 372 and 379 us; 32768 x 1024 x 4096 102, 104 and 102, 16384 x 4096 x
+// 1024 63, 64 and 63).
 constexpr int BAND = 8;
 __device__ __forceinline__ void band_order(int in, int mt, int nt, int *m, int *n) {
     const int band = in / (BAND * nt), first = band * BAND;
@@ -408,8 +409,10 @@ __device__ __forceinline__ void store_boxes(const f32x2 (&run)[64], int32_t dtyp
 // from each thread's registers, a sector at a time; others through the warp's
 // box, so that neighbouring lanes write neighbouring units.  One element at
 // a time from the registers touched 32 sectors a store: 8941 x 3329 x 144 by
-// 11 experts to f16 334 us, so 46; 20930 x 263 x 135 by 19 115 and 20; up to
-// 1.2 us are lost where a tile has a few rows alone.
+// 11 experts to f16 334 us, so 46; 20930 x 263 x 135 by 19 115 and 20.  Tiles of
+// a few rows lose up to 1.2 us by it, and wide f32 results of few blocks more: the
+// weight gradient 2433 x 1747 by 31 experts from 898 rows took 240 us one element
+// at a time and takes 252, 1520 x 2529 by 16 from 4838 118 and 121.
 __device__ __forceinline__ void store_rows(const Params &p, const f32x2 (&run)[64], unsigned char *box, int lane,
                                            int64_t index, int rows, int64_t left) {
     const int w = p.out_dtype == CHELIS_DTYPE_F32 ? 4 : 2;
