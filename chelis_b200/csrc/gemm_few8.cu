@@ -59,9 +59,9 @@ __device__ __forceinline__ float scaled(float v, float s, float w) {
 }
 
 // NT: tokens of one pass over the weights, in eights.
-// Three blocks a multiprocessor with two blocks of K in flight a warp: 10.4 us
-// for 16 rows by 8 matrices of 4096 x 1024 out of memory (3.2 TB/s), against
-// 11.5 us for two with four.  What is left is latency (a strip's loads start
+// Three blocks a multiprocessor with two blocks of K in flight a warp: 9.8 us for
+// 16 rows by 8 matrices of 4096 x 1024 out of memory (3.4 TB/s); two with four
+// took 10 % longer.  What is left is latency (a strip's loads start
 // once its expert's rows are known) and the 8-bit MMA itself, which this
 // machine runs by converting its operands to 16 bits (ALU 36 % busy).
 template <bool E5A, bool E5B, int NT>
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 1)
         // The scales are looked at as they pass, without a branch that would
         // keep the next block's loads behind it; where one is not admitted or
         // far from 1 the strip is done again.  16 rows by 8 matrices of 4096 x
-        // 1024 take 9 % longer for it (looked up before the loop or after it 14 to 18).
+        // 1024 take 7 % longer for it (looked up before the loop or after it 14 to 18).
         uint32_t far = 0, bits = 0;
         auto look = [&](float scale) {
             const uint32_t b = __float_as_uint(scale) & sign;
