@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(PACK_THREADS)
             if (!is_a) {
                 g = quad / quads;
                 quad -= g * quads;
+                if (start[g + 1] == start[g]) continue;  // no rows: nothing reads them
             }
             kb0 = static_cast<int>(quad) * QUAD;
             kbs = p.kblocks - kb0;

@@ -226,6 +226,20 @@ def test_a_scale_that_is_no_power_of_two(cuda, case, side, bad):
     cuda.device_status()
 
 
+@pytest.mark.parametrize("case", [c for c in CASES if c[0] != "dweight" and c[4] and not c[-1]], ids=_id)
+def test_scales_under_no_numbers(cuda, case):
+    """Those of an expert without rows, and of rows that no expert holds, are
+    nobody's: whatever they are, nothing changes and nothing is reported."""
+    c = Case(np.random.default_rng(6), *case)
+    c.counts[-1] -= 1  # the last row is held by none
+    good = c.run(cuda)
+    a, b = c.operands(cuda)
+    a.scales[:, -1] = float("nan")
+    b.scales[1] = 1.5  # the second expert has no rows
+    assert (c.run(cuda, (a, b)) == good).all()
+    cuda.device_status()
+
+
 @pytest.mark.parametrize("case", [c[:-1] + (True,) for c in CASES if c[1] < 3000], ids=_id)
 def test_any_scales(cuda, case):
     """any_scales takes them all, in the gradients too: fractions, zeros,
