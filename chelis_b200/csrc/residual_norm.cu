@@ -1,0 +1,873 @@
+// residual_norm.cu -- what stands between two blocks, one pass over a row:
+//
+//   u = N(branch) g1 + b1,   y = scale x + gate u,   h = N(y) g2 + b2
+//
+// and its gradients.  N is layer_norm's or the root-mean-square norm; every part
+// is optional; rows are f32, bf16 or f16, everything between is f32.  With n1, n2
+// the normalised rows, r1, r2 what they were multiplied by:
+//
+//   q  = dh g2,             dt = dy + r2 (q - mean(q) - n2 mean(q n2)),  dx = scale dt
+//   w  = dt gate g1,        dbranch = r1 (w - mean(w) - n1 mean(w n1))
+//   dg2 = sum dh n2,  db2 = sum dh,  s1 = sum dt n1,  s0 = sum dt over a gate's rows,
+//   dgate = g1 s1 + b1 s0,  dg1 = sum gate s1,  db1 = sum gate s0
+//
+// (the rms norm without the means of q and w; without a first norm dgate = sum
+// dt branch, kept as s1).  A row's variance is taken about its warps' own means,
+// put together exactly, so a mean far from 0 costs no digits.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace chelis {
+
+extern std::atomic<uint64_t> g_launches;
+
+namespace rnorm {
+
+using experts::from_f32;
+using experts::load_pack;
+using experts::Pack;
+using experts::store_pack;
+using experts::to_f32;
+using experts::warp_sum;
+
+constexpr int MAX_HIDDEN = 8192;
+
+struct Params {
+    int64_t rows;
+    int32_t hidden, rms;
+    const void *x, *branch;
+    const float *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
+    int64_t per_gate;  // rows that share a gate
+    float scale, eps;
+    void *y, *h;
+    int32_t staged;    // the parameters fit in shared memory beside the ring
+};
+
+// V consecutive f32 parameters.
+template <int N>
+__device__ __forceinline__ void load_params(const float *p, float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4 *>(p + i));
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __ldg(p + i);
+    }
+}
+
+// The threads of one row: W warps, TEAMS of them in a block.
+//
+// Rows come through shared memory: a team's first lane copies the next STAGES
+// rows of every operand there in bulk while this one is worked on (operands whose
+// rows no 16 bytes divide are read from global memory where they are wanted).
+// Each thread keeps E values of a row, in packs of N, pack i from column
+// (t + i THREADS) N on, and reads its parameters once for all of its rows.
+constexpr int THREADS = 512;
+constexpr int MAX_STAGES = 4;
+constexpr int MAX_ARRAYS = 4;
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+template <int W>
+struct Shared {
+    static constexpr int TEAMS = THREADS / (32 * W);
+    float2 slots[TEAMS][2][2][W];  // of each team two in turn, for one row's sums and another's
+    uint64_t landed[TEAMS][MAX_STAGES];
+};
+
+// A row's operands; NULL: not there.
+struct Rows {
+    const void *of[MAX_ARRAYS];
+    int32_t arrays;     // that are there
+    int32_t row_bytes;  // rounded up to 16
+    int32_t stages;
+};
+
+template <typename T, bool VEC, int W, int PACKS>
+struct Team {
+    static constexpr int TEAMS = Shared<W>::TEAMS, SPAN = W * 32, N = Pack<T, VEC>::N, E = PACKS * N;
+    Shared<W> &shared;
+    const int t, id, warp, lane, hidden;
+    const bool second;        // the half of the warp that looks after the second of two sums
+    const uint32_t tries;
+    float inv, own_inv;       // 1 / hidden, 1 / values of this warp's (0 for none)
+    float slot_own, slot_inv;  // of the warp whose slot this lane reads
+    int turn = 0;
+    bool in[PACKS];
+    // the ring
+    unsigned char *ring, *at;
+    int stage_bytes, stage = 0;
+    uint32_t phase = 0;
+    bool dead = false;  // a wait ran out: reported, no more waits
+
+    __device__ __forceinline__ Team(Shared<W> &sh, unsigned char *smem, const Rows &rows, int h)
+        : shared(sh), t(threadIdx.x % SPAN), id(threadIdx.x / SPAN), warp(threadIdx.x / 32 % W), lane(threadIdx.x & 31),
+          hidden(h), second((threadIdx.x & 16) != 0), tries(*static_cast<volatile uint32_t *>(&g_wait_tries)),
+          stage_bytes(rows.arrays * rows.row_bytes) {
+        const int own = values_of(warp), other = values_of(lane % W);
+        inv = 1.0f / static_cast<float>(h);
+        own_inv = own ? 1.0f / static_cast<float>(own) : 0.0f;
+        slot_own = static_cast<float>(other);
+        slot_inv = other ? 1.0f / static_cast<float>(other) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) in[i] = col(i) < hidden;
+        ring = smem + static_cast<size_t>(id) * rows.stages * stage_bytes;
+        at = ring + t * N * sizeof(T);
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < TEAMS; ++k)
+                for (int s = 0; s < MAX_STAGES; ++s) mbar_init(&sh.landed[k][s], 1);
+            fence_mbarrier_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ int values_of(int w) const {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) n += min(max(hidden - (w * 32 + i * SPAN) * N, 0), 32 * N);
+        return n;
+    }
+    __device__ __forceinline__ int col(int i) const { return (t + i * SPAN) * N; }
+    __device__ __forceinline__ void barrier() const {
+        if constexpr (W > 1) asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "n"(SPAN) : "memory");
+        else __syncwarp();
+    }
+    // Row `row` on its way to stage `s`, by one thread.
+    __device__ __forceinline__ void fetch(const Rows &rows, int64_t row, int s) {
+        unsigned char *dst = ring + s * stage_bytes;
+        uint64_t *bar = &shared.landed[id][s];
+        mbar_arrive_expect_tx(bar, stage_bytes);
+#pragma unroll
+        for (int a = 0; a < MAX_ARRAYS; ++a)
+            if (rows.of[a]) {
+                bulk_load(dst, static_cast<const unsigned char *>(rows.of[a]) + row * rows.row_bytes, rows.row_bytes, bar);
+                dst += rows.row_bytes;
+            }
+    }
+    __device__ __forceinline__ bool wait_for(uint64_t *bar) const {
+        for (uint32_t i = 0; i < tries; ++i)
+            if (mbar_try_wait(bar, phase)) return true;
+        report_device_error(DEVERR_TIMEOUT_PRODUCER);
+        return false;
+    }
+    __device__ __forceinline__ void wait() {
+        if (VEC && !dead) dead = !wait_for(&shared.landed[id][stage]);
+    }
+    __device__ __forceinline__ void next(int stages) {
+        at += stage_bytes;
+        if (++stage == stages) {
+            at -= stages * stage_bytes;
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    // Pack i of operand `a`, the `place`th of those that are there.
+    __device__ __forceinline__ void value(const Rows &rows, int a, int place, int64_t row, int i, float (&v)[N]) const {
+        Pack<T, VEC> k;
+        if constexpr (VEC)
+            *reinterpret_cast<uint4 *>(&k) =
+                *reinterpret_cast<const uint4 *>(at + place * rows.row_bytes + i * (SPAN * N * static_cast<int>(sizeof(T))));
+        else
+            k = load_pack<T, false>(static_cast<const T *>(rows.of[a]) + row * hidden + col(i));
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = to_f32(k.v[c]);
+    }
+    template <typename F>
+    __device__ __forceinline__ void store(void *to, int64_t row, int i, F f) const {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int c = 0; c < N; ++c) o.v[c] = from_f32<T>(f(i * N + c));
+        store_pack<T, VEC>(static_cast<T *>(to) + row * hidden + t * N + i * (SPAN * N), o);
+    }
+    // This thread's parameters, `absent` where there are none.
+    __device__ __forceinline__ void params(const float *p, float absent, float (&v)[E]) const {
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) params(p, absent, i, *reinterpret_cast<float(*)[N]>(&v[i * N]));
+    }
+    __device__ __forceinline__ void params(const float *p, float absent, int i, float (&v)[N]) const {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = absent;
+        if (p && in[i]) load_params<N>(p + col(i), v);
+    }
+    // The same of a copy in shared memory (stage_params): of each 8 the first four
+    // lie in one half, the others in the other, so that a warp reads whole lines.
+    __device__ __forceinline__ void staged(const float *p, int i, float (&v)[N]) const {
+        if constexpr (N == 8) {
+            const float4 a = reinterpret_cast<const float4 *>(p)[t + i * SPAN], b = reinterpret_cast<const float4 *>(p)[t + i * SPAN + hidden / 8];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else if constexpr (N == 4) {
+            const float4 a = reinterpret_cast<const float4 *>(p)[t + i * SPAN];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        }
+    }
+
+    // Sums over the team, the same bits in every thread, two at a time: the lower
+    // half of a warp adds up the first, the upper half the second.  One barrier;
+    // the slots are taken in turn, so the next sum's need not wait for this one's
+    // readers.
+    __device__ __forceinline__ float2 (*slot())[W] {
+        turn ^= 1;
+        return shared.slots[id][turn];
+    }
+    // The warp's sum of a in its lower half, of b in its upper.
+    __device__ __forceinline__ float halves_sum(float a, float b) const {
+        float v = (second ? b : a) + __shfl_xor_sync(0xffffffffu, second ? a : b, 16);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+        return v;
+    }
+    __device__ __forceinline__ static float slots_sum(float v) {
+#pragma unroll
+        for (int off = W / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+        return v;
+    }
+    __device__ __forceinline__ static void both(float v, float &a, float &b) {
+        a = __shfl_sync(0xffffffffu, v, 0);
+        b = __shfl_sync(0xffffffffu, v, 16);
+    }
+    __device__ __forceinline__ void sum2(float &a, float &b) {
+        float v = halves_sum(a, b);
+        if constexpr (W > 1) {
+            float2(*s)[W] = slot();
+            if ((lane & 15) == 0) s[second][warp].x = v;
+            barrier();
+            v = slots_sum(s[second][lane % W].x);
+        }
+        both(v, a, b);
+    }
+    // Reciprocal root, one Newton step past the hardware's.
+    __device__ __forceinline__ static float root(float v) {
+        const float r = rsqrtf(v);
+        return v < INFINITY ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
+    }
+    // Mean and reciprocal root of what a row is divided by, of two rows at once (or
+    // one twice): each warp's sum, its squares about its own mean, then the team's.
+    __device__ __forceinline__ void stats2(const float (&u)[E], const float (&v)[E], bool two, bool rms, float eps, float *mean_u,
+                                           float *r_u, float *mean_v, float *r_v) {
+        float su = 0.0f, sv = 0.0f, sum = 0.0f, cu = 0.0f, cv = 0.0f;
+        if (!rms) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) su += u[e];
+            if (two)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sv += v[e];
+            sum = halves_sum(su, sv);
+            both(sum * own_inv, cu, cv);
+        }
+        float qu = 0.0f, qv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i)
+            if (in[i]) {
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    const float d = u[i * N + c] - cu;
+                    qu = fmaf(d, d, qu);
+                }
+                if (two)
+#pragma unroll
+                    for (int c = 0; c < N; ++c) {
+                        const float d = v[i * N + c] - cv;
+                        qv = fmaf(d, d, qv);
+                    }
+            }
+        float q = halves_sum(qu, qv), mean = sum * own_inv;
+        if constexpr (W > 1) {
+            float2(*s)[W] = slot();
+            if ((lane & 15) == 0) s[second][warp] = make_float2(sum, q);
+            barrier();
+            const float2 o = s[second][lane % W];
+            mean = slots_sum(o.x) * inv;
+            const float d = rms ? 0.0f : fmaf(o.x, slot_inv, -mean);
+            q = slots_sum(fmaf(slot_own * d, d, o.y));
+        }
+        const float r = root(fmaf(q, inv, eps));
+        both(mean, *mean_u, *mean_v);
+        both(r, *r_u, *r_v);
+    }
+    // Copies that a wait gave up on land before the block leaves.
+    __device__ __forceinline__ void drain(int stages) {
+        if (VEC && dead && t == 0)
+            for (int s = 0; s < stages; ++s) wait_for(&shared.landed[id][s]);
+    }
+};
+
+// By the whole block: parameters as Team::staged takes them, times `factor`'s if
+// that is given, `absent` where there are none.
+template <int N>
+__device__ __forceinline__ void stage_params(float *to, const float *p, const float *factor, float absent, int hidden) {
+    for (int c = threadIdx.x; c < hidden; c += THREADS) {
+        const int at = N == 8 ? (c / 8 * 4 + c % 4) + (c & 4 ? hidden / 2 : 0) : c;
+        to[at] = (p ? __ldg(p + c) : absent) * (factor ? __ldg(factor + c) : 1.0f);
+    }
+}
+
+// y = scale x + N1(branch) c1 + c0 with c1 = gate g1, c0 = gate b1, h = N2(y) g2 + b2.
+template <typename T, bool VEC, int W, int PACKS>
+__global__ void __launch_bounds__(THREADS, 1)
+    fwd_kernel(const Params p, const Rows in) {
+    using G = Team<T, VEC, W, PACKS>;
+    constexpr int N = G::N, E = G::E;
+    extern __shared__ __align__(128) unsigned char rows_smem[];
+    __shared__ Shared<W> shared;
+    G team(shared, rows_smem, in, p.hidden);
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS, me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
+    const int64_t first = p.rows * me / teams, last = p.rows * (me + 1) / teams;
+    if (VEC && team.t == 0)
+        for (int s = 0; s < in.stages && first + s < last; ++s) team.fetch(in, first + s, s);
+    const bool rms = p.rms != 0, post = p.post_gamma != nullptr, pre = p.pre_gamma != nullptr, branch = p.branch != nullptr;
+    // one gate at most: it goes into c1 and c0
+    const bool staged = VEC && p.staged, one_gate = p.per_gate >= p.rows;
+    float *const c1 = reinterpret_cast<float *>(rows_smem + static_cast<size_t>(G::TEAMS) * in.stages * in.arrays * in.row_bytes);
+    float *const c0 = c1 + p.hidden, *const g2 = c0 + p.hidden, *const b2 = g2 + p.hidden;
+    if (staged) {
+        const float *g = one_gate ? p.gate : nullptr;
+        stage_params<N>(c1, p.post_gamma, g, 1.0f, p.hidden);
+        stage_params<N>(c0, p.post_beta, g, 0.0f, p.hidden);
+        stage_params<N>(g2, p.pre_gamma, nullptr, 1.0f, p.hidden);
+        stage_params<N>(b2, p.pre_beta, nullptr, 0.0f, p.hidden);
+        __syncthreads();
+    }
+    const float *gate = nullptr;
+    int64_t gate_end = first;
+    for (int64_t row = first; row < last; ++row) {
+        if (p.gate && !(staged && one_gate) && row >= gate_end) {
+            const int64_t group = row / p.per_gate;
+            gate = p.gate + group * p.hidden;
+            gate_end = (group + 1) * p.per_gate;
+        }
+        team.wait();
+        float v[E], mean = 0.0f, r = 1.0f, none;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            float u[N] = {};
+            if (team.in[i]) team.value(in, branch ? 1 : 0, branch ? 1 : 0, row, i, u);
+#pragma unroll
+            for (int c = 0; c < N; ++c) v[i * N + c] = u[c];
+        }
+        if (branch) {
+            if (post) team.stats2(v, v, false, rms, p.eps, &mean, &r, &none, &none);
+            const float shift = -mean * r;
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i)
+                if (team.in[i]) {
+                    float x[N], k[N];
+                    if (staged) {
+                        float z[N];
+                        team.staged(c1, i, k);
+                        team.staged(c0, i, z);
+#pragma unroll
+                        for (int c = 0; c < N; ++c) v[i * N + c] = fmaf(fmaf(v[i * N + c], r, shift), k[c], z[c]);
+                    } else if (post) {
+                        team.params(p.post_gamma, 1.0f, i, k);
+#pragma unroll
+                        for (int c = 0; c < N; ++c) v[i * N + c] = fmaf(v[i * N + c], r, shift) * k[c];
+                        if (p.post_beta) {
+                            team.params(p.post_beta, 0.0f, i, k);
+#pragma unroll
+                            for (int c = 0; c < N; ++c) v[i * N + c] += k[c];
+                        }
+                    }
+                    if (gate) {
+                        team.params(gate, 1.0f, i, k);
+#pragma unroll
+                        for (int c = 0; c < N; ++c) v[i * N + c] *= k[c];
+                    }
+                    team.value(in, 0, 0, row, i, x);
+#pragma unroll
+                    for (int c = 0; c < N; ++c) v[i * N + c] = fmaf(p.scale, x[c], v[i * N + c]);
+                    team.store(p.y, row, i, [&](int e) { return v[e]; });
+                }
+        }
+        if (pre) {
+            team.stats2(v, v, false, rms, p.eps, &mean, &r, &none, &none);
+            const float shift = -mean * r;
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i)
+                if (team.in[i]) {
+                    float g[N], k[N];
+                    if (staged) {
+                        team.staged(g2, i, g);
+                        team.staged(b2, i, k);
+                    } else {
+                        team.params(p.pre_gamma, 0.0f, i, g);
+                        team.params(p.pre_beta, 0.0f, i, k);
+                    }
+                    team.store(p.h, row, i, [&](int e) { return fmaf(fmaf(v[e], r, shift), g[e % N], k[e % N]); });
+                }
+        }
+        if (VEC) {
+            // every thread has read the row once the last statistics' barrier is
+            // passed (of the second norm: they need all of y)
+            if (!pre || W == 1) team.barrier();
+            if (team.t == 0 && row + in.stages < last) team.fetch(in, row + in.stages, team.stage);
+            team.next(in.stages);
+        }
+    }
+    team.drain(in.stages);
+}
+
+// ---- backward -------------------------------------------------------------
+// A team's rows are consecutive, in units that lie within one gate's rows; the
+// sums over them (s1, s0 of a unit, dg2, db2 of the team) stay in registers and
+// go to partial sums that fold_kernel adds up in order.
+struct Backward {
+    int64_t rows;
+    int32_t hidden, rms;
+    const float *post_gamma, *gate, *pre_gamma;
+    int64_t per_gate, groups, chunks;  // units = groups * chunks
+    float scale, eps;
+    void *dx, *dbranch;
+    float *unit_sums;  // [units][2][hidden]: s1, s0; NULL: not needed
+    float *team_sums;  // [teams][2][hidden]: dg2, db2; NULL: not needed
+};
+enum { DY = 0, DH = 1, Y = 2, BRANCH = 3 };  // of Rows
+
+template <typename T, bool VEC, int W, int PACKS>
+__global__ void __launch_bounds__(THREADS, 1)
+    bwd_kernel(const Backward p, const Rows in) {
+    using G = Team<T, VEC, W, PACKS>;
+    constexpr int N = G::N, E = G::E;
+    constexpr bool HOLD = E <= 8;  // parameters stay in registers
+    extern __shared__ __align__(128) unsigned char rows_smem[];
+    __shared__ Shared<W> shared;
+    G team(shared, rows_smem, in, p.hidden);
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS, me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
+    const int64_t units = p.groups * p.chunks;
+    auto unit_first = [&](int64_t u) { return u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks) / p.chunks; };
+    auto unit_last = [&](int64_t u) { return u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks + 1) / p.chunks; };
+    // the row after the last one on its way
+    int64_t ahead_unit = me, ahead = me < units ? unit_first(me) : 0, ahead_last = me < units ? unit_last(me) : 0;
+    auto fetch = [&](int s) {
+        while (ahead == ahead_last) {
+            ahead_unit += teams;
+            if (ahead_unit >= units) return;
+            ahead = unit_first(ahead_unit);
+            ahead_last = unit_last(ahead_unit);
+        }
+        team.fetch(in, ahead++, s);
+    };
+    if (VEC && team.t == 0 && me < units)
+        for (int s = 0; s < in.stages; ++s) fetch(s);
+
+    const bool rms = p.rms != 0, pre = in.of[DH] != nullptr, has_dy = in.of[DY] != nullptr;
+    const bool has_branch = in.of[BRANCH] != nullptr, post = p.post_gamma != nullptr;
+    const int at_dh = has_dy ? 1 : 0, at_y = at_dh + 1, at_b = at_dh + (pre ? 2 : 0);
+    const float inv = team.inv;
+    float s1[E], s0[E], dg2[E], db2[E], g2[HOLD ? E : 1], c1[HOLD ? E : 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) dg2[e] = db2[e] = 0.0f;
+    if constexpr (HOLD) team.params(p.pre_gamma, 0.0f, g2);
+    for (int64_t unit = me; unit < units; unit += teams) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s1[e] = s0[e] = 0.0f;
+        const float *gate = p.gate ? p.gate + unit / p.chunks * p.hidden : nullptr;
+        if constexpr (HOLD) {  // gate times gamma
+            float g[E];
+            team.params(p.post_gamma, 1.0f, c1);
+            team.params(gate, 1.0f, g);
+#pragma unroll
+            for (int e = 0; e < E; ++e) c1[e] *= g[e];
+        }
+        const int64_t last = unit_last(unit);
+        for (int64_t row = unit_first(unit); row < last; ++row) {
+            team.wait();
+            float v[E], b[E], dt[E], mean2, r2, mean1 = 0.0f, r1 = 1.0f;
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i) {
+                float u[N] = {}, w[N] = {};
+                if (pre && team.in[i]) team.value(in, Y, at_y, row, i, u);
+                if (has_branch && team.in[i]) team.value(in, BRANCH, at_b, row, i, w);
+#pragma unroll
+                for (int c = 0; c < N; ++c) v[i * N + c] = u[c], b[i * N + c] = w[c];
+            }
+            if (pre) {
+                team.stats2(v, b, post, rms, p.eps, &mean2, &r2, &mean1, &r1);
+                const float shift2 = -mean2 * r2;
+                float sq = 0.0f, sqn = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PACKS; ++i)
+                    if (team.in[i]) {
+                        float d[N], g[N];
+                        team.value(in, DH, at_dh, row, i, d);
+                        if constexpr (!HOLD) load_params<N>(p.pre_gamma + team.col(i), g);
+#pragma unroll
+                        for (int c = 0; c < N; ++c) {
+                            const int e = i * N + c;
+                            if constexpr (HOLD) g[c] = g2[e];
+                            v[e] = fmaf(v[e], r2, shift2);
+                            dg2[e] = fmaf(d[c], v[e], dg2[e]);
+                            db2[e] += d[c];
+                            dt[e] = d[c] * g[c];
+                            sq += dt[e];
+                            sqn = fmaf(dt[e], v[e], sqn);
+                        }
+                    }
+                team.sum2(sq, sqn);
+                sq = rms ? 0.0f : sq * inv;
+                sqn *= inv;
+#pragma unroll
+                for (int e = 0; e < E; ++e) dt[e] = (dt[e] - fmaf(v[e], sqn, sq)) * r2;
+            } else {
+                if (post) team.stats2(b, b, false, rms, p.eps, &mean1, &r1, &mean2, &r2);
+#pragma unroll
+                for (int e = 0; e < E; ++e) dt[e] = 0.0f;
+            }
+            if (!post) mean1 = 0.0f, r1 = 1.0f;
+            const float shift1 = -mean1 * r1;
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i)
+                if (team.in[i]) {
+                    if (has_dy) {
+                        float d[N];
+                        team.value(in, DY, 0, row, i, d);
+#pragma unroll
+                        for (int c = 0; c < N; ++c) dt[i * N + c] += d[c];
+                    }
+                    team.store(p.dx, row, i, [&](int e) { return p.scale * dt[e]; });
+                }
+            if (p.dbranch) {
+                float sw = 0.0f, swn = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PACKS; ++i)
+                    if (team.in[i]) {
+                        float g[N];
+#pragma unroll
+                        for (int c = 0; c < N; ++c) g[c] = 1.0f;
+                        if constexpr (!HOLD) {
+                            if (post) load_params<N>(p.post_gamma + team.col(i), g);
+                            if (gate) {
+                                float k[N];
+                                load_params<N>(gate + team.col(i), k);
+#pragma unroll
+                                for (int c = 0; c < N; ++c) g[c] *= k[c];
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < N; ++c) {
+                            const int e = i * N + c;
+                            if constexpr (HOLD) g[c] = c1[e];
+                            b[e] = fmaf(b[e], r1, shift1);  // the branch itself without a norm
+                            s1[e] = fmaf(dt[e], b[e], s1[e]);
+                            s0[e] += dt[e];
+                            dt[e] *= g[c];
+                            sw += dt[e];
+                            swn = fmaf(dt[e], b[e], swn);
+                        }
+                    }
+                if (post) {
+                    team.sum2(sw, swn);
+                    sw = rms ? 0.0f : sw * inv;
+                    swn *= inv;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) dt[e] = (dt[e] - fmaf(b[e], swn, sw)) * r1;
+                }
+#pragma unroll
+                for (int i = 0; i < PACKS; ++i)
+                    if (team.in[i]) team.store(p.dbranch, row, i, [&](int e) { return dt[e]; });
+            }
+            if (VEC) {
+                // the last sum's barrier says that every thread has read the row
+                if (!post || W == 1) team.barrier();
+                if (team.t == 0) fetch(team.stage);
+                team.next(in.stages);
+            }
+        }
+        if (p.unit_sums) {
+            float *dst = p.unit_sums + unit * 2 * p.hidden;
+#pragma unroll
+            for (int i = 0; i < PACKS; ++i)
+                if (team.in[i])
+#pragma unroll
+                    for (int c = 0; c < N; ++c) {
+                        dst[team.col(i) + c] = s1[i * N + c];
+                        dst[p.hidden + team.col(i) + c] = s0[i * N + c];
+                    }
+        }
+    }
+    if (p.team_sums) {
+        float *dst = p.team_sums + me * 2 * p.hidden;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i)
+            if (team.in[i])
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    dst[team.col(i) + c] = dg2[i * N + c];
+                    dst[p.hidden + team.col(i) + c] = db2[i * N + c];
+                }
+    }
+    team.drain(in.stages);
+}
+
+// Sums of `count` rows of [..][2][hidden], both halves, in a fixed order: 32
+// columns a block, 8 threads of each taking every 8th row (with 32 of them the 8
+// groups of 16384 x 4096 rows took 30 us, the blocks' own launch most of it).
+constexpr int FOLD_SLICES = 8;
+__device__ __forceinline__ void fold2(const float *src, int64_t count, int hidden, float (*part)[2][32], float *a, float *b) {
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    float u = 0.0f, v = 0.0f;
+    if (col < hidden) {
+#pragma unroll 8
+        for (int64_t i = slice; i < count; i += FOLD_SLICES) {
+            u += __ldg(src + i * 2 * hidden + col);
+            v += __ldg(src + i * 2 * hidden + hidden + col);
+        }
+    }
+    part[slice][0][lane] = u;
+    part[slice][1][lane] = v;
+    __syncthreads();
+    *a = *b = 0.0f;
+    if (slice == 0)
+#pragma unroll
+        for (int s = 0; s < FOLD_SLICES; ++s) *a += part[s][0][lane], *b += part[s][1][lane];
+}
+struct Fold {
+    const float *unit_sums, *team_sums;
+    int64_t groups, chunks, teams;
+    int32_t hidden;
+    const float *post_gamma, *post_beta, *gate;
+    float *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
+    float *by_group;  // [groups][2][hidden]: gate times s1, s0 (more than one group)
+};
+__global__ void __launch_bounds__(32 * FOLD_SLICES)
+    fold_kernel(const Fold p) {
+    __shared__ float part[FOLD_SLICES][2][32];
+    const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
+    const int64_t groups = p.unit_sums ? p.groups : 0, all = groups + (p.team_sums ? 1 : 0);
+    const bool writes = threadIdx.x < 32 && col < p.hidden;
+    for (int64_t group = blockIdx.y; group < all; group += gridDim.y, __syncthreads()) {
+        float a, b;
+        if (group == groups) {  // the second norm's, over all teams
+            fold2(p.team_sums, p.teams, p.hidden, part, &a, &b);
+            if (writes && p.dpre_gamma) p.dpre_gamma[col] = a;
+            if (writes && p.dpre_beta) p.dpre_beta[col] = b;
+            continue;
+        }
+        fold2(p.unit_sums + group * p.chunks * 2 * p.hidden, p.chunks, p.hidden, part, &a, &b);
+        if (!writes) continue;
+        const int64_t at = group * p.hidden + col;
+        if (p.dgate) {
+            float d = a;
+            if (p.post_gamma) d = p.post_beta ? fmaf(p.post_gamma[col], a, p.post_beta[col] * b) : p.post_gamma[col] * a;
+            p.dgate[at] = d;
+        }
+        if (!p.post_gamma) continue;
+        const float g = p.gate ? p.gate[at] : 1.0f;
+        if (p.by_group) {
+            p.by_group[group * 2 * p.hidden + col] = g * a;
+            p.by_group[(group * 2 + 1) * p.hidden + col] = g * b;
+        } else {
+            if (p.dpost_gamma) p.dpost_gamma[col] = g * a;
+            if (p.dpost_beta) p.dpost_beta[col] = g * b;
+        }
+    }
+}
+__global__ void __launch_bounds__(32 * FOLD_SLICES)
+    fold_groups_kernel(const float *__restrict__ by_group, int64_t groups, int hidden, float *__restrict__ dgamma,
+                       float *__restrict__ dbeta) {
+    __shared__ float part[FOLD_SLICES][2][32];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+    float a, b;
+    fold2(by_group, groups, hidden, part, &a, &b);
+    if (threadIdx.x < 32 && col < hidden) {
+        if (dgamma) dgamma[col] = a;
+        if (dbeta) dbeta[col] = b;
+    }
+}
+
+// The ring's shape and the grid for f(T, VEC, W, PACKS, grid, shared memory): MOST
+// values a thread (8 where one warp can take the row so), the fewest warps a team.
+// `params`: bytes of parameters that would lie beside the ring; *staged, whether they do.
+template <int MOST, typename F>
+void launch(int32_t dtype, bool vec, int64_t hidden, Rows &in, int64_t rows, int64_t params, int32_t *staged, F f) {
+    const int each = hidden <= 256 ? 8 : (MOST == 8 && hidden > 4096 ? 16 : MOST);
+    int warps = 1;
+    while (warps < 16 && hidden > static_cast<int64_t>(warps) * 32 * each) warps *= 2;
+    const int teams = 16 / warps;
+    in.row_bytes = static_cast<int32_t>((hidden * experts::width(dtype) + 15) / 16 * 16);
+    const int64_t stage = static_cast<int64_t>(in.arrays) * in.row_bytes * teams;
+    // the parameters, where that leaves two stages, or the one that there is
+    const int64_t room = 208 * 1024, beside = vec ? (room - params) / stage : 0;
+    *staged = params > 0 && (beside >= 2 || (beside == 1 && room / stage == 1));
+    const int64_t stages = vec ? (*staged ? beside : room / stage) : 0;
+    in.stages = static_cast<int32_t>(stages > MAX_STAGES ? MAX_STAGES : stages);
+    int64_t grid = sm_count();
+    if (grid > (rows + teams - 1) / teams) grid = (rows + teams - 1) / teams;
+    const size_t smem = static_cast<size_t>(stage) * in.stages + (*staged ? params : 0);
+    experts::by_type(dtype, vec, [&](auto t, auto v) {
+        constexpr int N = experts::Pack<decltype(t), decltype(v)::value>::N;
+        const unsigned g = static_cast<unsigned>(grid);
+        auto with = [&](auto w, auto e) { f(t, v, w, std::integral_constant<int, decltype(e)::value / N>{}, g, smem); };
+        using E = std::integral_constant<int, MOST>;
+        if (each == 8 && warps == 1) with(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+        else if (warps == 16) {
+            if constexpr (MOST == 8) {
+                if (each == 16) with(std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+                else with(std::integral_constant<int, 16>{}, E{});
+            } else if constexpr (MOST == 16) with(std::integral_constant<int, 16>{}, E{});
+        } else if (warps == 8) with(std::integral_constant<int, 8>{}, E{});
+        else if (warps == 4) with(std::integral_constant<int, 4>{}, E{});
+        else if (warps == 2) with(std::integral_constant<int, 2>{}, E{});
+        else with(std::integral_constant<int, 1>{}, E{});
+    });
+}
+
+int check(const char *op, int32_t dtype, int32_t kind, int64_t rows, int64_t hidden, int64_t groups) {
+    if (!experts::is_act(dtype)) return set_error(CHELIS_CUDA_ERR_UNSUPPORTED, "%s takes f32, bf16 or f16", op);
+    if (kind != CHELIS_NORM_LAYER && kind != CHELIS_NORM_RMS)
+        return set_error(CHELIS_CUDA_ERR_UNSUPPORTED, "%s: unknown norm %d", op, kind);
+    if (rows < 0 || hidden < 0) return set_error(CHELIS_CUDA_ERR_DOMAIN, "numeric trap: domain in %s at i64", op);
+    if (hidden > MAX_HIDDEN) return set_error(CHELIS_CUDA_ERR_UNSUPPORTED, "%s admits rows of <= %d", op, MAX_HIDDEN);
+    if (groups < 1 || rows % groups != 0)
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "%s: the gate's groups divide the rows", op);
+    return CHELIS_CUDA_OK;
+}
+bool aligned(std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (!experts::aligned16(p)) return false;
+    return true;
+}
+
+}  // namespace rnorm
+}  // namespace chelis
+
+using namespace chelis;
+
+extern "C" int chelis_cuda_residual_norm(int32_t dtype, int32_t kind, int64_t rows, int64_t hidden, const void *x,
+                                         const void *branch, const float *post_gamma, const float *post_beta,
+                                         const float *gate, int64_t groups, float scale, const float *pre_gamma,
+                                         const float *pre_beta, float eps, void *y, void *h) {
+    CHELIS_TRY(rnorm::check("residual_norm", dtype, kind, rows, hidden, groups));
+    if (rows == 0 || hidden == 0) return CHELIS_CUDA_OK;
+    if (!branch && (post_gamma || gate || y || scale != 1.0f))
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "residual_norm: without a branch there is the second norm alone");
+    if ((post_beta && !post_gamma) || (pre_beta && !pre_gamma))
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "residual_norm: a beta without its gamma");
+    if (!x || (branch && !y) || (pre_gamma && !h) || (!branch && !pre_gamma))
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "residual_norm: null operand");
+    rnorm::Params p{rows, static_cast<int32_t>(hidden), kind == CHELIS_NORM_RMS, x, branch, post_gamma, post_beta, gate,
+                    pre_gamma, pre_beta, rows / groups, scale, eps, y, h, 0};
+    const bool vec = hidden * experts::width(dtype) % 16 == 0 &&
+                     rnorm::aligned({x, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta, y, h});
+    rnorm::Rows in{{x, branch, nullptr, nullptr}, branch ? 2 : 1, 0, 0};
+    int rc = CHELIS_CUDA_OK;
+    const auto run = [&](auto t, auto v, auto w, auto packs, unsigned grid, size_t smem) {
+        auto kernel = rnorm::fwd_kernel<decltype(t), decltype(v)::value, decltype(w)::value, decltype(packs)::value>;
+        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+                        "cudaFuncSetAttribute");
+        if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, current_stream()>>>(p, in);
+    };
+    // few rows: eight values a thread, a row over as many warps as there are
+    if (rows <= sm_count()) rnorm::launch<8>(dtype, vec, hidden, in, rows, 0, &p.staged, run);
+    else rnorm::launch<32>(dtype, vec, hidden, in, rows, 16 * hidden, &p.staged, run);
+    CHELIS_TRY(rc);
+    g_launches++;
+    CHELIS_LAUNCH_CHECK("rnorm::fwd_kernel");
+    return CHELIS_CUDA_OK;
+}
+
+extern "C" int chelis_cuda_residual_norm_bwd(int32_t dtype, int32_t kind, int64_t rows, int64_t hidden, const void *dy,
+                                             const void *dh, const void *y, const void *branch, const float *post_gamma,
+                                             const float *post_beta, const float *gate, int64_t groups, float scale,
+                                             const float *pre_gamma, float eps, void *dx, void *dbranch,
+                                             float *dpost_gamma, float *dpost_beta, float *dgate, float *dpre_gamma,
+                                             float *dpre_beta) {
+    CHELIS_TRY(rnorm::check("residual_norm_bwd", dtype, kind, rows, hidden, groups));
+    if (hidden == 0) return CHELIS_CUDA_OK;
+    cudaStream_t s = current_stream();
+    if ((!post_gamma && (post_beta || dpost_gamma || dpost_beta)) || (!gate && dgate) ||
+        (!pre_gamma && (dpre_gamma || dpre_beta)))
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "residual_norm_bwd: a gradient of what is not there");
+    if (rows == 0) {
+        auto zero = [&](float *p, int64_t n) {
+            return p ? check_cuda(cudaMemsetAsync(p, 0, static_cast<size_t>(n) * 4, s), "memset") : CHELIS_CUDA_OK;
+        };
+        CHELIS_TRY(zero(dpost_gamma, hidden));
+        CHELIS_TRY(zero(dpost_beta, hidden));
+        CHELIS_TRY(zero(dgate, groups * hidden));
+        CHELIS_TRY(zero(dpre_gamma, hidden));
+        return zero(dpre_beta, hidden);
+    }
+    const bool needs_branch = post_gamma || gate;
+    if (!dx || (!dy && !dh) || (pre_gamma && !y) || (dh != nullptr) != (pre_gamma != nullptr) ||
+        (needs_branch && (!branch || !dbranch)))
+        return set_error(CHELIS_CUDA_ERR_DOMAIN, "residual_norm_bwd: null operand");
+    const bool vec = hidden * experts::width(dtype) % 16 == 0 &&
+                     rnorm::aligned({dy, dh, y, branch, post_gamma, gate, pre_gamma, dx, dbranch});
+    rnorm::Rows in{{dy, dh, dh ? y : nullptr, needs_branch ? branch : nullptr},
+                   (dy ? 1 : 0) + (dh ? 2 : 0) + (needs_branch ? 1 : 0), 0, 0};
+    rnorm::Backward p{};
+    p.rows = rows;
+    p.hidden = static_cast<int32_t>(hidden);
+    p.rms = kind == CHELIS_NORM_RMS;
+    p.post_gamma = post_gamma;
+    p.gate = gate;
+    p.pre_gamma = pre_gamma;
+    p.per_gate = rows / groups;
+    p.groups = groups;
+    p.scale = scale;
+    p.eps = eps;
+    p.dx = dx;
+    p.dbranch = dbranch;
+    const bool unit_sums = dpost_gamma || dpost_beta || dgate, team_sums = dpre_gamma || dpre_beta;
+    const bool by_group = groups > 1 && (dpost_gamma || dpost_beta);
+    void *scratch = nullptr;
+    auto body = [&]() -> int {
+        int rc = CHELIS_CUDA_OK;
+        float *sums = nullptr;
+        size_t unit_n = 0, team_n = 0;
+        int64_t teams = 0;
+        int32_t staged = 0;
+        rnorm::launch<8>(dtype, vec, hidden, in, rows, 0, &staged, [&](auto t, auto v, auto w, auto packs, unsigned grid, size_t smem) {
+            constexpr int W = decltype(w)::value;
+            teams = static_cast<int64_t>(grid) * (rnorm::THREADS / (32 * W));
+            p.chunks = teams / groups < 1 ? 1 : teams / groups;
+            if (p.chunks > p.per_gate) p.chunks = p.per_gate;
+            unit_n = unit_sums ? static_cast<size_t>(groups) * p.chunks * 2 * hidden : 0;
+            team_n = team_sums ? static_cast<size_t>(teams) * 2 * hidden : 0;
+            const size_t group_n = by_group ? static_cast<size_t>(groups) * 2 * hidden : 0;
+            rc = scratch_alloc(&scratch, (unit_n + team_n + group_n) * sizeof(float), s);
+            if (rc != CHELIS_CUDA_OK) return;
+            sums = static_cast<float *>(scratch);
+            p.unit_sums = unit_sums ? sums : nullptr;
+            p.team_sums = team_sums ? sums + unit_n : nullptr;
+            auto kernel = rnorm::bwd_kernel<decltype(t), decltype(v)::value, W, decltype(packs)::value>;
+            rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+                            "cudaFuncSetAttribute");
+            if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, s>>>(p, in);
+        });
+        CHELIS_TRY(rc);
+        g_launches++;
+        CHELIS_LAUNCH_CHECK("rnorm::bwd_kernel");
+        if (!unit_sums && !team_sums) return CHELIS_CUDA_OK;
+        rnorm::Fold f{p.unit_sums, p.team_sums, groups, p.chunks, teams, p.hidden, post_gamma, post_beta, gate, dgate,
+                      dpost_gamma, dpost_beta, dpre_gamma, dpre_beta, by_group ? sums + unit_n + team_n : nullptr};
+        int64_t high = (unit_sums ? groups : 0) + (team_sums ? 1 : 0);
+        if (high > 65535) high = 65535;
+        const unsigned wide = static_cast<unsigned>((hidden + 31) / 32);
+        rnorm::fold_kernel<<<dim3(wide, static_cast<unsigned>(high)), 32 * rnorm::FOLD_SLICES, 0, s>>>(f);
+        g_launches++;
+        CHELIS_LAUNCH_CHECK("rnorm::fold_kernel");
+        if (by_group) {
+            rnorm::fold_groups_kernel<<<wide, 32 * rnorm::FOLD_SLICES, 0, s>>>(f.by_group, groups, p.hidden, dpost_gamma, dpost_beta);
+            g_launches++;
+            CHELIS_LAUNCH_CHECK("rnorm::fold_groups_kernel");
+        }
+        return CHELIS_CUDA_OK;
+    };
+    const int rc = body();
+    scratch_free(scratch, s);
+    return rc;
+}

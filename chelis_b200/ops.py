@@ -8,6 +8,7 @@ tensors.  Names and argument meanings follow the reference's operations
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 from typing import NamedTuple
@@ -818,3 +819,329 @@ def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
            dy.data.data_ptr(), dy.scales.data_ptr(), x.data.data_ptr(), x.scales.data_ptr(),
            _ptr(offsets), max(groups, 1), int(any_scales), _ACT[dtype], out.data_ptr())
     return out
+
+
+# ---------------------------------------------------------------- a feed-forward sublayer in 16 bits
+
+_HALF = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
+_ACTIVATION = {None: L.ACT_NONE, "relu": L.ACT_RELU, "gelu": L.ACT_GELU, "silu": L.ACT_SILU}
+_NORM = {"layer": L.NORM_LAYER, "rms": L.NORM_RMS}
+
+
+def _begin(name: str, *tensors: torch.Tensor | None) -> None:
+    """_prepare, and all tensors on one device, the current one."""
+    dev = -1
+    for t in tensors:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            raise ValueError("chelis_b200 ops take CUDA tensors (device memory)")
+        if not t.is_contiguous():
+            raise ValueError("chelis_b200 ops take contiguous tensors")
+        if dev < 0:
+            dev = at
+        elif at != dev:
+            raise ValueError(f"{name}: tensors on different devices")
+    _on_device(name, dev)
+
+
+def _on_device(name: str, dev: int) -> None:
+    current = torch.cuda.current_device()
+    if dev >= 0 and dev != current:
+        raise ValueError(f"{name}: the tensors' device is not the current one")
+    if current not in _initialised:
+        L.call("chelis_cuda_init", current)
+        _initialised.add(current)
+    L.load().chelis_cuda_set_stream(_raw_stream(current))
+
+
+def _half(name: str, t: torch.Tensor) -> int:
+    if t.dtype not in _HALF:
+        raise ValueError(f"{name} takes bf16 or f16 tensors")
+    return _HALF[t.dtype]
+
+
+def _activation(name: str, activation: str | None) -> int:
+    if activation not in _ACTIVATION:
+        raise ValueError(f"{name}: activations are relu, gelu and silu")
+    return _ACTIVATION[activation]
+
+
+def matmul16(a: torch.Tensor, b: torch.Tensor, trans_a: bool = False, trans_b: bool = False, *,
+             bias: torch.Tensor | None = None, activation: str | None = None,
+             residual: torch.Tensor | None = None, keep_pre: bool = False,
+             through: tuple[torch.Tensor, str] | None = None, dtype: torch.dtype | None = None):
+    """act(op(a).op(b) + bias) + residual of two bf16 or two f16 matrices: f32
+    sums on the tensor cores, what follows them in the same kernel, one
+    rounding to dtype (f32 or the operands' own, the default).  activation is
+    relu, gelu (exact) or silu; bias [n] is f32 or of the operands' type, and
+    residual [m, n] of dtype.  keep_pre: (y, z) with z = op(a).op(b) + bias, what
+    the activation's gradient needs.
+
+    through=(z, activation) gives the gradient through an activation that was
+    taken at z [m, n], (op(a).op(b)) * act'(z), and goes with none of the
+    others."""
+    dt = _half("matmul16", a)
+    if b.dtype != a.dtype or a.dim() != 2 or b.dim() != 2:
+        raise ValueError("matmul16 takes two bf16 or two f16 matrices")
+    dtype = a.dtype if dtype is None else dtype
+    if dtype != a.dtype and dtype != torch.float32:
+        raise ValueError("matmul16 gives f32 or its operands' type")
+    m, k = a.shape[::-1] if trans_a else a.shape
+    k2, n = b.shape[::-1] if trans_b else b.shape
+    if k != k2:
+        raise ValueError(f"contraction extents differ: {k} vs {k2}")
+    z = None
+    if through is not None:
+        if bias is not None or activation is not None or residual is not None or keep_pre:
+            raise ValueError("matmul16: through goes with no bias, activation, residual or keep_pre")
+        z, activation = through
+    act = _activation("matmul16", activation)
+    if bias is not None and (bias.shape != (n,) or bias.dtype not in (a.dtype, torch.float32)):
+        raise ValueError("matmul16: bias is [n], f32 or of the operands' type")
+    for t in (residual, z):
+        if t is not None and (t.shape != (m, n) or t.dtype != dtype):
+            raise ValueError("matmul16: residual and through are [m, n] of the result's type")
+    _begin("matmul16", a, b, bias, residual, z)
+    out = torch.empty(m, n, dtype=dtype, device=a.device)
+    pre = torch.empty_like(out) if keep_pre else None
+    L.call("chelis_cuda_matmul16", dt, int(trans_a), int(trans_b), m, n, k, a.data_ptr(), b.data_ptr(),
+           _ptr(bias), 0 if bias is None else _ACT[bias.dtype], act, _ptr(residual), _ptr(z), _ptr(pre),
+           _ACT[dtype], out.data_ptr())
+    return (out, pre) if keep_pre else out
+
+
+def activation16_bwd(dy: torch.Tensor, pre: torch.Tensor, activation: str | None) -> torch.Tensor:
+    """dz = dy * act'(pre), of bf16 or f16 tensors."""
+    dt = _half("activation16_bwd", dy)
+    act = _activation("activation16_bwd", activation)
+    if pre.dtype != dy.dtype or pre.shape != dy.shape:
+        raise ValueError("activation16_bwd takes two tensors of one dtype and shape")
+    _begin("activation16_bwd", dy, pre)
+    dz = torch.empty_like(dy)
+    L.call("chelis_cuda_activation16_bwd", dt, act, dy.data_ptr(), pre.data_ptr(), dy.numel(), dz.data_ptr())
+    return dz
+
+
+def column_sums16(x: torch.Tensor) -> torch.Tensor:
+    """The f32 sums over the rows of a bf16 or f16 matrix."""
+    dt = _half("column_sums16", x)
+    if x.dim() != 2:
+        raise ValueError("column_sums16 takes a matrix")
+    _begin("column_sums16", x)
+    out = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+    L.call("chelis_cuda_column_sums16", dt, x.data_ptr(), x.shape[0], x.shape[1], out.data_ptr())
+    return out
+
+
+def matmul16_bwd(dy: torch.Tensor, a: torch.Tensor, b: torch.Tensor, trans_b: bool = False, *,
+                 through: tuple[torch.Tensor, str] | None = None, want_bias: bool = False,
+                 weight_dtype: torch.dtype = torch.float32):
+    """(da, db, dbias) of matmul16(a, b, trans_b=trans_b, bias=...) without an
+    activation; of one with an activation, given dy = activation16_bwd's.  db has
+    b's shape and weight_dtype (f32 or the operands' own), dbias is f32, None
+    without want_bias.  through=(z, activation): a was that activation taken at
+    z, and da is the gradient of z."""
+    if dy.dim() != 2 or a.dim() != 2 or b.dim() != 2 or not dy.dtype == a.dtype == b.dtype:
+        raise ValueError("matmul16_bwd takes matrices of one dtype")
+    if dy.shape != (a.shape[0], b.shape[0] if trans_b else b.shape[1]):
+        raise ValueError("matmul16_bwd: dy is not the product's shape")
+    da = matmul16(dy, b, trans_b=not trans_b, through=through)
+    if trans_b:
+        db = matmul16(dy, a, trans_a=True, dtype=weight_dtype)
+    else:
+        db = matmul16(a, dy, trans_a=True, dtype=weight_dtype)
+    return da, db, column_sums16(dy) if want_bias else None
+
+
+class ResidualNormGrads(NamedTuple):
+    """residual_norm_bwd's; None for what the forward call did not have."""
+    dx: torch.Tensor
+    dbranch: torch.Tensor | None
+    dpost_gamma: torch.Tensor | None
+    dpost_beta: torch.Tensor | None
+    dgate: torch.Tensor | None
+    dpre_gamma: torch.Tensor | None
+    dpre_beta: torch.Tensor | None
+
+
+def _check_norm(name, x, post_gamma, post_beta, gate, pre_gamma, pre_beta, kind):
+    """(dtype, kind, rows, hidden, groups) of residual_norm's arguments."""
+    dt = _act(name, x)
+    if kind not in _NORM:
+        raise ValueError(f"{name}: kinds are layer and rms")
+    if x.dim() < 2:
+        raise ValueError(f"{name} takes rows [..., hidden]")
+    hidden = x.shape[-1]
+    rows = x.numel() // hidden if hidden else 0
+    for t in (post_gamma, post_beta, pre_gamma, pre_beta):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (hidden,)):
+            raise ValueError(f"{name}: gammas and betas are f32 [hidden]")
+    if (post_beta is not None and post_gamma is None) or (pre_beta is not None and pre_gamma is None):
+        raise ValueError(f"{name}: a beta without its gamma")
+    groups = 1
+    if gate is not None:
+        if gate.dtype != torch.float32 or gate.dim() not in (1, 2) or gate.shape[-1] != hidden:
+            raise ValueError(f"{name}: a gate is f32 [hidden] or [groups, hidden]")
+        groups = gate.shape[0] if gate.dim() == 2 else 1
+        if groups < 1 or rows % groups:
+            raise ValueError(f"{name}: the gate's groups divide the rows")
+    return dt, _NORM[kind], rows, hidden, groups
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, *, post_gamma: torch.Tensor | None = None,
+                  post_beta: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                  scale: float = 1.0, pre_gamma: torch.Tensor | None = None,
+                  pre_beta: torch.Tensor | None = None, eps: float = 1e-5, kind: str = "layer"):
+    """What stands between two blocks, in one pass over the rows [..., hidden]:
+    (y, h) with y = scale * x + gate * N(branch) and h = N(y), each norm with its
+    own gamma and beta and left out without a gamma (h is None then), the gate
+    [hidden], [groups, hidden] (equal runs of rows) or None.  kind is layer or rms.
+    x, branch, y and h are f32, bf16 or f16, the parameters f32; h is taken of y
+    before it is rounded.  With branch None: (x, N(x)), the first norm of all."""
+    dt, norm, rows, hidden, groups = _check_norm("residual_norm", x, post_gamma, post_beta, gate, pre_gamma,
+                                                 pre_beta, kind)
+    if branch is None:
+        if post_gamma is not None or gate is not None or scale != 1.0 or pre_gamma is None:
+            raise ValueError("residual_norm: without a branch there is the second norm alone")
+    elif branch.shape != x.shape or branch.dtype != x.dtype:
+        raise ValueError("residual_norm: x and branch are of one dtype and shape")
+    _begin("residual_norm", x, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    y = None if branch is None else torch.empty_like(x)
+    h = None if pre_gamma is None else torch.empty_like(x)
+    L.call("chelis_cuda_residual_norm", dt, norm, rows, hidden, x.data_ptr(), _ptr(branch), _ptr(post_gamma),
+           _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma), _ptr(pre_beta), float(eps),
+           _ptr(y), _ptr(h))
+    return x if y is None else y, h
+
+
+def residual_norm_bwd(dy: torch.Tensor | None, dh: torch.Tensor | None, y: torch.Tensor,
+                      branch: torch.Tensor | None, *, post_gamma: torch.Tensor | None = None,
+                      post_beta: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                      scale: float = 1.0, pre_gamma: torch.Tensor | None = None,
+                      pre_beta: torch.Tensor | None = None, eps: float = 1e-5,
+                      kind: str = "layer") -> ResidualNormGrads:
+    """The gradients of residual_norm, from dy (None: nothing else reads y) and
+    dh (with pre_gamma), its result y, its branch and its parameters."""
+    dt, norm, rows, hidden, groups = _check_norm("residual_norm_bwd", y, post_gamma, post_beta, gate, pre_gamma,
+                                                 pre_beta, kind)
+    if (dh is None) != (pre_gamma is None):
+        raise ValueError("residual_norm_bwd: dh goes with pre_gamma")
+    if dy is None and dh is None:
+        raise ValueError("residual_norm_bwd takes dy, dh or both")
+    if branch is None and (post_gamma is not None or gate is not None or scale != 1.0):
+        raise ValueError("residual_norm_bwd: without a branch there is the second norm alone")
+    for t in (dy, dh, branch):
+        if t is not None and (t.shape != y.shape or t.dtype != y.dtype):
+            raise ValueError("residual_norm_bwd: dy, dh, y and branch are of one dtype and shape")
+    _begin("residual_norm_bwd", dy, dh, y, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+
+    def like(p):
+        return None if p is None else torch.empty_like(p)
+
+    g = ResidualNormGrads(torch.empty_like(y), like(branch), like(post_gamma), like(post_beta), like(gate),
+                          like(pre_gamma), like(pre_beta))
+    L.call("chelis_cuda_residual_norm_bwd", dt, norm, rows, hidden, _ptr(dy), _ptr(dh), y.data_ptr(),
+           _ptr(branch), _ptr(post_gamma), _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma),
+           float(eps), *(_ptr(t) for t in g))
+    return g
+
+
+def expert_balance(logits: torch.Tensor, experts: torch.Tensor, mask: torch.Tensor | None = None):
+    """(loss f32 [], counts int32 [experts + 1]) of a router's logits [tokens,
+    experts] and the experts [tokens, k] that it chose: loss = E / (k N^2) sum_e
+    counts[e] sum_t softmax(logits[t])_e over the N tokens that count, all or
+    those where mask (bool [tokens]) is true; 1 where both are even.  counts are
+    the tokens' pairs by expert, then N.  An id of -1 counts nowhere."""
+    dt = _act("expert_balance", logits)
+    _check_i32("expert_balance", experts)
+    if logits.dim() != 2 or experts.dim() != 2 or experts.shape[0] != logits.shape[0]:
+        raise ValueError("expert_balance takes logits [tokens, experts] and experts [tokens, k]")
+    tokens, n = logits.shape
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != (tokens,)):
+        raise ValueError("expert_balance: mask is bool [tokens]")
+    _begin("expert_balance", logits, experts, mask)
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    counts = torch.empty(n + 1, dtype=torch.int32, device=logits.device)
+    L.call("chelis_cuda_expert_balance", dt, logits.data_ptr(), experts.data_ptr(), _ptr(mask), tokens, n,
+           experts.shape[1], loss.data_ptr(), counts.data_ptr())
+    return loss, counts
+
+
+def expert_balance_bwd(logits: torch.Tensor, counts: torch.Tensor, k: int, weight: float = 1.0,
+                       dloss: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                       add: torch.Tensor | None = None) -> torch.Tensor:
+    """dlogits = weight * dloss * (the gradient of expert_balance's loss) + add,
+    rounded once: the gradient through the probabilities, the counts held
+    constant.  dloss is an f32 scalar on the device (None: 1), add another
+    gradient of the logits (expert_route_bwd's)."""
+    dt = _act("expert_balance_bwd", logits)
+    _check_i32("expert_balance_bwd", counts)
+    if logits.dim() != 2 or counts.shape != (logits.shape[1] + 1,):
+        raise ValueError("expert_balance_bwd takes logits [tokens, experts] and expert_balance's counts")
+    tokens, n = logits.shape
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != (tokens,)):
+        raise ValueError("expert_balance_bwd: mask is bool [tokens]")
+    if dloss is not None and (dloss.dtype != torch.float32 or dloss.numel() != 1):
+        raise ValueError("expert_balance_bwd: dloss is one f32 number")
+    if add is not None and (add.dtype != logits.dtype or add.shape != logits.shape):
+        raise ValueError("expert_balance_bwd: add has the logits' dtype and shape")
+    _begin("expert_balance_bwd", logits, counts, dloss, mask, add)
+    dlogits = torch.empty_like(logits)
+    L.call("chelis_cuda_expert_balance_bwd", dt, logits.data_ptr(), counts.data_ptr(), _ptr(mask), tokens, n, k,
+           float(weight), _ptr(dloss), _ptr(add), dlogits.data_ptr())
+    return dlogits
+
+
+def _tensor_list(name: str, tensors: list):
+    """What the C entries take of a list of tensors: (pointers, sizes, dtypes),
+    host arrays."""
+    devices = {t.get_device() for t in tensors}
+    if len(devices) > 1:
+        raise ValueError(f"{name}: tensors on different devices")
+    if -1 in devices:
+        raise ValueError("chelis_b200 ops take CUDA tensors (device memory)")
+    if not all([t.is_contiguous() for t in tensors]):
+        raise ValueError("chelis_b200 ops take contiguous tensors")
+    _on_device(name, devices.pop() if devices else -1)
+    try:
+        dtypes = array.array("i", [_ACT[t.dtype] for t in tensors])
+    except KeyError:
+        raise ValueError(f"{name} takes f32, bf16 or f16 tensors") from None
+    return (array.array("Q", [t.data_ptr() for t in tensors]),
+            array.array("q", [t.numel() for t in tensors]), dtypes)
+
+
+def _address(a: array.array) -> int:
+    return a.buffer_info()[0]
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """The Euclidean norm over all numbers of a list of f32, bf16 or f16
+    tensors, an f32 scalar on the device; sums in f64."""
+    grads = list(grads)
+    src = _tensor_list("grad_norm", grads)
+    norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
+    L.call("chelis_cuda_grad_norm", len(grads), *map(_address, src), norm.data_ptr())
+    return norm
+
+
+def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
+    """Scale a list of f32, bf16 or f16 tensors by min(1, max_norm / norm), norm
+    their grad_norm, which is returned: in place, or with out into tensors of the
+    same sizes (f32, bf16 or f16), which are written in any case.  A norm that is
+    not finite changes nothing.  Tensors that overlap are refused."""
+    grads = list(grads)
+    src = dst = _tensor_list("clip_grads", grads)
+    if out is not None:
+        out = list(out)
+        dst = _tensor_list("clip_grads", out)
+        if dst[1] != src[1]:
+            raise ValueError("clip_grads: out has the gradients' sizes")
+        if out and out[0].get_device() != grads[0].get_device():
+            raise ValueError("clip_grads: tensors on different devices")
+    norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
+    L.call("chelis_cuda_clip_grads", len(grads), *map(_address, src), _address(dst[0]), _address(dst[2]),
+           float(max_norm), norm.data_ptr())
+    return norm

@@ -686,6 +686,86 @@ int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int
                               int any_scales, int32_t out_dtype, void *out);
 
 /* =========================================================================
+ * A feed-forward sublayer in 16 bits: the product with what follows it, the
+ * norms around a block, the router's balance loss, gradient clipping.  New: the
+ * reference has none of them.  Arguments of one call must not overlap unless
+ * said otherwise.
+ * ========================================================================= */
+enum { CHELIS_ACT_NONE = 0, CHELIS_ACT_RELU = 1, CHELIS_ACT_GELU = 2, CHELIS_ACT_SILU = 3 };
+/* z = op(a) . op(b) + bias and out = act(z) + residual, [m][n] of out_dtype, from
+ * bf16 or f16 matrices a [m][k] ([k][m] when trans_a) and b [k][n] ([n][k] when
+ * trans_b); sums f32, act taken of them, each result rounded once.  gelu is
+ * z Phi(z), silu z / (1 + e^-z).  bias [n] (f32 or dtype), residual, pre (where z
+ * is stored) and through [m][n] may be NULL; residual, pre and through have
+ * out_dtype, which is f32 or dtype.  With through, out is instead the gradient
+ * through an activation that was taken at through: (op(a) . op(b)) * act'(through);
+ * it goes with no bias, residual or pre.  residual may be out. */
+int chelis_cuda_matmul16(int32_t dtype, int trans_a, int trans_b, int64_t m, int64_t n, int64_t k,
+                         const void *a, const void *b, const void *bias, int32_t bias_dtype,
+                         int32_t activation, const void *residual, const void *through, void *pre,
+                         int32_t out_dtype, void *out);
+/* dz = dy * act'(pre), count numbers of dtype (bf16 or f16); dz may be dy. */
+int chelis_cuda_activation16_bwd(int32_t dtype, int32_t activation, const void *dy, const void *pre,
+                                 int64_t count, void *dz);
+/* out[c] = sum over rows of x [rows][cols] (bf16 or f16), f32 in a fixed order:
+ * the gradient of a bias. */
+int chelis_cuda_column_sums16(int32_t dtype, const void *x, int64_t rows, int64_t cols, float *out);
+
+/* What stands between two blocks, rows of f32, bf16 or f16 (hidden <= 8192):
+ *   u = N(branch) post_gamma + post_beta   (branch itself without post_gamma)
+ *   y = scale x + gate u                   (gate 1 when NULL)
+ *   h = N(y) pre_gamma + pre_beta          (with pre_gamma)
+ * N(v) = (v - mean) / sqrt(var + eps) (CHELIS_NORM_LAYER) or v / sqrt(mean(v^2) +
+ * eps) (CHELIS_NORM_RMS).  Parameters are f32 [hidden], betas may be NULL; gate
+ * is [groups][hidden], of which row r takes row r / (rows / groups) (groups
+ * divides rows).  h is of y before it is rounded.  branch == NULL: h = N(x) alone,
+ * with no post_gamma, gate or y and scale 1. */
+enum { CHELIS_NORM_LAYER = 0, CHELIS_NORM_RMS = 1 };
+int chelis_cuda_residual_norm(int32_t dtype, int32_t kind, int64_t rows, int64_t hidden, const void *x,
+                              const void *branch, const float *post_gamma, const float *post_beta,
+                              const float *gate, int64_t groups, float scale, const float *pre_gamma,
+                              const float *pre_beta, float eps, void *y, void *h);
+/* Its gradients, from those of y (dy, NULL for none) and h (dh, with pre_gamma).
+ * y and branch are the forward pass's; branch may be NULL where it is neither
+ * normed nor gated.  dbranch NULL: no branch.  Parameter gradients are f32 sums in
+ * a fixed order; those of absent parameters are NULL, others may be NULL together
+ * with their parameter alone. */
+int chelis_cuda_residual_norm_bwd(int32_t dtype, int32_t kind, int64_t rows, int64_t hidden,
+                                  const void *dy, const void *dh, const void *y, const void *branch,
+                                  const float *post_gamma, const float *post_beta, const float *gate,
+                                  int64_t groups, float scale, const float *pre_gamma, float eps,
+                                  void *dx, void *dbranch, float *dpost_gamma, float *dpost_beta,
+                                  float *dgate, float *dpre_gamma, float *dpre_beta);
+
+/* The load of the experts and the loss that balances it:
+ *   loss = E / (k N^2) sum_e c_e sum_t softmax(logits[t])_e
+ * over the N tokens with mask[t] != 0 (all of them when mask is NULL), c_e their
+ * pairs of expert e among ids [T][k] (-1: a pair that went nowhere); 1 where both
+ * are even, 0 without tokens.  counts [E + 1]: c, then N.  Logits of masked tokens
+ * are not read; an expert at -inf has probability 0, as all have in a row of -inf. */
+int chelis_cuda_expert_balance(int32_t dtype, const void *logits, const int32_t *ids, const uint8_t *mask,
+                               int64_t tokens, int32_t experts, int32_t k, float *loss, int32_t *counts);
+/* dlogits = add + weight * *dloss * dloss/dlogits, rounded once; add (of dtype)
+ * and dloss (1 when NULL) may be NULL; dlogits may be add.  counts is
+ * chelis_cuda_expert_balance's and is held constant. */
+int chelis_cuda_expert_balance_bwd(int32_t dtype, const void *logits, const int32_t *counts,
+                                   const uint8_t *mask, int64_t tokens, int32_t experts, int32_t k,
+                                   float weight, const float *dloss, const void *add, void *dlogits);
+
+/* *norm = sqrt(sum of g^2) over n tensors of f32, bf16 or f16 (data[i] with
+ * counts[i] numbers of dtypes[i]); f64 sums in a fixed order, so squares outside
+ * f32 are no matter (a norm outside it is infinite).  data, counts and dtypes are host arrays, read
+ * before the call returns. */
+int chelis_cuda_grad_norm(int32_t n, const void *const *data, const int64_t *counts, const int32_t *dtypes,
+                          float *norm);
+/* The same, and out[i] = data[i] * min(1, max_norm / norm), rounded once to
+ * out_dtypes[i].  out[i] may be data[i] (of one dtype); with all of them so, nothing
+ * is written where the norm is within bounds.  A norm that is not finite changes
+ * nothing.  Outputs that overlap one another, or other inputs, are refused. */
+int chelis_cuda_clip_grads(int32_t n, const void *const *data, const int64_t *counts, const int32_t *dtypes,
+                           void *const *out, const int32_t *out_dtypes, float max_norm, float *norm);
+
+/* =========================================================================
  * Generated-entry device ABI (emit.rs:838-958, `f_device`): inputs borrowed,
  * outputs newly allocated owners the caller releases.  One entry per program
  * this backend ships whole.
