@@ -67,16 +67,16 @@ __device__ __forceinline__ double squares(const float (&v)[N]) {
     return d;
 }
 
-// Numbers [lo, hi) of a tensor: single ones up to 16 bytes' alignment, packs,
-// single ones.  f(pack index...) is given the element's offset.
-template <typename T>
-__device__ __forceinline__ double chunk_squares(const T *p, int64_t count) {
+// `count` numbers by THREADS threads: single ones up to 16 bytes' alignment, packs,
+// single ones.
+template <int THREADS, typename T>
+__device__ __forceinline__ double chunk_squares(const T *p, int64_t count, int thread) {
     constexpr int N = 16 / sizeof(T), DEEP = 8;
     double sum = 0.0;
     const int64_t skew = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T);
     const int64_t head = skew < count ? skew : count, packs = (count - head) / N;
     const uint4 *q = reinterpret_cast<const uint4 *>(p + head);
-    int64_t i = threadIdx.x;
+    int64_t i = thread;
     for (; i + (DEEP - 1) * THREADS < packs; i += DEEP * THREADS) {
         uint4 u[DEEP];
 #pragma unroll
@@ -94,15 +94,22 @@ __device__ __forceinline__ double chunk_squares(const T *p, int64_t count) {
         sum += squares(v);
     }
     const int64_t tail = head + packs * N;
-    if (threadIdx.x < head) {
-        const double v = experts::to_f32(p[threadIdx.x]);
+    if (thread < head) {
+        const double v = experts::to_f32(p[thread]);
         sum = fma(v, v, sum);
     }
-    if (tail + threadIdx.x < count) {
-        const double v = experts::to_f32(p[tail + threadIdx.x]);
+    if (tail + thread < count) {
+        const double v = experts::to_f32(p[tail + thread]);
         sum = fma(v, v, sum);
     }
     return sum;
+}
+
+template <int THREADS>
+__device__ __forceinline__ double squares_part(const Entry &e, int64_t at, int64_t count, int thread) {
+    if (e.in == CHELIS_DTYPE_F32) return chunk_squares<THREADS>(static_cast<const float *>(e.src) + at, count, thread);
+    if (e.in == CHELIS_DTYPE_BF16) return chunk_squares<THREADS>(static_cast<const __nv_bfloat16 *>(e.src) + at, count, thread);
+    return chunk_squares<THREADS>(static_cast<const __half *>(e.src) + at, count, thread);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -146,9 +153,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         const Entry &e = table.t[tensor];
         const int64_t at = static_cast<int64_t>(c - e.first) * CHUNK;
         const int64_t count = e.count - at < CHUNK ? e.count - at : CHUNK;
-        if (e.in == CHELIS_DTYPE_F32) sum += chunk_squares(static_cast<const float *>(e.src) + at, count);
-        else if (e.in == CHELIS_DTYPE_BF16) sum += chunk_squares(static_cast<const __nv_bfloat16 *>(e.src) + at, count);
-        else sum += chunk_squares(static_cast<const __half *>(e.src) + at, count);
+        sum += squares_part<THREADS>(e, at, count, threadIdx.x);
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -167,15 +172,15 @@ __global__ void __launch_bounds__(THREADS)
     if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
-template <typename T, typename U>
-__device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, float c) {
+template <int THREADS, typename T, typename U>
+__device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, float c, int thread) {
     constexpr int N = 16 / sizeof(T), DEEP = 8;
     const int64_t skew = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T);
     int64_t head = skew < count ? skew : count;
     // packs want the result aligned as well as the source
     const bool packed = (reinterpret_cast<uintptr_t>(o + head) & (N * sizeof(U) - 1)) == 0;
     if (!packed) {
-        for (int64_t i = threadIdx.x; i < count; i += THREADS) o[i] = experts::from_f32<U>(experts::to_f32(p[i]) * c);
+        for (int64_t i = thread; i < count; i += THREADS) o[i] = experts::from_f32<U>(experts::to_f32(p[i]) * c);
         return;
     }
     const int64_t packs = (count - head) / N;
@@ -192,7 +197,7 @@ __device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, flo
         if constexpr (sizeof(r) == 32) gemm8::store32(o + head + i * N, reinterpret_cast<const uint32_t(&)[8]>(r));
         else *reinterpret_cast<Out *>(o + head + i * N) = r;
     };
-    int64_t i = threadIdx.x;
+    int64_t i = thread;
     for (; i + (DEEP - 1) * THREADS < packs; i += DEEP * THREADS) {
         uint4 u[DEEP];
 #pragma unroll
@@ -202,16 +207,28 @@ __device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, flo
     }
     for (; i < packs; i += THREADS) put(i, q[i]);
     const int64_t tail = head + packs * N;
-    if (threadIdx.x < head) o[threadIdx.x] = experts::from_f32<U>(experts::to_f32(p[threadIdx.x]) * c);
-    if (tail + threadIdx.x < count)
-        o[tail + threadIdx.x] = experts::from_f32<U>(experts::to_f32(p[tail + threadIdx.x]) * c);
+    if (thread < head) o[thread] = experts::from_f32<U>(experts::to_f32(p[thread]) * c);
+    if (tail + thread < count)
+        o[tail + thread] = experts::from_f32<U>(experts::to_f32(p[tail + thread]) * c);
 }
-template <typename T>
-__device__ __forceinline__ void scale_to(const Entry &e, int64_t at, int64_t count, float c) {
+template <int THREADS, typename T>
+__device__ __forceinline__ void scale_as(const Entry &e, int64_t at, int64_t count, float c, int thread) {
     const T *p = static_cast<const T *>(e.src) + at;
-    if (e.out == CHELIS_DTYPE_F32) scale_chunk(p, static_cast<float *>(e.dst) + at, count, c);
-    else if (e.out == CHELIS_DTYPE_BF16) scale_chunk(p, static_cast<__nv_bfloat16 *>(e.dst) + at, count, c);
-    else scale_chunk(p, static_cast<__half *>(e.dst) + at, count, c);
+    if (e.out == CHELIS_DTYPE_F32) scale_chunk<THREADS>(p, static_cast<float *>(e.dst) + at, count, c, thread);
+    else if (e.out == CHELIS_DTYPE_BF16) scale_chunk<THREADS>(p, static_cast<__nv_bfloat16 *>(e.dst) + at, count, c, thread);
+    else scale_chunk<THREADS>(p, static_cast<__half *>(e.dst) + at, count, c, thread);
+}
+
+template <int THREADS>
+__device__ __forceinline__ void scale_part(const Entry &e, int64_t at, int64_t count, float c, int thread) {
+    if (e.in == CHELIS_DTYPE_F32) scale_as<THREADS, float>(e, at, count, c, thread);
+    else if (e.in == CHELIS_DTYPE_BF16) scale_as<THREADS, __nv_bfloat16>(e, at, count, c, thread);
+    else scale_as<THREADS, __half>(e, at, count, c, thread);
+}
+
+// A norm that is reported as infinite or NaN changes nothing.
+__device__ __forceinline__ float factor(double norm, float max_norm) {
+    return norm > max_norm && static_cast<float>(norm) < INFINITY ? static_cast<float>(max_norm / norm) : 1.0f;
 }
 
 template <int N>
@@ -220,8 +237,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const double v = total_norm(sums, n);
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = static_cast<float>(v);
-    // a norm that is reported as infinite or NaN changes nothing
-    const float c = v > max_norm && static_cast<float>(v) < INFINITY ? static_cast<float>(max_norm / v) : 1.0f;
+    const float c = factor(v, max_norm);
     const int first = block_first(table.chunks, blockIdx.x), last = block_first(table.chunks, blockIdx.x + 1);
     int tensor = first < last ? tensor_of(table, last - 1) : 0;
     for (int chunk = last - 1; chunk >= first; --chunk) {
@@ -230,9 +246,34 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (c == 1.0f && e.src == e.dst) continue;  // as they are
         const int64_t at = static_cast<int64_t>(chunk - e.first) * CHUNK;
         const int64_t count = e.count - at < CHUNK ? e.count - at : CHUNK;
-        if (e.in == CHELIS_DTYPE_F32) scale_to<float>(e, at, count, c);
-        else if (e.in == CHELIS_DTYPE_BF16) scale_to<__nv_bfloat16>(e, at, count, c);
-        else scale_to<__half>(e, at, count, c);
+        scale_part<THREADS>(e, at, count, c, threadIdx.x);
+    }
+}
+
+// Few numbers: all of them by one block, which needs no scratch and no second
+// launch; a warp takes a chunk.
+constexpr int64_t FEW_NUMBERS = 65536;
+constexpr int FEW_CHUNK = 1024;
+
+template <bool SCALE>
+__global__ void __launch_bounds__(THREADS)
+    small_kernel(const __grid_constant__ Table<FEW> table, float max_norm, float *norm) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    double sum = 0.0;
+    for (int c = warp; c < table.chunks; c += THREADS / 32) {
+        const Entry &e = table.t[tensor_of(table, c)];
+        const int64_t at = static_cast<int64_t>(c - e.first) * FEW_CHUNK;
+        sum += squares_part<32>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, lane);
+    }
+    const double v = sqrt(block_sum(sum));
+    if (threadIdx.x == 0) *norm = static_cast<float>(v);
+    if (!SCALE) return;
+    const float f = factor(v, max_norm);
+    for (int c = warp; c < table.chunks; c += THREADS / 32) {
+        const Entry &e = table.t[tensor_of(table, c)];
+        if (f == 1.0f && e.src == e.dst) continue;
+        const int64_t at = static_cast<int64_t>(c - e.first) * FEW_CHUNK;
+        scale_part<32>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, f, lane);
     }
 }
 
@@ -309,7 +350,7 @@ int launch_after(void (*kernel)(Args...), unsigned grid, const char *name, Given
 constexpr int NORM_BLOCKS = 2, SCALE_BLOCKS = 2;  // a multiprocessor
 
 // f(table) for tensors `first` on, as many as a table has; the next first.
-template <int N, typename F>
+template <int N, int CHUNK, typename F>
 int with_table(int32_t *first, int32_t n, const void *const *data, const int64_t *counts, const int32_t *dtypes,
                void *const *out, const int32_t *out_dtypes, F f) {
     Table<N> table;
@@ -331,6 +372,20 @@ template <int N>
 int run(int32_t n, const void *const *data, const int64_t *counts, const int32_t *dtypes, void *const *out,
         const int32_t *out_dtypes, float max_norm, float *norm) {
     cudaStream_t s = current_stream();
+    if constexpr (N == FEW) {
+        int64_t numbers = 0;
+        for (int32_t i = 0; i < n && numbers <= FEW_NUMBERS; ++i) numbers += counts[i];
+        if (numbers <= FEW_NUMBERS) {
+            int32_t first = 0;
+            return with_table<FEW, FEW_CHUNK>(&first, n, data, counts, dtypes, out, out_dtypes, [&](const Table<FEW> &table) -> int {
+                if (out) small_kernel<true><<<1, THREADS, 0, s>>>(table, max_norm, norm);
+                else small_kernel<false><<<1, THREADS, 0, s>>>(table, max_norm, norm);
+                g_launches++;
+                CHELIS_LAUNCH_CHECK("clip::small_kernel");
+                return CHELIS_CUDA_OK;
+            });
+        }
+    }
     const int64_t tables = (static_cast<int64_t>(n) + N - 1) / N, most = sm_count() * NORM_BLOCKS;
     void *scratch = nullptr;
     CHELIS_TRY(scratch_alloc(&scratch, static_cast<size_t>((tables < 1 ? 1 : tables) * most) * sizeof(double), s));
@@ -338,7 +393,7 @@ int run(int32_t n, const void *const *data, const int64_t *counts, const int32_t
     auto body = [&]() -> int {
         int blocks = 0;
         for (int32_t first = 0; first < n;)
-            CHELIS_TRY(with_table<N>(&first, n, data, counts, dtypes, out, out_dtypes, [&](const Table<N> &table) -> int {
+            CHELIS_TRY((with_table<N, CHUNK>(&first, n, data, counts, dtypes, out, out_dtypes, [&](const Table<N> &table) -> int {
                 if (table.chunks == 0) return CHELIS_CUDA_OK;
                 const unsigned grid = grid_of(table.chunks, NORM_BLOCKS);
                 norm_kernel<N><<<grid, THREADS, 0, s>>>(table, sums + blocks);
@@ -346,18 +401,18 @@ int run(int32_t n, const void *const *data, const int64_t *counts, const int32_t
                 CHELIS_LAUNCH_CHECK("clip::norm_kernel");
                 blocks += static_cast<int>(grid);
                 return CHELIS_CUDA_OK;
-            }));
+            })));
         if (!out || blocks == 0)
             return launch_after(total_kernel, 1, "clip::total_kernel", static_cast<const double *>(sums), blocks, norm);
         float *report = norm;  // by the first launch alone
         for (int32_t first = 0; first < n;)
-            CHELIS_TRY(with_table<N>(&first, n, data, counts, dtypes, out, out_dtypes, [&](const Table<N> &table) -> int {
+            CHELIS_TRY((with_table<N, CHUNK>(&first, n, data, counts, dtypes, out, out_dtypes, [&](const Table<N> &table) -> int {
                 if (table.chunks == 0) return CHELIS_CUDA_OK;
                 CHELIS_TRY(launch_after(scale_kernel<N>, grid_of(table.chunks, SCALE_BLOCKS), "clip::scale_kernel", table,
                                         static_cast<const double *>(sums), blocks, max_norm, report));
                 report = nullptr;
                 return CHELIS_CUDA_OK;
-            }));
+            })));
         return CHELIS_CUDA_OK;
     };
     const int rc = body();

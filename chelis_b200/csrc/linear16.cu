@@ -609,21 +609,27 @@ __global__ void __launch_bounds__(256)
 
 // ---- unaligned operands ---------------------------------------------------
 // [rows][cols] to rows of ld = cols rounded up to 8 (TMA's 16 bytes); the last
-// columns are never read as the map ends at cols.
+// columns are never read as the map ends at cols.  Both operands' copies in one
+// launch.
+struct Repack {
+    const uint16_t *src;
+    uint16_t *dst;      // NULL: none
+    int64_t rows, cols, ld;
+};
 __global__ void __launch_bounds__(256)
-    repack_kernel(const uint16_t *__restrict__ src, int64_t rows, int64_t cols, int64_t ld, uint16_t *__restrict__ dst) {
-    const int64_t groups = ld / 8, all = rows * groups;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t row = i / groups, c = (i - row * groups) * 8;
-        const uint16_t *s = src + row * cols + c;
+    repack_kernel(const Repack a, const Repack b) {
+    const int64_t first = a.dst ? a.rows * (a.ld / 8) : 0, all = first + (b.dst ? b.rows * (b.ld / 8) : 0);
+    for (int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; j < all; j += static_cast<int64_t>(gridDim.x) * 256) {
+        const Repack &p = j < first ? a : b;
+        const int64_t i = j < first ? j : j - first, groups = p.ld / 8, row = i / groups, c = (i - row * groups) * 8;
+        const uint16_t *s = p.src + row * p.cols + c;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = c + 2 * j < cols ? s[2 * j] : 0, hi = c + 2 * j + 1 < cols ? s[2 * j + 1] : 0;
-            w[j] = lo | hi << 16;
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = c + 2 * k < p.cols ? __ldg(s + 2 * k) : 0, hi = c + 2 * k + 1 < p.cols ? __ldg(s + 2 * k + 1) : 0;
+            w[k] = lo | hi << 16;
         }
-        *reinterpret_cast<uint4 *>(dst + row * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(p.dst + row * p.ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -644,7 +650,18 @@ __global__ void __launch_bounds__(256)
 // n = 8 g .. 8 g + 7 of rows k = 4 t .. 4 t + 3; pairs of k are put together from
 // two rows (PRMT), and MMA j of four has n = 8 g + 2 j and 8 g + 2 j + 1.
 constexpr int FEW_WARPS = 8;
-constexpr int FEW_ROWS = 32;
+
+// Whether few_kernel takes a product: up to 16 rows it reads the weights once, and
+// does so faster than the pairs fill their tiles, of which rows are mostly missing;
+// more rows read them again, which pays while that costs less than the pairs' set-up.
+// us in a graph, pairs and few: 8 rows 1024 x 1024 10.6, 4.8, of [n][k] 10.5, 3.6;
+// 4096 x 4096 20.5, 12.0; 16 rows 16384 x 4096 30.8, 32.7; 32 rows 4096 x 1024 11.4,
+// 10.1, 4096 x 4096 19.8, 19.4, 16384 x 1024 14.9, 21.9; 64 rows 1024 x 1024 10.6, 7.8,
+// 4096 x 1024 11.5, 11.7.
+bool few_rows(int64_t m, int64_t n, int64_t k) {
+    const int64_t passes = (m + 15) / 16;
+    return passes == 1 || (passes <= 4 && n <= (int64_t{1} << 23) / passes / k);
+}
 
 __device__ __forceinline__ uint4 load8(const uint16_t *p, int64_t left, bool vec) {
     if (left <= 0) return make_uint4(0, 0, 0, 0);
@@ -873,19 +890,12 @@ int make_map(CUtensorMap *map, const void *base, int64_t cols, int64_t ld, int64
 }
 
 // An operand as TMA can read it: itself, or a copy whose rows start on 16 bytes.
-int aligned_operand(const void *src, int64_t rows, int64_t cols, const void **out, void **copy, int64_t *ld, cudaStream_t s) {
-    *copy = nullptr;
-    *out = src;
-    *ld = cols;
-    if (cols % 8 == 0 && experts::aligned16(src)) return CHELIS_CUDA_OK;
-    *ld = round8(cols);
-    CHELIS_TRY(scratch_alloc(copy, static_cast<size_t>(rows) * *ld * 2, s));
-    repack_kernel<<<blocks8::grid_for((rows * *ld / 8 + 255) / 256, 16), 256, 0, s>>>(
-        static_cast<const uint16_t *>(src), rows, cols, *ld, static_cast<uint16_t *>(*copy));
-    g_launches++;
-    *out = *copy;
-    return check_cuda(cudaGetLastError(), "linear16::repack_kernel");
+Repack repack_of(const void *src, int64_t rows, int64_t cols) {
+    Repack r{static_cast<const uint16_t *>(src), nullptr, rows, cols, cols};
+    if (cols % 8 != 0 || !experts::aligned16(src)) r.ld = round8(cols);
+    return r;
 }
+bool needs_copy(const Repack &r) { return r.ld != r.cols || !experts::aligned16(r.src); }
 
 int join(const float *parts, int32_t count, int64_t m, int64_t n, const Finish &f, cudaStream_t s) {
     if (n % 4 == 0)
@@ -954,17 +964,28 @@ int run_pairs(bool bf, bool amn, bool bmn, int64_t m, int64_t n, int64_t k, cons
     if (tiles > INT32_MAX / 256)
         return set_error(CHELIS_CUDA_ERR_UNSUPPORTED, "matmul16: more than 2^23 tiles of 256 x 256");
     p.parts = gemm8::part_count(tiles, p.kblocks, sm_count() / 2, 4, 16);
-    void *copy_a = nullptr, *copy_b = nullptr, *sums = nullptr;
+    Repack ra = repack_of(a, amn ? k : m, amn ? m : k), rb = repack_of(b, bmn ? k : n, bmn ? n : k);
+    void *scratch = nullptr;
     auto body = [&]() -> int {
-        const void *pa, *pb;
-        int64_t lda, ldb;
-        CHELIS_TRY(aligned_operand(a, amn ? k : m, amn ? m : k, &pa, &copy_a, &lda, s));
-        CHELIS_TRY(aligned_operand(b, bmn ? k : n, bmn ? n : k, &pb, &copy_b, &ldb, s));
+        // scratch: the operands' copies, the parts' results
+        const size_t size_a = needs_copy(ra) ? static_cast<size_t>(ra.rows) * ra.ld * 2 : 0;
+        const size_t size_b = needs_copy(rb) ? static_cast<size_t>(rb.rows) * rb.ld * 2 : 0;
+        const size_t size_sums = p.parts > 1 ? static_cast<size_t>(p.parts) * m * n * sizeof(float) : 0;
+        CHELIS_TRY(scratch_alloc(&scratch, size_a + size_b + size_sums, s));  // the sizes are multiples of 16
+        unsigned char *at = static_cast<unsigned char *>(scratch);
+        if (size_a) ra.dst = reinterpret_cast<uint16_t *>(at);
+        if (size_b) rb.dst = reinterpret_cast<uint16_t *>(at + size_a);
+        if (size_a + size_b) {
+            repack_kernel<<<blocks8::grid_for(static_cast<int64_t>((size_a + size_b) / 16 + 255) / 256, 16), 256, 0, s>>>(ra, rb);
+            g_launches++;
+            CHELIS_LAUNCH_CHECK("linear16::repack_kernel");
+        }
+        const void *pa = ra.dst ? ra.dst : a, *pb = rb.dst ? rb.dst : b;
         CUtensorMap ma, mb;
-        CHELIS_TRY(amn ? make_map(&ma, pa, m, lda, k, 64, bf) : make_map(&ma, pa, k, lda, m, 128, bf));
-        CHELIS_TRY(bmn ? make_map(&mb, pb, n, ldb, k, 64, bf) : make_map(&mb, pb, k, ldb, n, p.tn / 2, bf));
+        CHELIS_TRY(amn ? make_map(&ma, pa, m, ra.ld, k, 64, bf) : make_map(&ma, pa, k, ra.ld, m, 128, bf));
+        CHELIS_TRY(bmn ? make_map(&mb, pb, n, rb.ld, k, 64, bf) : make_map(&mb, pb, k, rb.ld, n, p.tn / 2, bf));
+        void *sums = at + size_a + size_b;
         if (p.parts > 1) {
-            CHELIS_TRY(scratch_alloc(&sums, static_cast<size_t>(p.parts) * m * n * sizeof(float), s));
             p.f = Finish{};
             p.f.out = sums;
             p.f.dtype = CHELIS_DTYPE_F32;
@@ -974,9 +995,7 @@ int run_pairs(bool bf, bool amn, bool bmn, int64_t m, int64_t n, int64_t k, cons
         return CHELIS_CUDA_OK;
     };
     const int rc = body();
-    scratch_free(sums, s);
-    scratch_free(copy_b, s);
-    scratch_free(copy_a, s);
+    scratch_free(scratch, s);
     return rc;
 }
 
@@ -1061,7 +1080,7 @@ extern "C" int chelis_cuda_matmul16(int32_t dtype, int trans_a, int trans_b, int
     f.aux_kind = residual ? linear16::AUX_RESIDUAL : through ? linear16::AUX_THROUGH : linear16::AUX_NONE;
     if (k == 0) return linear16::join(nullptr, 0, m, n, f, current_stream());
     const bool bf = dtype == CHELIS_DTYPE_BF16;
-    if (!trans_a && m <= linear16::FEW_ROWS) {
+    if (!trans_a && linear16::few_rows(m, n, k)) {
         if (trans_b) return bf ? linear16::run_few<true, false>(m, n, k, a, b, f) : linear16::run_few<false, false>(m, n, k, a, b, f);
         return bf ? linear16::run_few<true, true>(m, n, k, a, b, f) : linear16::run_few<false, true>(m, n, k, a, b, f);
     }

@@ -38,6 +38,77 @@ using experts::warp_sum;
 
 constexpr int MAX_HIDDEN = 8192;
 
+// Two values at a time where packs have pairs (packed f32 instructions): v + s, v a +
+// s, v a + w of N of them.
+using gemm8::f32x2;
+using gemm8::pack2;
+using gemm8::unpack2;
+template <int N>
+__device__ __forceinline__ void affine(float (&v)[N], float a, float s) {
+    if constexpr (N % 2 == 0) {
+        const f32x2 a2 = pack2(a, a), s2 = pack2(s, s);
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const float2 r = unpack2(gemm8::fma2(pack2(v[c], v[c + 1]), a2, s2));
+            v[c] = r.x, v[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = fmaf(v[c], a, s);
+    }
+}
+template <int N>
+__device__ __forceinline__ void multiply_add(float (&v)[N], const float (&a)[N], const float (&s)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const float2 r = unpack2(gemm8::fma2(pack2(v[c], v[c + 1]), pack2(a[c], a[c + 1]), pack2(s[c], s[c + 1])));
+            v[c] = r.x, v[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = fmaf(v[c], a[c], s[c]);
+    }
+}
+// Sum of v, and of the squares about `centre`.
+template <int N>
+__device__ __forceinline__ float values_sum(const float (&v)[N]) {
+    if constexpr (N % 2 == 0) {
+        f32x2 s = pack2(v[0], v[1]);
+#pragma unroll
+        for (int c = 2; c < N; c += 2) s = gemm8::add2(s, pack2(v[c], v[c + 1]));
+        const float2 r = unpack2(s);
+        return r.x + r.y;
+    } else {
+        float s = v[0];
+#pragma unroll
+        for (int c = 1; c < N; ++c) s += v[c];
+        return s;
+    }
+}
+template <int N>
+__device__ __forceinline__ float squares_about(const float *v, float centre) {
+    if constexpr (N % 2 == 0) {
+        const f32x2 m = pack2(-centre, -centre);
+        f32x2 q = 0ull;
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const f32x2 d = gemm8::add2(pack2(v[c], v[c + 1]), m);
+            q = gemm8::fma2(d, d, q);
+        }
+        const float2 r = unpack2(q);
+        return r.x + r.y;
+    } else {
+        float q = 0.0f;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            const float d = v[c] - centre;
+            q = fmaf(d, d, q);
+        }
+        return q;
+    }
+}
+
 struct Params {
     int64_t rows;
     int32_t hidden, rms;
@@ -259,11 +330,8 @@ struct Team {
                                            float *r_u, float *mean_v, float *r_v) {
         float su = 0.0f, sv = 0.0f, sum = 0.0f, cu = 0.0f, cv = 0.0f;
         if (!rms) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) su += u[e];
-            if (two)
-#pragma unroll
-                for (int e = 0; e < E; ++e) sv += v[e];
+            su = values_sum<E>(u);
+            if (two) sv = values_sum<E>(v);
             sum = halves_sum(su, sv);
             both(sum * own_inv, cu, cv);
         }
@@ -271,17 +339,8 @@ struct Team {
 #pragma unroll
         for (int i = 0; i < PACKS; ++i)
             if (in[i]) {
-#pragma unroll
-                for (int c = 0; c < N; ++c) {
-                    const float d = u[i * N + c] - cu;
-                    qu = fmaf(d, d, qu);
-                }
-                if (two)
-#pragma unroll
-                    for (int c = 0; c < N; ++c) {
-                        const float d = v[i * N + c] - cv;
-                        qv = fmaf(d, d, qv);
-                    }
+                qu += squares_about<N>(u + i * N, cu);
+                if (two) qv += squares_about<N>(v + i * N, cv);
             }
         float q = halves_sum(qu, qv), mean = sum * own_inv;
         if constexpr (W > 1) {
@@ -364,12 +423,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < PACKS; ++i)
                 if (team.in[i]) {
                     float x[N], k[N];
+                    float(&w)[N] = *reinterpret_cast<float(*)[N]>(&v[i * N]);
                     if (staged) {
                         float z[N];
                         team.staged(c1, i, k);
                         team.staged(c0, i, z);
-#pragma unroll
-                        for (int c = 0; c < N; ++c) v[i * N + c] = fmaf(fmaf(v[i * N + c], r, shift), k[c], z[c]);
+                        affine<N>(w, r, shift);
+                        multiply_add<N>(w, k, z);
                     } else if (post) {
                         team.params(p.post_gamma, 1.0f, i, k);
 #pragma unroll
@@ -386,8 +446,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int c = 0; c < N; ++c) v[i * N + c] *= k[c];
                     }
                     team.value(in, 0, 0, row, i, x);
+                    float scale[N];
 #pragma unroll
-                    for (int c = 0; c < N; ++c) v[i * N + c] = fmaf(p.scale, x[c], v[i * N + c]);
+                    for (int c = 0; c < N; ++c) scale[c] = p.scale;
+                    multiply_add<N>(x, scale, w);
+#pragma unroll
+                    for (int c = 0; c < N; ++c) w[c] = x[c];
                     team.store(p.y, row, i, [&](int e) { return v[e]; });
                 }
         }
@@ -405,7 +469,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                         team.params(p.pre_gamma, 0.0f, i, g);
                         team.params(p.pre_beta, 0.0f, i, k);
                     }
-                    team.store(p.h, row, i, [&](int e) { return fmaf(fmaf(v[e], r, shift), g[e % N], k[e % N]); });
+                    float(&w)[N] = *reinterpret_cast<float(*)[N]>(&v[i * N]);
+                    affine<N>(w, r, shift);
+                    multiply_add<N>(w, g, k);
+                    team.store(p.h, row, i, [&](int e) { return v[e]; });
                 }
         }
         if (VEC) {

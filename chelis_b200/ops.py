@@ -11,6 +11,7 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -826,6 +827,21 @@ def matmul8_wgrad(dy: Blocks8, x: Blocks8, offsets: torch.Tensor | None = None,
 _HALF = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
 _ACTIVATION = {None: L.ACT_NONE, "relu": L.ACT_RELU, "gelu": L.ACT_GELU, "silu": L.ACT_SILU}
 _NORM = {"layer": L.NORM_LAYER, "rms": L.NORM_RMS}
+_dtype_of = operator.attrgetter("dtype")
+
+
+_entries: dict[str, object] = {}
+
+
+def _call(name: str, *args) -> None:
+    """L.call with the entry looked up once: these calls are mostly the host's
+    where few tokens are concerned."""
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(L.load(), name)
+    status = f(*args)
+    if status:
+        L.check(status)
 
 
 def _begin(name: str, *tensors: torch.Tensor | None) -> None:
@@ -851,9 +867,9 @@ def _on_device(name: str, dev: int) -> None:
     if dev >= 0 and dev != current:
         raise ValueError(f"{name}: the tensors' device is not the current one")
     if current not in _initialised:
-        L.call("chelis_cuda_init", current)
+        _call("chelis_cuda_init", current)
         _initialised.add(current)
-    L.load().chelis_cuda_set_stream(_raw_stream(current))
+    _call("chelis_cuda_set_stream", _raw_stream(current))
 
 
 def _half(name: str, t: torch.Tensor) -> int:
@@ -906,7 +922,7 @@ def matmul16(a: torch.Tensor, b: torch.Tensor, trans_a: bool = False, trans_b: b
     _begin("matmul16", a, b, bias, residual, z)
     out = torch.empty(m, n, dtype=dtype, device=a.device)
     pre = torch.empty_like(out) if keep_pre else None
-    L.call("chelis_cuda_matmul16", dt, int(trans_a), int(trans_b), m, n, k, a.data_ptr(), b.data_ptr(),
+    _call("chelis_cuda_matmul16", dt, int(trans_a), int(trans_b), m, n, k, a.data_ptr(), b.data_ptr(),
            _ptr(bias), 0 if bias is None else _ACT[bias.dtype], act, _ptr(residual), _ptr(z), _ptr(pre),
            _ACT[dtype], out.data_ptr())
     return (out, pre) if keep_pre else out
@@ -920,7 +936,7 @@ def activation16_bwd(dy: torch.Tensor, pre: torch.Tensor, activation: str | None
         raise ValueError("activation16_bwd takes two tensors of one dtype and shape")
     _begin("activation16_bwd", dy, pre)
     dz = torch.empty_like(dy)
-    L.call("chelis_cuda_activation16_bwd", dt, act, dy.data_ptr(), pre.data_ptr(), dy.numel(), dz.data_ptr())
+    _call("chelis_cuda_activation16_bwd", dt, act, dy.data_ptr(), pre.data_ptr(), dy.numel(), dz.data_ptr())
     return dz
 
 
@@ -931,7 +947,7 @@ def column_sums16(x: torch.Tensor) -> torch.Tensor:
         raise ValueError("column_sums16 takes a matrix")
     _begin("column_sums16", x)
     out = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
-    L.call("chelis_cuda_column_sums16", dt, x.data_ptr(), x.shape[0], x.shape[1], out.data_ptr())
+    _call("chelis_cuda_column_sums16", dt, x.data_ptr(), x.shape[0], x.shape[1], out.data_ptr())
     return out
 
 
@@ -1010,7 +1026,7 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, *, post_gamma: t
     _begin("residual_norm", x, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
     y = None if branch is None else torch.empty_like(x)
     h = None if pre_gamma is None else torch.empty_like(x)
-    L.call("chelis_cuda_residual_norm", dt, norm, rows, hidden, x.data_ptr(), _ptr(branch), _ptr(post_gamma),
+    _call("chelis_cuda_residual_norm", dt, norm, rows, hidden, x.data_ptr(), _ptr(branch), _ptr(post_gamma),
            _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma), _ptr(pre_beta), float(eps),
            _ptr(y), _ptr(h))
     return x if y is None else y, h
@@ -1042,7 +1058,7 @@ def residual_norm_bwd(dy: torch.Tensor | None, dh: torch.Tensor | None, y: torch
 
     g = ResidualNormGrads(torch.empty_like(y), like(branch), like(post_gamma), like(post_beta), like(gate),
                           like(pre_gamma), like(pre_beta))
-    L.call("chelis_cuda_residual_norm_bwd", dt, norm, rows, hidden, _ptr(dy), _ptr(dh), y.data_ptr(),
+    _call("chelis_cuda_residual_norm_bwd", dt, norm, rows, hidden, _ptr(dy), _ptr(dh), y.data_ptr(),
            _ptr(branch), _ptr(post_gamma), _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma),
            float(eps), *(_ptr(t) for t in g))
     return g
@@ -1053,7 +1069,8 @@ def expert_balance(logits: torch.Tensor, experts: torch.Tensor, mask: torch.Tens
     experts] and the experts [tokens, k] that it chose: loss = E / (k N^2) sum_e
     counts[e] sum_t softmax(logits[t])_e over the N tokens that count, all or
     those where mask (bool [tokens]) is true; 1 where both are even.  counts are
-    the tokens' pairs by expert, then N.  An id of -1 counts nowhere."""
+    the tokens' pairs by expert, then N.  An id of -1 counts nowhere; other ids
+    outside [0, experts) too, and they raise at the next device_status()."""
     dt = _act("expert_balance", logits)
     _check_i32("expert_balance", experts)
     if logits.dim() != 2 or experts.dim() != 2 or experts.shape[0] != logits.shape[0]:
@@ -1064,7 +1081,7 @@ def expert_balance(logits: torch.Tensor, experts: torch.Tensor, mask: torch.Tens
     _begin("expert_balance", logits, experts, mask)
     loss = torch.empty((), dtype=torch.float32, device=logits.device)
     counts = torch.empty(n + 1, dtype=torch.int32, device=logits.device)
-    L.call("chelis_cuda_expert_balance", dt, logits.data_ptr(), experts.data_ptr(), _ptr(mask), tokens, n,
+    _call("chelis_cuda_expert_balance", dt, logits.data_ptr(), experts.data_ptr(), _ptr(mask), tokens, n,
            experts.shape[1], loss.data_ptr(), counts.data_ptr())
     return loss, counts
 
@@ -1089,7 +1106,7 @@ def expert_balance_bwd(logits: torch.Tensor, counts: torch.Tensor, k: int, weigh
         raise ValueError("expert_balance_bwd: add has the logits' dtype and shape")
     _begin("expert_balance_bwd", logits, counts, dloss, mask, add)
     dlogits = torch.empty_like(logits)
-    L.call("chelis_cuda_expert_balance_bwd", dt, logits.data_ptr(), counts.data_ptr(), _ptr(mask), tokens, n, k,
+    _call("chelis_cuda_expert_balance_bwd", dt, logits.data_ptr(), counts.data_ptr(), _ptr(mask), tokens, n, k,
            float(weight), _ptr(dloss), _ptr(add), dlogits.data_ptr())
     return dlogits
 
@@ -1097,20 +1114,20 @@ def expert_balance_bwd(logits: torch.Tensor, counts: torch.Tensor, k: int, weigh
 def _tensor_list(name: str, tensors: list):
     """What the C entries take of a list of tensors: (pointers, sizes, dtypes),
     host arrays."""
-    devices = {t.get_device() for t in tensors}
+    devices = set(map(torch.Tensor.get_device, tensors))
     if len(devices) > 1:
         raise ValueError(f"{name}: tensors on different devices")
     if -1 in devices:
         raise ValueError("chelis_b200 ops take CUDA tensors (device memory)")
-    if not all([t.is_contiguous() for t in tensors]):
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
         raise ValueError("chelis_b200 ops take contiguous tensors")
     _on_device(name, devices.pop() if devices else -1)
     try:
-        dtypes = array.array("i", [_ACT[t.dtype] for t in tensors])
+        dtypes = array.array("i", map(_ACT.__getitem__, map(_dtype_of, tensors)))
     except KeyError:
         raise ValueError(f"{name} takes f32, bf16 or f16 tensors") from None
-    return (array.array("Q", [t.data_ptr() for t in tensors]),
-            array.array("q", [t.numel() for t in tensors]), dtypes)
+    return (array.array("Q", map(torch.Tensor.data_ptr, tensors)),
+            array.array("q", map(torch.Tensor.numel, tensors)), dtypes)
 
 
 def _address(a: array.array) -> int:
@@ -1123,7 +1140,7 @@ def grad_norm(grads) -> torch.Tensor:
     grads = list(grads)
     src = _tensor_list("grad_norm", grads)
     norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
-    L.call("chelis_cuda_grad_norm", len(grads), *map(_address, src), norm.data_ptr())
+    _call("chelis_cuda_grad_norm", len(grads), *map(_address, src), norm.data_ptr())
     return norm
 
 
@@ -1133,15 +1150,16 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     same sizes (f32, bf16 or f16), which are written in any case.  A norm that is
     not finite changes nothing.  Tensors that overlap are refused."""
     grads = list(grads)
-    src = dst = _tensor_list("clip_grads", grads)
-    if out is not None:
-        out = list(out)
-        dst = _tensor_list("clip_grads", out)
-        if dst[1] != src[1]:
+    n, own = len(grads), out is None
+    if not own:
+        grads += out
+        if len(grads) != 2 * n:
             raise ValueError("clip_grads: out has the gradients' sizes")
-        if out and out[0].get_device() != grads[0].get_device():
-            raise ValueError("clip_grads: tensors on different devices")
+    ptrs, counts, dtypes = _tensor_list("clip_grads", grads)
+    if not own and counts[:n] != counts[n:]:
+        raise ValueError("clip_grads: out has the gradients' sizes")
     norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
-    L.call("chelis_cuda_clip_grads", len(grads), *map(_address, src), _address(dst[0]), _address(dst[2]),
-           float(max_norm), norm.data_ptr())
+    at, kinds, skip = _address(ptrs), _address(dtypes), 0 if own else n
+    _call("chelis_cuda_clip_grads", n, at, _address(counts), kinds, at + skip * ptrs.itemsize,
+          kinds + skip * dtypes.itemsize, float(max_norm), norm.data_ptr())
     return norm

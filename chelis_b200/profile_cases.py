@@ -19,6 +19,9 @@
     python -m chelis_b200.profile_cases experts     # routed feed-forward: 8-bit quantisers of 16384 x
                                                     # 4096 bf16, an 8-bit product 16384 x 1024 x 4096,
                                                     # the way back of 8 rows a token of 1024 bf16
+    python -m chelis_b200.profile_cases sublayer    # 16-bit feed-forward sublayer: the products 16384 x
+                                                    # 4096 x 1024 and back with what follows them, the
+                                                    # gated norms, the balance loss, gradient clipping
 
 Each case builds its inputs on the device, runs the hot path once and
 synchronises; inputs exceed the 126 MB L2 except where the case is smaller
@@ -55,6 +58,25 @@ def run(case: str) -> None:
     elif case == "block8":
         x, dy, w = W.torch_block_inputs(**W.BLOCK_SHAPE)
         ops.block_step(x, w, W.BLOCK_SHAPE["heads"], 1e-5, dy)
+    elif case == "sublayer":
+        from . import dense
+        gen = torch.Generator(device="cuda").manual_seed(5)
+
+        def randn(*shape):
+            return torch.randn(shape, generator=gen, device="cuda")
+        d, ff = 1024, 4096
+        p = dense.Sublayer(randn(d), (randn(d, ff) / 32).bfloat16(), (randn(ff, d) / 64).bfloat16(), randn(d), randn(ff),
+                           randn(d), randn(d), randn(d), randn(d))
+        x, dy = randn(16384, d).bfloat16(), randn(16384, d).bfloat16()
+        _, saved = dense.feed_forward(x, p)
+        grads = dense.feed_forward_bwd(dy, saved, p)
+        ops.clip_grads(grads.values(), 1.0)
+        wide = randn(16384, 4096)
+        ops.residual_norm_bwd(wide, wide, wide, wide, post_gamma=randn(4096), gate=randn(8, 4096), pre_gamma=randn(4096))
+        logits = randn(16384, 64)
+        ids = logits.topk(8, -1).indices.int()
+        _, counts = ops.expert_balance(logits, ids)
+        ops.expert_balance_bwd(logits, counts, 8)
     elif case in ("attention", "attention16"):
         bh = 128 if case == "attention" else 16
         g = torch.Generator(device="cuda").manual_seed(3)

@@ -5,6 +5,8 @@ logits that differ by at most 32); an expert's sum of T of them within
 T u more; the loss is a sum of positive terms: (110 + T) u of it.  The gradient
 p (c - sum p c) has two of them and 40 roundings more, of terms no larger than
 p (c + sum p c): 300 u of that."""
+import math
+
 import numpy as np
 import pytest
 
@@ -114,6 +116,23 @@ def test_gradient_against_differences(cuda):
     live = np.ones(50, dtype=bool)
     numeric = (_ref(l + 1e-6 * d, hids, live, 2)[0] - _ref(l - 1e-6 * d, hids, live, 2)[0]) / 2e-6
     assert abs(numeric - (g * d).sum()) <= 1e-5 * np.abs(g * d).sum() + 1e-8
+
+
+def test_offsets_past_32_bits(cuda):
+    import torch
+    t, e = (1 << 21) + 77, 1024
+    x = torch.zeros(t, e, device="cuda", dtype=torch.bfloat16)
+    x[-3:, 5] = 8.0
+    ids = torch.zeros(t, 1, dtype=torch.int32, device="cuda")
+    ids[-3:] = 5
+    loss, counts = cuda.expert_balance(x, ids)
+    assert int(counts[0]) == t - 3 and int(counts[5]) == 3 and int(counts[e]) == t
+    g = cuda.expert_balance_bwd(x, counts, 1, float(t))
+    p = math.exp(8) / (math.exp(8) + e - 1)
+    q = 1 / (math.exp(8) + e - 1)
+    want = e / t * p * (3 - (p * 3 + q * (t - 3)))
+    assert abs(float(g[t - 1, 5]) - want) <= 2.0 ** -8 * abs(want) + 1e-4 * abs(want)
+    assert abs(float(loss) - 1.0) < 1e-3
 
 
 def test_bad_ids_are_reported(cuda):

@@ -167,6 +167,19 @@ def test_same_bits_captured_and_on_two_streams(cuda):
         assert torch.equal(norm, n) and all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_offsets_past_32_bits(cuda):
+    import torch
+    n = (1 << 31) + 12345
+    big = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    big[-5:] = 3.0
+    small = torch.ones(7, device="cuda")
+    ref = math.sqrt(0.25 * (n - 5) + 45 + 7)
+    norm = cuda.clip_grads([small, big], ref / 2)
+    assert abs(float(norm) - ref) <= 8 * U * ref
+    assert (big[-5:] == 1.5).all() and (big[-100:-5] == 0.25).all() and (big[:100] == 0.25).all() and (small == 0.5).all()
+    assert bool((big[(1 << 31) - 100:(1 << 31) + 100] == 0.25).all())
+
+
 def test_refusals(cuda):
     import torch
     from chelis_b200 import lib as L

@@ -31,10 +31,10 @@ def _operands(rng, m, n, k, ta, tb, dtype):
     return a, b, fa.T if ta else fa, fb.T if tb else fb
 
 
-# m <= 32: few rows; tiles alone and many, ends of every kind; parts (a long k)
+# few rows (m <= 16, or little to read); tiles alone and many, ends of every kind; parts (a long k)
 SHAPES = [(1, 1, 1), (1, 16, 8), (1, 4096, 1024), (3, 17, 33), (8, 1000, 264), (9, 65, 72), (17, 72, 512), (32, 200, 200),
           (33, 8, 16), (64, 128, 64), (128, 256, 128), (200, 136, 72), (257, 300, 100), (300, 257, 65), (129, 31, 70),
-          (700, 1000, 264), (100, 264, 4160), (1500, 2600, 192)]
+          (700, 1000, 264), (100, 264, 4160), (1500, 2600, 192), (50, 129, 40), (64, 1024, 72), (40, 3000, 4104), (20, 4104, 2056)]
 
 
 @pytest.mark.parametrize("tb", [False, True])
@@ -342,6 +342,28 @@ def test_captured_and_on_other_streams(cuda):
     for (_, _, y, _), got in zip(sets, eager):
         assert all(torch.equal(y, g) for g in got)
     cuda.device_status()
+
+
+def test_offsets_past_32_bits(cuda):
+    """Results, residuals and column sums of more than 2^31 numbers: the last rows
+    are those of a small product."""
+    import torch
+    m, n = (1 << 19) + 300, 4104
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    a = torch.randn((m, 16), generator=gen, device="cuda").bfloat16()
+    b = torch.randn((16, n), generator=gen, device="cuda").bfloat16()
+    res = torch.randn((m, n), device="cuda", dtype=torch.bfloat16)
+    y, z = cuda.matmul16(a, b, activation="gelu", residual=res, keep_pre=True)
+    for rows in (slice(0, 300), slice(m - 300, m)):
+        sy, sz = cuda.matmul16(a[rows].contiguous(), b, activation="gelu", residual=res[rows].contiguous(), keep_pre=True)
+        assert torch.equal(y[rows], sy) and torch.equal(z[rows], sz)
+    g = cuda.activation16_bwd(y, z, "silu")
+    assert torch.equal(g[-300:], cuda.activation16_bwd(sy, sz, "silu"))
+    ones = torch.ones_like(res)
+    assert torch.equal(cuda.column_sums16(ones), torch.full((n,), float(m), device="cuda"))
+    w = cuda.matmul16(a, ones, trans_a=True, dtype=torch.float32)  # sums over all rows
+    ref = a.double().sum(0)
+    assert float((w.double() - ref[:, None]).abs().max()) <= (m + 2) * 2.0 ** -23 * float(a.double().abs().sum(0).max())
 
 
 def test_refusals(cuda):

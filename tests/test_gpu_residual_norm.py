@@ -244,6 +244,26 @@ def test_captured_on_two_streams(cuda):
     cuda.device_status()
 
 
+def test_offsets_past_32_bits(cuda):
+    """Rows that begin past 2^31 numbers come out as they do alone."""
+    import torch
+    rows, hidden = (1 << 19) + 40, 4096
+    rng = np.random.default_rng(5)
+    dev, _ = _params(rng, hidden, "layer", True, 1, True)
+    x, b = (torch.randn((rows, hidden), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    y, h = cuda.residual_norm(x, b, **dev)
+    g = cuda.residual_norm_bwd(x, b, y, b, **dev)
+    for at in (slice(0, 40), slice(rows - 40, rows)):
+        part = [t[at].contiguous() for t in (x, b, y)]
+        sy, sh = cuda.residual_norm(part[0], part[1], **dev)
+        # a row's sums may be taken by another number of warps: a step of bf16 apart at most
+        for got, want in ((y[at], sy), (h[at], sh)):
+            assert ((got.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 1e-6).all()
+        sg = cuda.residual_norm_bwd(part[0], part[1], part[2], part[1], **dev)
+        for got, want in ((g.dx[at], sg.dx), (g.dbranch[at], sg.dbranch)):
+            assert torch.equal(got, want)
+
+
 def test_refusals(cuda):
     import torch
     x = torch.zeros(6, 40, device="cuda")
