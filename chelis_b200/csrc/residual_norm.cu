@@ -14,6 +14,14 @@
 // (the rms norm without the means of q and w; without a first norm dgate = sum
 // dt branch, kept as s1).  A row's variance is taken about its warps' own means,
 // put together exactly, so a mean far from 0 costs no digits.
+//
+// 16384 x 1024 bf16, both norms, gate and residual: 34 us (134 MB, 3.9 TB/s; the
+// floor is 20): bound by a row's chain of sums at 16 warps a multiprocessor.  With 8
+// values a thread it took 62 (84 instructions a value, most of them a row's fixed
+// ones), with 32 and IEEE divisions away 44, with the parameters in shared memory 34.
+// Gradients of 16384 x 4096 f32 with 8 gates: 299 us (1.61 GB, 5.4 TB/s; the floor is
+// 246), 643 with rows loaded as they were wanted, 461 through the ring of bulk copies,
+// and the rest by reciprocals, sums of two at once and pointers carried along.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
