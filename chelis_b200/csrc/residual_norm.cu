@@ -226,6 +226,7 @@ struct Team {
     }
     // Row `row` on its way to stage `s`, by one thread.
     __device__ __forceinline__ void fetch(const Rows &rows, int64_t row, int s) {
+        if (dead) return;
         unsigned char *dst = ring + s * stage_bytes;
         uint64_t *bar = &shared.landed[id][s];
         mbar_arrive_expect_tx(bar, stage_bytes);
@@ -364,10 +365,12 @@ struct Team {
         both(mean, *mean_u, *mean_v);
         both(r, *r_u, *r_v);
     }
-    // Copies that a wait gave up on land before the block leaves.
-    __device__ __forceinline__ void drain(int stages) {
-        if (VEC && dead && t == 0)
-            for (int s = 0; s < stages; ++s) wait_for(&shared.landed[id][s]);
+    // Copies that a wait gave up on get another 200 us to land before the block
+    // leaves; none are issued after one was.
+    __device__ __forceinline__ void drain() const {
+        if (!VEC || !dead || t != 0) return;
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000) __nanosleep(1000);
     }
 };
 
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             team.next(in.stages);
         }
     }
-    team.drain(in.stages);
+    team.drain();
 }
 
 // ---- backward -------------------------------------------------------------
@@ -683,7 +686,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     dst[p.hidden + team.col(i) + c] = db2[i * N + c];
                 }
     }
-    team.drain(in.stages);
+    team.drain();
 }
 
 // Sums of `count` rows of [..][2][hidden], both halves, in a fixed order: 32

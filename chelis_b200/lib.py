@@ -51,6 +51,8 @@ FORMAT_E4M3, FORMAT_E5M2 = 0, 1
 BLOCKS_ROWS, BLOCKS_TILES = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 NORM_LAYER, NORM_RMS = 0, 1
+(PACKED_MATMUL16, PACKED_ACTIVATION16_BWD, PACKED_COLUMN_SUMS16, PACKED_RESIDUAL_NORM, PACKED_RESIDUAL_NORM_BWD,
+ PACKED_EXPERT_BALANCE, PACKED_EXPERT_BALANCE_BWD, PACKED_GRAD_NORM, PACKED_CLIP_GRADS) = range(9)
 GEMM_3XTF32, GEMM_EXACT_TREE = 0, 1
 DGEMM_AUTO, DGEMM_DMMA, DGEMM_FFMA = 0, 1, 2
 ROWS_EXACT, ROWS_FAST = 0, 1
@@ -191,6 +193,7 @@ SIGNATURES = {
     "chelis_cuda_expert_balance_bwd": (c_int, [c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_vp, c_vp, c_vp]),
     "chelis_cuda_grad_norm": (c_int, [c_i32, c_vp, c_vp, c_vp, c_vp]),
     "chelis_cuda_clip_grads": (c_int, [c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_f32, c_vp]),
+    "chelis_cuda_call_packed": (c_int, [c_i32, ctypes.c_char_p]),
     "chelis_cuda_dp_shard": (c_int, [c_i64, c_i32, c_i32, ctypes.POINTER(c_i64), ctypes.POINTER(c_i64)]),
     "chelis_cuda_dp_unique_id": (c_int, [c_vp]),
     "chelis_cuda_dp_init": (c_int, [c_i32, c_i32, c_vp]),

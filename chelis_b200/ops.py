@@ -12,6 +12,7 @@ import array
 import contextlib
 import ctypes
 import operator
+import struct
 from typing import NamedTuple
 
 import torch
@@ -830,22 +831,40 @@ _NORM = {"layer": L.NORM_LAYER, "rms": L.NORM_RMS}
 _dtype_of = operator.attrgetter("dtype")
 
 
-_entries: dict[str, object] = {}
+class _Packed:
+    """An entry called with its arguments packed (chelis_cuda_call_packed): with
+    few tokens a call is mostly the binding's.  fmt: q an integer or a pointer, d a
+    float; the stream comes first."""
+
+    def __init__(self, entry: int, fmt: str):
+        self.entry, self.pack, self.f = entry, struct.Struct("=q" + fmt).pack, None
+
+    def __call__(self, *args) -> None:
+        if self.f is None:
+            self.f = L.load().chelis_cuda_call_packed
+        status = self.f(self.entry, self.pack(*args))
+        if status:
+            L.check(status)
 
 
-def _call(name: str, *args) -> None:
-    """L.call with the entry looked up once: these calls are mostly the host's
-    where few tokens are concerned."""
-    f = _entries.get(name)
-    if f is None:
-        f = _entries[name] = getattr(L.load(), name)
-    status = f(*args)
-    if status:
-        L.check(status)
+_matmul16 = _Packed(L.PACKED_MATMUL16, "16q")
+_activation16_bwd = _Packed(L.PACKED_ACTIVATION16_BWD, "6q")
+_column_sums16 = _Packed(L.PACKED_COLUMN_SUMS16, "5q")
+_residual_norm = _Packed(L.PACKED_RESIDUAL_NORM, "10qd2qd2q")
+_residual_norm_bwd = _Packed(L.PACKED_RESIDUAL_NORM_BWD, "12qdqd7q")
+_expert_balance = _Packed(L.PACKED_EXPERT_BALANCE, "9q")
+_expert_balance_bwd = _Packed(L.PACKED_EXPERT_BALANCE_BWD, "7qd3q")
+_grad_norm = _Packed(L.PACKED_GRAD_NORM, "5q")
+_clip_grads = _Packed(L.PACKED_CLIP_GRADS, "6qdq")
 
 
-def _begin(name: str, *tensors: torch.Tensor | None) -> None:
-    """_prepare, and all tensors on one device, the current one."""
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _begin(name: str, *tensors: torch.Tensor | None) -> int:
+    """The stream for a call on these tensors, which are contiguous and lie on one
+    device, the current one."""
     dev = -1
     for t in tensors:
         if t is None:
@@ -859,17 +878,17 @@ def _begin(name: str, *tensors: torch.Tensor | None) -> None:
             dev = at
         elif at != dev:
             raise ValueError(f"{name}: tensors on different devices")
-    _on_device(name, dev)
+    return _on_device(name, dev)
 
 
-def _on_device(name: str, dev: int) -> None:
+def _on_device(name: str, dev: int) -> int:
     current = torch.cuda.current_device()
     if dev >= 0 and dev != current:
         raise ValueError(f"{name}: the tensors' device is not the current one")
     if current not in _initialised:
-        _call("chelis_cuda_init", current)
+        L.call("chelis_cuda_init", current)
         _initialised.add(current)
-    _call("chelis_cuda_set_stream", _raw_stream(current))
+    return _raw_stream(current)
 
 
 def _half(name: str, t: torch.Tensor) -> int:
@@ -919,11 +938,11 @@ def matmul16(a: torch.Tensor, b: torch.Tensor, trans_a: bool = False, trans_b: b
     for t in (residual, z):
         if t is not None and (t.shape != (m, n) or t.dtype != dtype):
             raise ValueError("matmul16: residual and through are [m, n] of the result's type")
-    _begin("matmul16", a, b, bias, residual, z)
+    stream = _begin("matmul16", a, b, bias, residual, z)
     out = torch.empty(m, n, dtype=dtype, device=a.device)
     pre = torch.empty_like(out) if keep_pre else None
-    _call("chelis_cuda_matmul16", dt, int(trans_a), int(trans_b), m, n, k, a.data_ptr(), b.data_ptr(),
-           _ptr(bias), 0 if bias is None else _ACT[bias.dtype], act, _ptr(residual), _ptr(z), _ptr(pre),
+    _matmul16(stream, dt, int(trans_a), int(trans_b), m, n, k, a.data_ptr(), b.data_ptr(),
+           _at(bias), 0 if bias is None else _ACT[bias.dtype], act, _at(residual), _at(z), _at(pre),
            _ACT[dtype], out.data_ptr())
     return (out, pre) if keep_pre else out
 
@@ -934,9 +953,9 @@ def activation16_bwd(dy: torch.Tensor, pre: torch.Tensor, activation: str | None
     act = _activation("activation16_bwd", activation)
     if pre.dtype != dy.dtype or pre.shape != dy.shape:
         raise ValueError("activation16_bwd takes two tensors of one dtype and shape")
-    _begin("activation16_bwd", dy, pre)
+    stream = _begin("activation16_bwd", dy, pre)
     dz = torch.empty_like(dy)
-    _call("chelis_cuda_activation16_bwd", dt, act, dy.data_ptr(), pre.data_ptr(), dy.numel(), dz.data_ptr())
+    _activation16_bwd(stream, dt, act, dy.data_ptr(), pre.data_ptr(), dy.numel(), dz.data_ptr())
     return dz
 
 
@@ -945,9 +964,9 @@ def column_sums16(x: torch.Tensor) -> torch.Tensor:
     dt = _half("column_sums16", x)
     if x.dim() != 2:
         raise ValueError("column_sums16 takes a matrix")
-    _begin("column_sums16", x)
+    stream = _begin("column_sums16", x)
     out = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
-    _call("chelis_cuda_column_sums16", dt, x.data_ptr(), x.shape[0], x.shape[1], out.data_ptr())
+    _column_sums16(stream, dt, x.data_ptr(), x.shape[0], x.shape[1], out.data_ptr())
     return out
 
 
@@ -1023,12 +1042,12 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, *, post_gamma: t
             raise ValueError("residual_norm: without a branch there is the second norm alone")
     elif branch.shape != x.shape or branch.dtype != x.dtype:
         raise ValueError("residual_norm: x and branch are of one dtype and shape")
-    _begin("residual_norm", x, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    stream = _begin("residual_norm", x, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
     y = None if branch is None else torch.empty_like(x)
     h = None if pre_gamma is None else torch.empty_like(x)
-    _call("chelis_cuda_residual_norm", dt, norm, rows, hidden, x.data_ptr(), _ptr(branch), _ptr(post_gamma),
-           _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma), _ptr(pre_beta), float(eps),
-           _ptr(y), _ptr(h))
+    _residual_norm(stream, dt, norm, rows, hidden, x.data_ptr(), _at(branch), _at(post_gamma),
+           _at(post_beta), _at(gate), groups, float(scale), _at(pre_gamma), _at(pre_beta), float(eps),
+           _at(y), _at(h))
     return x if y is None else y, h
 
 
@@ -1051,16 +1070,16 @@ def residual_norm_bwd(dy: torch.Tensor | None, dh: torch.Tensor | None, y: torch
     for t in (dy, dh, branch):
         if t is not None and (t.shape != y.shape or t.dtype != y.dtype):
             raise ValueError("residual_norm_bwd: dy, dh, y and branch are of one dtype and shape")
-    _begin("residual_norm_bwd", dy, dh, y, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
+    stream = _begin("residual_norm_bwd", dy, dh, y, branch, post_gamma, post_beta, gate, pre_gamma, pre_beta)
 
     def like(p):
         return None if p is None else torch.empty_like(p)
 
     g = ResidualNormGrads(torch.empty_like(y), like(branch), like(post_gamma), like(post_beta), like(gate),
                           like(pre_gamma), like(pre_beta))
-    _call("chelis_cuda_residual_norm_bwd", dt, norm, rows, hidden, _ptr(dy), _ptr(dh), y.data_ptr(),
-           _ptr(branch), _ptr(post_gamma), _ptr(post_beta), _ptr(gate), groups, float(scale), _ptr(pre_gamma),
-           float(eps), *(_ptr(t) for t in g))
+    _residual_norm_bwd(stream, dt, norm, rows, hidden, _at(dy), _at(dh), y.data_ptr(),
+           _at(branch), _at(post_gamma), _at(post_beta), _at(gate), groups, float(scale), _at(pre_gamma),
+           float(eps), *(_at(t) for t in g))
     return g
 
 
@@ -1078,10 +1097,10 @@ def expert_balance(logits: torch.Tensor, experts: torch.Tensor, mask: torch.Tens
     tokens, n = logits.shape
     if mask is not None and (mask.dtype != torch.bool or mask.shape != (tokens,)):
         raise ValueError("expert_balance: mask is bool [tokens]")
-    _begin("expert_balance", logits, experts, mask)
+    stream = _begin("expert_balance", logits, experts, mask)
     loss = torch.empty((), dtype=torch.float32, device=logits.device)
     counts = torch.empty(n + 1, dtype=torch.int32, device=logits.device)
-    _call("chelis_cuda_expert_balance", dt, logits.data_ptr(), experts.data_ptr(), _ptr(mask), tokens, n,
+    _expert_balance(stream, dt, logits.data_ptr(), experts.data_ptr(), _at(mask), tokens, n,
            experts.shape[1], loss.data_ptr(), counts.data_ptr())
     return loss, counts
 
@@ -1104,16 +1123,16 @@ def expert_balance_bwd(logits: torch.Tensor, counts: torch.Tensor, k: int, weigh
         raise ValueError("expert_balance_bwd: dloss is one f32 number")
     if add is not None and (add.dtype != logits.dtype or add.shape != logits.shape):
         raise ValueError("expert_balance_bwd: add has the logits' dtype and shape")
-    _begin("expert_balance_bwd", logits, counts, dloss, mask, add)
+    stream = _begin("expert_balance_bwd", logits, counts, dloss, mask, add)
     dlogits = torch.empty_like(logits)
-    _call("chelis_cuda_expert_balance_bwd", dt, logits.data_ptr(), counts.data_ptr(), _ptr(mask), tokens, n, k,
-           float(weight), _ptr(dloss), _ptr(add), dlogits.data_ptr())
+    _expert_balance_bwd(stream, dt, logits.data_ptr(), counts.data_ptr(), _at(mask), tokens, n, k,
+           float(weight), _at(dloss), _at(add), dlogits.data_ptr())
     return dlogits
 
 
 def _tensor_list(name: str, tensors: list):
-    """What the C entries take of a list of tensors: (pointers, sizes, dtypes),
-    host arrays."""
+    """The stream for a call on a list of tensors, and what it takes of them:
+    (pointers, sizes, dtypes), host arrays."""
     devices = set(map(torch.Tensor.get_device, tensors))
     if len(devices) > 1:
         raise ValueError(f"{name}: tensors on different devices")
@@ -1121,12 +1140,12 @@ def _tensor_list(name: str, tensors: list):
         raise ValueError("chelis_b200 ops take CUDA tensors (device memory)")
     if not all(map(torch.Tensor.is_contiguous, tensors)):
         raise ValueError("chelis_b200 ops take contiguous tensors")
-    _on_device(name, devices.pop() if devices else -1)
+    stream = _on_device(name, devices.pop() if devices else -1)
     try:
         dtypes = array.array("i", map(_ACT.__getitem__, map(_dtype_of, tensors)))
     except KeyError:
         raise ValueError(f"{name} takes f32, bf16 or f16 tensors") from None
-    return (array.array("Q", map(torch.Tensor.data_ptr, tensors)),
+    return (stream, array.array("Q", map(torch.Tensor.data_ptr, tensors)),
             array.array("q", map(torch.Tensor.numel, tensors)), dtypes)
 
 
@@ -1138,9 +1157,9 @@ def grad_norm(grads) -> torch.Tensor:
     """The Euclidean norm over all numbers of a list of f32, bf16 or f16
     tensors, an f32 scalar on the device; sums in f64."""
     grads = list(grads)
-    src = _tensor_list("grad_norm", grads)
+    stream, *src = _tensor_list("grad_norm", grads)
     norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
-    _call("chelis_cuda_grad_norm", len(grads), *map(_address, src), norm.data_ptr())
+    _grad_norm(stream, len(grads), *map(_address, src), norm.data_ptr())
     return norm
 
 
@@ -1155,11 +1174,11 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
         grads += out
         if len(grads) != 2 * n:
             raise ValueError("clip_grads: out has the gradients' sizes")
-    ptrs, counts, dtypes = _tensor_list("clip_grads", grads)
+    stream, ptrs, counts, dtypes = _tensor_list("clip_grads", grads)
     if not own and counts[:n] != counts[n:]:
         raise ValueError("clip_grads: out has the gradients' sizes")
     norm = torch.empty((), dtype=torch.float32, device="cuda" if not grads else grads[0].device)
     at, kinds, skip = _address(ptrs), _address(dtypes), 0 if own else n
-    _call("chelis_cuda_clip_grads", n, at, _address(counts), kinds, at + skip * ptrs.itemsize,
-          kinds + skip * dtypes.itemsize, float(max_norm), norm.data_ptr())
+    _clip_grads(stream, n, at, _address(counts), kinds, at + skip * ptrs.itemsize,
+                kinds + skip * dtypes.itemsize, float(max_norm), norm.data_ptr())
     return norm

@@ -765,6 +765,16 @@ int chelis_cuda_grad_norm(int32_t n, const void *const *data, const int64_t *cou
 int chelis_cuda_clip_grads(int32_t n, const void *const *data, const int64_t *counts, const int32_t *dtypes,
                            void *const *out, const int32_t *out_dtypes, float max_norm, float *norm);
 
+/* One of the entries above with its arguments in an array, for bindings that pay by
+ * the argument: the stream (chelis_cuda_set_stream), then the arguments in order,
+ * eight bytes each; integers and pointers as int64, floats as double. */
+enum {
+    CHELIS_PACKED_MATMUL16 = 0, CHELIS_PACKED_ACTIVATION16_BWD = 1, CHELIS_PACKED_COLUMN_SUMS16 = 2,
+    CHELIS_PACKED_RESIDUAL_NORM = 3, CHELIS_PACKED_RESIDUAL_NORM_BWD = 4, CHELIS_PACKED_EXPERT_BALANCE = 5,
+    CHELIS_PACKED_EXPERT_BALANCE_BWD = 6, CHELIS_PACKED_GRAD_NORM = 7, CHELIS_PACKED_CLIP_GRADS = 8
+};
+int chelis_cuda_call_packed(int32_t entry, const int64_t *args);
+
 /* =========================================================================
  * Generated-entry device ABI (emit.rs:838-958, `f_device`): inputs borrowed,
  * outputs newly allocated owners the caller releases.  One entry per program

@@ -282,7 +282,7 @@ def test_unaligned_bases_and_neighbours(cuda):
             out = torch.full((shift + m * n + 64,), 9.0, dtype=torch.bfloat16, device="cuda")
             pre = torch.full_like(out, 9.0)
             y, z = out[shift:shift + m * n], pre[shift:shift + m * n]
-            cuda._begin("test", a)
+            cuda._prepare(a, b)
             L.call("chelis_cuda_matmul16", L.DTYPE_BF16, 0, 0, m, n, k, a.data_ptr(), b.data_ptr(), None, 0, L.ACT_RELU,
                    None, None, z.data_ptr(), L.DTYPE_BF16, y.data_ptr())
             ref = a.double() @ b.double()

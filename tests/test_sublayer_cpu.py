@@ -114,6 +114,54 @@ def test_gradient_lists_refuse():
     assert clip([a], [(None, 64, F32)]) == DOMAIN and clip([a], [(4096, 64, L.DTYPE_F64)]) == UNSUPPORTED
 
 
+def test_packed_entries_take_their_arguments_in_order():
+    """Each entry packed refuses what it refuses called by its arguments, with the
+    same message; the last argument is looked at too."""
+    import struct
+    lib = L.load()
+
+    def same(entry, fmt, direct, *args):
+        status = direct(*args)
+        text = L.last_error()
+        packed = struct.pack("=q" + fmt, 0, *[0 if a is None else a for a in args])
+        assert lib.chelis_cuda_call_packed(entry, packed) == status != OK and L.last_error() == text
+
+    P = 1 << 40  # never read
+    f = lib.chelis_cuda_matmul16
+    good = (BF, 0, 1, 4, 5, 6, P, P, P, BF, 2, P, None, P, BF, P)
+    for i, bad in ((0, F32), (3, -1), (4, 1 << 31), (5, -1), (6, None), (7, None), (9, L.DTYPE_F16), (10, 9), (12, P), (14, L.DTYPE_F16),
+                   (15, None)):
+        same(L.PACKED_MATMUL16, "16q", f, *good[:i], bad, *good[i + 1:])
+    same(L.PACKED_ACTIVATION16_BWD, "6q", lib.chelis_cuda_activation16_bwd, BF, 1, P, P, 4, None)
+    same(L.PACKED_ACTIVATION16_BWD, "6q", lib.chelis_cuda_activation16_bwd, BF, 1, P, P, -4, P)
+    same(L.PACKED_COLUMN_SUMS16, "5q", lib.chelis_cuda_column_sums16, BF, P, 4, 4, None)
+    f = lib.chelis_cuda_residual_norm
+    good = (F32, 1, 4, 8, P, P, P, P, P, 2, 0.5, P, P, 1e-5, P, P)
+    for i, bad in ((0, 9), (1, 2), (2, -1), (3, 9000), (4, None), (5, None), (6, None), (9, 3), (11, None), (14, None), (15, None)):
+        same(L.PACKED_RESIDUAL_NORM, "10qd2qd2q", f, *good[:i], bad, *good[i + 1:])
+    same(L.PACKED_RESIDUAL_NORM, "10qd2qd2q", f, F32, 1, 4, 8, P, None, None, None, None, 1, 0.5, P, P, 1e-5, None, P)
+    f = lib.chelis_cuda_residual_norm_bwd
+    good = (F32, 1, 4, 8, P, P, P, P, P, P, P, 2, 0.5, P, 1e-5, P, P, P, P, P, P, P)
+    for i, bad in ((0, 9), (2, -1), (5, None), (6, None), (7, None), (8, None), (10, None), (11, 3), (13, None), (15, None), (16, None)):
+        same(L.PACKED_RESIDUAL_NORM_BWD, "12qdqd7q", f, *good[:i], bad, *good[i + 1:])
+    f = lib.chelis_cuda_expert_balance
+    good = (F32, P, P, None, 4, 8, 2, P, P)
+    for i, bad in ((0, 9), (1, None), (2, None), (4, -1), (5, 2000), (6, 9), (7, None), (8, None)):
+        same(L.PACKED_EXPERT_BALANCE, "9q", f, *good[:i], bad, *good[i + 1:])
+    f = lib.chelis_cuda_expert_balance_bwd
+    good = (F32, P, P, None, 4, 8, 2, 1.0, None, None, P)
+    for i, bad in ((0, 9), (1, None), (2, None), (4, -1), (6, 0), (10, None)):
+        same(L.PACKED_EXPERT_BALANCE_BWD, "7qd3q", f, *good[:i], bad, *good[i + 1:])
+    n, data, counts, dtypes = _list((1024, 64, F32))
+    at = [ctypes.addressof(v) for v in (data, counts, dtypes)]
+    same(L.PACKED_GRAD_NORM, "5q", lib.chelis_cuda_grad_norm, n, *at, None)
+    same(L.PACKED_GRAD_NORM, "5q", lib.chelis_cuda_grad_norm, -1, *at, P)
+    same(L.PACKED_CLIP_GRADS, "6qdq", lib.chelis_cuda_clip_grads, n, *at, at[0], at[2], -1.0, P)
+    same(L.PACKED_CLIP_GRADS, "6qdq", lib.chelis_cuda_clip_grads, n, *at, at[0], at[2], 1.0, None)
+    assert lib.chelis_cuda_call_packed(99, struct.pack("=q", 0)) == UNSUPPORTED
+    assert lib.chelis_cuda_call_packed(0, None) == DOMAIN
+
+
 class _Fake:
     def __init__(self, device, contiguous=True):
         self.device_index, self.contiguous = device, contiguous
