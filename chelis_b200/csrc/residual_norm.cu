@@ -19,9 +19,12 @@
 // floor is 20): bound by a row's chain of sums at 16 warps a multiprocessor.  With 8
 // values a thread it took 62 (84 instructions a value, most of them a row's fixed
 // ones), with 32 and IEEE divisions away 44, with the parameters in shared memory 34.
-// Gradients of 16384 x 4096 f32 with 8 gates: 299 us (1.61 GB, 5.4 TB/s; the floor is
+// Gradients of 16384 x 4096 f32 with 8 gates: 291 us (1.61 GB, 5.5 TB/s; the floor is
 // 246), 643 with rows loaded as they were wanted, 461 through the ring of bulk copies,
-// and the rest by reciprocals, sums of two at once and pointers carried along.
+// and the rest by reciprocals, sums of two at once, pointers carried along and packed
+// instructions.  16384 x 1024 bf16, one norm 39 us (134 MB, 3.5 TB/s), both 72 (2.8
+// TB/s): instructions and a row's chains of sums at 16 warps a multiprocessor; 64 to 86
+// and 107 with every team's sums written out and folded by few warps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -80,7 +83,7 @@ __device__ __forceinline__ void multiply_add(float (&v)[N], const float (&a)[N],
 }
 // Sum of v, and of the squares about `centre`.
 template <int N>
-__device__ __forceinline__ float values_sum(const float (&v)[N]) {
+__device__ __forceinline__ float values_sum(const float *v) {
     if constexpr (N % 2 == 0) {
         f32x2 s = pack2(v[0], v[1]);
 #pragma unroll
@@ -117,6 +120,78 @@ __device__ __forceinline__ float squares_about(const float *v, float centre) {
     }
 }
 
+// to = a b, sum += a b, sum += a, of N of them; the sum of a b; a =
+// (a + b w + c0) s (rounded so, a row that cancels gives 0).
+template <int N>
+__device__ __forceinline__ void product(float *to, const float *a, const float *b) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const float2 r = unpack2(gemm8::mul2(pack2(a[c], a[c + 1]), pack2(b[c], b[c + 1])));
+            to[c] = r.x, to[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) to[c] = a[c] * b[c];
+    }
+}
+template <int N>
+__device__ __forceinline__ void accumulate(float *sum, const float *a, const float *b) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const float2 r = unpack2(gemm8::fma2(pack2(a[c], a[c + 1]), pack2(b[c], b[c + 1]), pack2(sum[c], sum[c + 1])));
+            sum[c] = r.x, sum[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) sum[c] = fmaf(a[c], b[c], sum[c]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void accumulate(float *sum, const float *a) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const float2 r = unpack2(gemm8::add2(pack2(sum[c], sum[c + 1]), pack2(a[c], a[c + 1])));
+            sum[c] = r.x, sum[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) sum[c] += a[c];
+    }
+}
+template <int N>
+__device__ __forceinline__ float products_sum(const float *a, const float *b) {
+    if constexpr (N % 2 == 0) {
+        f32x2 s = gemm8::mul2(pack2(a[0], a[1]), pack2(b[0], b[1]));
+#pragma unroll
+        for (int c = 2; c < N; c += 2) s = gemm8::fma2(pack2(a[c], a[c + 1]), pack2(b[c], b[c + 1]), s);
+        const float2 r = unpack2(s);
+        return r.x + r.y;
+    } else {
+        float s = a[0] * b[0];
+#pragma unroll
+        for (int c = 1; c < N; ++c) s = fmaf(a[c], b[c], s);
+        return s;
+    }
+}
+template <int N>
+__device__ __forceinline__ void combine(float *a, const float *b, float w, float c0, float s) {
+    if constexpr (N % 2 == 0) {
+        const f32x2 s2 = pack2(s, s), w2 = pack2(w, w), c2 = pack2(c0, c0);
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            const f32x2 t = gemm8::fma2(pack2(b[c], b[c + 1]), w2, c2);
+            const float2 r = unpack2(gemm8::mul2(gemm8::add2(pack2(a[c], a[c + 1]), t), s2));
+            a[c] = r.x, a[c + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) a[c] = (a[c] + fmaf(b[c], w, c0)) * s;
+    }
+}
+
 struct Params {
     int64_t rows;
     int32_t hidden, rms;
@@ -140,6 +215,17 @@ __device__ __forceinline__ void load_params(const float *p, float (&v)[N]) {
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __ldg(p + i);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void store_sums(float *p, const float *v) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = v[i];
     }
 }
 
@@ -286,7 +372,8 @@ struct Team {
     // lie in one half, the others in the other, so that a warp reads whole lines.
     __device__ __forceinline__ void staged(const float *p, int i, float (&v)[N]) const {
         if constexpr (N == 8) {
-            const float4 a = reinterpret_cast<const float4 *>(p)[t + i * SPAN], b = reinterpret_cast<const float4 *>(p)[t + i * SPAN + hidden / 8];
+            const float4 *f = reinterpret_cast<const float4 *>(p) + t + i * SPAN;
+            const float4 a = f[0], b = f[hidden / 8];
             v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         } else if constexpr (N == 4) {
             const float4 a = reinterpret_cast<const float4 *>(p)[t + i * SPAN];
@@ -335,8 +422,8 @@ struct Team {
     }
     // Mean and reciprocal root of what a row is divided by, of two rows at once (or
     // one twice): each warp's sum, its squares about its own mean, then the team's.
-    __device__ __forceinline__ void stats2(const float (&u)[E], const float (&v)[E], bool two, bool rms, float eps, float *mean_u,
-                                           float *r_u, float *mean_v, float *r_v) {
+    __device__ __forceinline__ void stats2(const float (&u)[E], const float (&v)[E], bool two, bool rms, float eps,
+                                           float *mean_u, float *r_u, float *mean_v, float *r_v) {
         float su = 0.0f, sv = 0.0f, sum = 0.0f, cu = 0.0f, cv = 0.0f;
         if (!rms) {
             su = values_sum<E>(u);
@@ -393,14 +480,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ __align__(128) unsigned char rows_smem[];
     __shared__ Shared<W> shared;
     G team(shared, rows_smem, in, p.hidden);
-    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS, me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS;
+    const int64_t me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
     const int64_t first = p.rows * me / teams, last = p.rows * (me + 1) / teams;
     if (VEC && team.t == 0)
         for (int s = 0; s < in.stages && first + s < last; ++s) team.fetch(in, first + s, s);
     const bool rms = p.rms != 0, post = p.post_gamma != nullptr, pre = p.pre_gamma != nullptr, branch = p.branch != nullptr;
     // one gate at most: it goes into c1 and c0
     const bool staged = VEC && p.staged, one_gate = p.per_gate >= p.rows;
-    float *const c1 = reinterpret_cast<float *>(rows_smem + static_cast<size_t>(G::TEAMS) * in.stages * in.arrays * in.row_bytes);
+    float *const c1 =
+        reinterpret_cast<float *>(rows_smem + static_cast<size_t>(G::TEAMS) * in.stages * in.arrays * in.row_bytes);
     float *const c0 = c1 + p.hidden, *const g2 = c0 + p.hidden, *const b2 = g2 + p.hidden;
     if (staged) {
         const float *g = one_gate ? p.gate : nullptr;
@@ -499,8 +588,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // ---- backward -------------------------------------------------------------
 // A team's rows are consecutive, in units that lie within one gate's rows; the
-// sums over them (s1, s0 of a unit, dg2, db2 of the team) stay in registers and
-// go to partial sums that fold_kernel adds up in order.
+// sums over them (s1, s0 of a unit, dg2, db2 of the team) stay in registers.  A
+// block's teams are put together in shared memory (with more than one gate only dg2
+// and db2), and fold_kernel adds up the blocks', or units', sums in order.
 struct Backward {
     int64_t rows;
     int32_t hidden, rms;
@@ -508,46 +598,64 @@ struct Backward {
     int64_t per_gate, groups, chunks;  // units = groups * chunks
     float scale, eps;
     void *dx, *dbranch;
-    float *unit_sums;  // [units][2][hidden]: s1, s0; NULL: not needed
-    float *team_sums;  // [teams][2][hidden]: dg2, db2; NULL: not needed
+    float *unit_sums;  // [units][2][hidden], with one gate [blocks][2][hidden]: s1, s0; NULL: not needed
+    float *pre_sums;   // [blocks][2][hidden]: dg2, db2; NULL: not needed
+    int32_t staged;    // the parameters lie in shared memory beside the ring
 };
 enum { DY = 0, DH = 1, Y = 2, BRANCH = 3 };  // of Rows
+// What a kernel is made for: the second norm, the branch, or whichever is there.
+enum { PRE = 1, POST = 2, ANY = 3 };
 
-template <typename T, bool VEC, int W, int PACKS>
+template <typename T, bool VEC, int W, int PACKS, int PARTS>
 __global__ void __launch_bounds__(THREADS, 1)
     bwd_kernel(const Backward p, const Rows in) {
     using G = Team<T, VEC, W, PACKS>;
     constexpr int N = G::N, E = G::E;
-    constexpr bool HOLD = E <= 8;  // parameters stay in registers
+    constexpr bool HOLD = E <= 8 && PARTS == ANY;  // parameters stay in registers
     extern __shared__ __align__(128) unsigned char rows_smem[];
     __shared__ Shared<W> shared;
     G team(shared, rows_smem, in, p.hidden);
-    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS, me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
+    const int64_t teams = static_cast<int64_t>(gridDim.x) * G::TEAMS;
+    const int64_t me = static_cast<int64_t>(blockIdx.x) * G::TEAMS + team.id;
     const int64_t units = p.groups * p.chunks;
-    auto unit_first = [&](int64_t u) { return u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks) / p.chunks; };
-    auto unit_last = [&](int64_t u) { return u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks + 1) / p.chunks; };
+    // (With fewer and 32-bit divisions here the compiler lays them into every row's
+    // path: 16384 x 4096 f32 with 8 gates then takes 318 us for 291.)
+    auto unit_rows = [&](int64_t u, int64_t *first, int64_t *last) {
+        *first = u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks) / p.chunks;
+        *last = u / p.chunks * p.per_gate + p.per_gate * (u % p.chunks + 1) / p.chunks;
+    };
     // the row after the last one on its way
-    int64_t ahead_unit = me, ahead = me < units ? unit_first(me) : 0, ahead_last = me < units ? unit_last(me) : 0;
+    int64_t ahead_unit = me, ahead = 0, ahead_last = 0;
+    if (me < units) unit_rows(me, &ahead, &ahead_last);
     auto fetch = [&](int s) {
         while (ahead == ahead_last) {
             ahead_unit += teams;
             if (ahead_unit >= units) return;
-            ahead = unit_first(ahead_unit);
-            ahead_last = unit_last(ahead_unit);
+            unit_rows(ahead_unit, &ahead, &ahead_last);
         }
         team.fetch(in, ahead++, s);
     };
     if (VEC && team.t == 0 && me < units)
         for (int s = 0; s < in.stages; ++s) fetch(s);
 
-    const bool rms = p.rms != 0, pre = in.of[DH] != nullptr, has_dy = in.of[DY] != nullptr;
-    const bool has_branch = in.of[BRANCH] != nullptr, post = p.post_gamma != nullptr;
+    const bool rms = p.rms != 0, has_dy = in.of[DY] != nullptr;
+    const bool pre = PARTS == ANY ? in.of[DH] != nullptr : PARTS == PRE;
+    const bool has_branch = PARTS == ANY ? in.of[BRANCH] != nullptr : PARTS == POST;
+    const bool post = PARTS != PRE && p.post_gamma != nullptr;
     const int at_dh = has_dy ? 1 : 0, at_y = at_dh + 1, at_b = at_dh + (pre ? 2 : 0);
     const float inv = team.inv;
     float s1[E], s0[E], dg2[E], db2[E], g2[HOLD ? E : 1], c1[HOLD ? E : 1];
 #pragma unroll
-    for (int e = 0; e < E; ++e) dg2[e] = db2[e] = 0.0f;
+    for (int e = 0; e < E; ++e) s1[e] = s0[e] = dg2[e] = db2[e] = 0.0f;
     if constexpr (HOLD) team.params(p.pre_gamma, 0.0f, g2);
+    const bool staged = !HOLD && VEC && p.staged;
+    float *const held =
+        reinterpret_cast<float *>(rows_smem + static_cast<size_t>(G::TEAMS) * in.stages * in.arrays * in.row_bytes);
+    if (staged) {  // the second norm's gamma, or the first's times the gate
+        if (pre) stage_params<N>(held, p.pre_gamma, nullptr, 1.0f, p.hidden);
+        else stage_params<N>(held, p.post_gamma, p.gate, 1.0f, p.hidden);
+        __syncthreads();
+    }
     for (int64_t unit = me; unit < units; unit += teams) {
 #pragma unroll
         for (int e = 0; e < E; ++e) s1[e] = s0[e] = 0.0f;
@@ -559,8 +667,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int e = 0; e < E; ++e) c1[e] *= g[e];
         }
-        const int64_t last = unit_last(unit);
-        for (int64_t row = unit_first(unit); row < last; ++row) {
+        int64_t row, last;
+        for (unit_rows(unit, &row, &last); row < last; ++row) {
             team.wait();
             float v[E], b[E], dt[E], mean2, r2, mean1 = 0.0f, r1 = 1.0f;
 #pragma unroll
@@ -580,24 +688,23 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (team.in[i]) {
                         float d[N], g[N];
                         team.value(in, DH, at_dh, row, i, d);
-                        if constexpr (!HOLD) load_params<N>(p.pre_gamma + team.col(i), g);
-#pragma unroll
-                        for (int c = 0; c < N; ++c) {
-                            const int e = i * N + c;
-                            if constexpr (HOLD) g[c] = g2[e];
-                            v[e] = fmaf(v[e], r2, shift2);
-                            dg2[e] = fmaf(d[c], v[e], dg2[e]);
-                            db2[e] += d[c];
-                            dt[e] = d[c] * g[c];
-                            sq += dt[e];
-                            sqn = fmaf(dt[e], v[e], sqn);
+                        if constexpr (!HOLD) {
+                            if (staged) team.staged(held, i, g);
+                            else load_params<N>(p.pre_gamma + team.col(i), g);
                         }
+                        float(&n)[N] = *reinterpret_cast<float(*)[N]>(&v[i * N]);
+                        affine<N>(n, r2, shift2);
+                        accumulate<N>(dg2 + i * N, d, n);
+                        accumulate<N>(db2 + i * N, d);
+                        product<N>(dt + i * N, d, HOLD ? g2 + i * N : g);
+                        sq += values_sum<N>(dt + i * N);
+                        sqn += products_sum<N>(dt + i * N, n);
                     }
                 team.sum2(sq, sqn);
                 sq = rms ? 0.0f : sq * inv;
                 sqn *= inv;
 #pragma unroll
-                for (int e = 0; e < E; ++e) dt[e] = (dt[e] - fmaf(v[e], sqn, sq)) * r2;
+                for (int i = 0; i < PACKS; ++i) combine<N>(dt + i * N, v + i * N, -sqn, -sq, r2);
             } else {
                 if (post) team.stats2(b, b, false, rms, p.eps, &mean1, &r1, &mean2, &r2);
 #pragma unroll
@@ -611,12 +718,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (has_dy) {
                         float d[N];
                         team.value(in, DY, 0, row, i, d);
-#pragma unroll
-                        for (int c = 0; c < N; ++c) dt[i * N + c] += d[c];
+                        accumulate<N>(dt + i * N, d);
                     }
-                    team.store(p.dx, row, i, [&](int e) { return p.scale * dt[e]; });
+                    float scaled[N];
+#pragma unroll
+                    for (int c = 0; c < N; ++c) scaled[c] = p.scale;
+                    product<N>(scaled, scaled, dt + i * N);
+                    team.store(p.dx, row, i, [&](int e) { return scaled[e - i * N]; });
                 }
-            if (p.dbranch) {
+            if (PARTS == ANY ? p.dbranch != nullptr : has_branch) {
                 float sw = 0.0f, swn = 0.0f;
 #pragma unroll
                 for (int i = 0; i < PACKS; ++i)
@@ -625,32 +735,29 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int c = 0; c < N; ++c) g[c] = 1.0f;
                         if constexpr (!HOLD) {
-                            if (post) load_params<N>(p.post_gamma + team.col(i), g);
-                            if (gate) {
+                            if (staged && !pre) team.staged(held, i, g);
+                            else if (post) load_params<N>(p.post_gamma + team.col(i), g);
+                            if (gate && !(staged && !pre)) {
                                 float k[N];
                                 load_params<N>(gate + team.col(i), k);
 #pragma unroll
                                 for (int c = 0; c < N; ++c) g[c] *= k[c];
                             }
                         }
-#pragma unroll
-                        for (int c = 0; c < N; ++c) {
-                            const int e = i * N + c;
-                            if constexpr (HOLD) g[c] = c1[e];
-                            b[e] = fmaf(b[e], r1, shift1);  // the branch itself without a norm
-                            s1[e] = fmaf(dt[e], b[e], s1[e]);
-                            s0[e] += dt[e];
-                            dt[e] *= g[c];
-                            sw += dt[e];
-                            swn = fmaf(dt[e], b[e], swn);
-                        }
+                        float(&n)[N] = *reinterpret_cast<float(*)[N]>(&b[i * N]);
+                        affine<N>(n, r1, shift1);  // the branch itself without a norm
+                        accumulate<N>(s1 + i * N, dt + i * N, n);
+                        accumulate<N>(s0 + i * N, dt + i * N);
+                        product<N>(dt + i * N, dt + i * N, HOLD ? c1 + i * N : g);
+                        sw += values_sum<N>(dt + i * N);
+                        swn += products_sum<N>(dt + i * N, n);
                     }
                 if (post) {
                     team.sum2(sw, swn);
                     sw = rms ? 0.0f : sw * inv;
                     swn *= inv;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) dt[e] = (dt[e] - fmaf(b[e], swn, sw)) * r1;
+                    for (int i = 0; i < PACKS; ++i) combine<N>(dt + i * N, b + i * N, -swn, -sw, r1);
                 }
 #pragma unroll
                 for (int i = 0; i < PACKS; ++i)
@@ -663,77 +770,104 @@ __global__ void __launch_bounds__(THREADS, 1)
                 team.next(in.stages);
             }
         }
-        if (p.unit_sums) {
+        if (p.unit_sums && p.groups > 1) {
             float *dst = p.unit_sums + unit * 2 * p.hidden;
 #pragma unroll
             for (int i = 0; i < PACKS; ++i)
-                if (team.in[i])
-#pragma unroll
-                    for (int c = 0; c < N; ++c) {
-                        dst[team.col(i) + c] = s1[i * N + c];
-                        dst[p.hidden + team.col(i) + c] = s0[i * N + c];
-                    }
+                if (team.in[i]) {
+                    store_sums<N>(dst + team.col(i), s1 + i * N);
+                    store_sums<N>(dst + p.hidden + team.col(i), s0 + i * N);
+                }
         }
     }
-    if (p.team_sums) {
-        float *dst = p.team_sums + me * 2 * p.hidden;
+    team.drain();
+    // The teams' sums put together in order, in the ring's memory.
+    const auto join = [&](float *to, const float (&a)[E], const float (&b)[E]) {
+        float *const all = reinterpret_cast<float *>(rows_smem);
+        float *const dst = to + static_cast<int64_t>(blockIdx.x) * 2 * p.hidden;
+        float *const mine = G::TEAMS > 1 ? all + team.id * 2 * p.hidden : dst;
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < PACKS; ++i)
-            if (team.in[i])
+            if (team.in[i]) {
+                store_sums<N>(mine + team.col(i), a + i * N);
+                store_sums<N>(mine + p.hidden + team.col(i), b + i * N);
+            }
+        if (G::TEAMS == 1) return;
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * p.hidden; c += THREADS) {
+            float sum = 0.0f;
 #pragma unroll
-                for (int c = 0; c < N; ++c) {
-                    dst[team.col(i) + c] = dg2[i * N + c];
-                    dst[p.hidden + team.col(i) + c] = db2[i * N + c];
-                }
-    }
-    team.drain();
+            for (int k = 0; k < G::TEAMS; ++k) sum += all[k * 2 * p.hidden + c];
+            dst[c] = sum;
+        }
+    };
+    if (p.unit_sums && p.groups == 1) join(p.unit_sums, s1, s0);
+    if (p.pre_sums) join(p.pre_sums, dg2, db2);
 }
 
 // Sums of `count` rows of [..][2][hidden], both halves, in a fixed order: 32
-// columns a block, 8 threads of each taking every 8th row (with 32 of them the 8
-// groups of 16384 x 4096 rows took 30 us, the blocks' own launch most of it).
-constexpr int FOLD_SLICES = 8;
+// columns a block, its warps taking a row each in turn.  FEW warps where there are
+// blocks enough for the machine (8 groups of 16384 x 4096 rows took 30 us with 32,
+// the blocks' own launch most of it), MANY where there are not (the 592 rows of 1024
+// of one group: 12 us with FEW).
+constexpr int FEW_WARPS = 8, MANY_WARPS = 32;
 __device__ __forceinline__ void fold2(const float *src, int64_t count, int hidden, float (*part)[2][32], float *a, float *b) {
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, slices = blockDim.x >> 5, col = blockIdx.x * 32 + lane;
     float u = 0.0f, v = 0.0f;
     if (col < hidden) {
-#pragma unroll 8
-        for (int64_t i = slice; i < count; i += FOLD_SLICES) {
-            u += __ldg(src + i * 2 * hidden + col);
-            v += __ldg(src + i * 2 * hidden + hidden + col);
+        const float *at = src + static_cast<int64_t>(slice) * 2 * hidden + col;
+        const int64_t step = static_cast<int64_t>(slices) * 2 * hidden;
+        int64_t i = slice;
+        for (; i + 7 * slices < count; i += 8 * slices, at += 8 * step) {  // all loads first
+            float x[8], y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = __ldg(at + k * step), y[k] = __ldg(at + k * step + hidden);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u += x[k], v += y[k];
         }
+        float x[7], y[7];
+#pragma unroll
+        for (int k = 0; k < 7; ++k) {
+            const bool there = i + k * slices < count;
+            x[k] = there ? __ldg(at + k * step) : 0.0f, y[k] = there ? __ldg(at + k * step + hidden) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 7; ++k) u += x[k], v += y[k];
     }
     part[slice][0][lane] = u;
     part[slice][1][lane] = v;
     __syncthreads();
     *a = *b = 0.0f;
     if (slice == 0)
-#pragma unroll
-        for (int s = 0; s < FOLD_SLICES; ++s) *a += part[s][0][lane], *b += part[s][1][lane];
+#pragma unroll 8
+        for (int s = 0; s < slices; ++s) *a += part[s][0][lane], *b += part[s][1][lane];
 }
+inline int fold_warps(int64_t blocks) { return blocks < 2 * sm_count() ? MANY_WARPS : FEW_WARPS; }
 struct Fold {
-    const float *unit_sums, *team_sums;
-    int64_t groups, chunks, teams;
+    const float *unit_sums, *pre_sums;
+    int64_t groups, chunks, blocks;  // partial sums of a group, of the second norm
     int32_t hidden;
     const float *post_gamma, *post_beta, *gate;
     float *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
     float *by_group;  // [groups][2][hidden]: gate times s1, s0 (more than one group)
 };
-__global__ void __launch_bounds__(32 * FOLD_SLICES)
+__global__ void __launch_bounds__(32 * MANY_WARPS)
     fold_kernel(const Fold p) {
-    __shared__ float part[FOLD_SLICES][2][32];
+    __shared__ float part[MANY_WARPS][2][32];
     const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
-    const int64_t groups = p.unit_sums ? p.groups : 0, all = groups + (p.team_sums ? 1 : 0);
+    const int64_t groups = p.unit_sums ? p.groups : 0, all = groups + (p.pre_sums ? 1 : 0);
     const bool writes = threadIdx.x < 32 && col < p.hidden;
     for (int64_t group = blockIdx.y; group < all; group += gridDim.y, __syncthreads()) {
         float a, b;
-        if (group == groups) {  // the second norm's, over all teams
-            fold2(p.team_sums, p.teams, p.hidden, part, &a, &b);
+        const bool second = group == groups;  // the second norm's, over all teams
+        fold2(second ? p.pre_sums : p.unit_sums + group * p.chunks * 2 * p.hidden, second ? p.blocks : p.chunks, p.hidden,
+              part, &a, &b);
+        if (second) {
             if (writes && p.dpre_gamma) p.dpre_gamma[col] = a;
             if (writes && p.dpre_beta) p.dpre_beta[col] = b;
             continue;
         }
-        fold2(p.unit_sums + group * p.chunks * 2 * p.hidden, p.chunks, p.hidden, part, &a, &b);
         if (!writes) continue;
         const int64_t at = group * p.hidden + col;
         if (p.dgate) {
@@ -752,10 +886,10 @@ __global__ void __launch_bounds__(32 * FOLD_SLICES)
         }
     }
 }
-__global__ void __launch_bounds__(32 * FOLD_SLICES)
+__global__ void __launch_bounds__(32 * MANY_WARPS)
     fold_groups_kernel(const float *__restrict__ by_group, int64_t groups, int hidden, float *__restrict__ dgamma,
                        float *__restrict__ dbeta) {
-    __shared__ float part[FOLD_SLICES][2][32];
+    __shared__ float part[MANY_WARPS][2][32];
     const int col = blockIdx.x * 32 + (threadIdx.x & 31);
     float a, b;
     fold2(by_group, groups, hidden, part, &a, &b);
@@ -899,47 +1033,69 @@ extern "C" int chelis_cuda_residual_norm_bwd(int32_t dtype, int32_t kind, int64_
     p.eps = eps;
     p.dx = dx;
     p.dbranch = dbranch;
-    const bool unit_sums = dpost_gamma || dpost_beta || dgate, team_sums = dpre_gamma || dpre_beta;
+    const bool unit_sums = dpost_gamma || dpost_beta || dgate, pre_sums = dpre_gamma || dpre_beta;
     const bool by_group = groups > 1 && (dpost_gamma || dpost_beta);
     void *scratch = nullptr;
     auto body = [&]() -> int {
         int rc = CHELIS_CUDA_OK;
         float *sums = nullptr;
-        size_t unit_n = 0, team_n = 0;
-        int64_t teams = 0;
-        int32_t staged = 0;
-        rnorm::launch<8>(dtype, vec, hidden, in, rows, 0, &staged, [&](auto t, auto v, auto w, auto packs, unsigned grid, size_t smem) {
-            constexpr int W = decltype(w)::value;
-            teams = static_cast<int64_t>(grid) * (rnorm::THREADS / (32 * W));
+        size_t unit_n = 0, pre_n = 0;
+        int64_t blocks = 0;
+        const auto run = [&](auto parts, auto t, auto v, auto w, auto packs, unsigned grid, size_t smem) {
+            constexpr int W = decltype(w)::value, TEAMS = rnorm::THREADS / (32 * W);
+            const int64_t teams = static_cast<int64_t>(grid) * TEAMS;
+            blocks = grid;
             p.chunks = teams / groups < 1 ? 1 : teams / groups;
             if (p.chunks > p.per_gate) p.chunks = p.per_gate;
-            unit_n = unit_sums ? static_cast<size_t>(groups) * p.chunks * 2 * hidden : 0;
-            team_n = team_sums ? static_cast<size_t>(teams) * 2 * hidden : 0;
+            unit_n = unit_sums ? static_cast<size_t>(groups > 1 ? groups * p.chunks : blocks) * 2 * hidden : 0;
+            pre_n = pre_sums ? static_cast<size_t>(blocks) * 2 * hidden : 0;
+            // the teams' sums, put together there
+            if (TEAMS > 1) smem = std::max(smem, static_cast<size_t>(TEAMS) * 2 * hidden * sizeof(float));
             const size_t group_n = by_group ? static_cast<size_t>(groups) * 2 * hidden : 0;
-            rc = scratch_alloc(&scratch, (unit_n + team_n + group_n) * sizeof(float), s);
+            rc = scratch_alloc(&scratch, (unit_n + pre_n + group_n) * sizeof(float), s);
             if (rc != CHELIS_CUDA_OK) return;
             sums = static_cast<float *>(scratch);
             p.unit_sums = unit_sums ? sums : nullptr;
-            p.team_sums = team_sums ? sums + unit_n : nullptr;
-            auto kernel = rnorm::bwd_kernel<decltype(t), decltype(v)::value, W, decltype(packs)::value>;
+            p.pre_sums = pre_sums ? sums + unit_n : nullptr;
+            auto kernel = rnorm::bwd_kernel<decltype(t), decltype(v)::value, W, decltype(packs)::value, decltype(parts)::value>;
             rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                             "cudaFuncSetAttribute");
             if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, s>>>(p, in);
-        });
+        };
+        using Any = std::integral_constant<int, rnorm::ANY>;
+        using Pre = std::integral_constant<int, rnorm::PRE>;
+        using Post = std::integral_constant<int, rnorm::POST>;
+        // Where there are more rows than teams of 8 values a thread, one norm's gradients
+        // in 16, which its sums leave registers for: 4800 x 1024 bf16 18.7 us for 22.5 with
+        // 8, 300 x 1024 9.7 for 8.6.  Both norms' in 8.
+        const bool many = vec && hidden > 256 && rows * hidden > sm_count() * 4096ll;
+        if (many && dh && !needs_branch && !dbranch)
+            rnorm::launch<16>(dtype, vec, hidden, in, rows, 4 * hidden, &p.staged, [&](auto t, auto v, auto... rest) {
+                if constexpr (decltype(v)::value) run(Pre{}, t, v, rest...);
+            });
+        else if (many && !dh && needs_branch)
+            rnorm::launch<16>(dtype, vec, hidden, in, rows, groups == 1 ? 4 * hidden : 0, &p.staged,
+                              [&](auto t, auto v, auto... rest) {
+                                  if constexpr (decltype(v)::value) run(Post{}, t, v, rest...);
+                              });
+        else
+            rnorm::launch<8>(dtype, vec, hidden, in, rows, 0, &p.staged, [&](auto... shape) { run(Any{}, shape...); });
         CHELIS_TRY(rc);
         g_launches++;
         CHELIS_LAUNCH_CHECK("rnorm::bwd_kernel");
-        if (!unit_sums && !team_sums) return CHELIS_CUDA_OK;
-        rnorm::Fold f{p.unit_sums, p.team_sums, groups, p.chunks, teams, p.hidden, post_gamma, post_beta, gate, dgate,
-                      dpost_gamma, dpost_beta, dpre_gamma, dpre_beta, by_group ? sums + unit_n + team_n : nullptr};
-        int64_t high = (unit_sums ? groups : 0) + (team_sums ? 1 : 0);
+        if (!unit_sums && !pre_sums) return CHELIS_CUDA_OK;
+        rnorm::Fold f{p.unit_sums, p.pre_sums, groups, groups > 1 ? p.chunks : blocks, blocks, p.hidden, post_gamma, post_beta,
+                      gate, dgate, dpost_gamma, dpost_beta, dpre_gamma, dpre_beta,
+                      by_group ? sums + unit_n + pre_n : nullptr};
+        int64_t high = (unit_sums ? groups : 0) + (pre_sums ? 1 : 0);
         if (high > 65535) high = 65535;
         const unsigned wide = static_cast<unsigned>((hidden + 31) / 32);
-        rnorm::fold_kernel<<<dim3(wide, static_cast<unsigned>(high)), 32 * rnorm::FOLD_SLICES, 0, s>>>(f);
+        rnorm::fold_kernel<<<dim3(wide, static_cast<unsigned>(high)), 32 * rnorm::fold_warps(wide * high), 0, s>>>(f);
         g_launches++;
         CHELIS_LAUNCH_CHECK("rnorm::fold_kernel");
         if (by_group) {
-            rnorm::fold_groups_kernel<<<wide, 32 * rnorm::FOLD_SLICES, 0, s>>>(f.by_group, groups, p.hidden, dpost_gamma, dpost_beta);
+            rnorm::fold_groups_kernel<<<wide, 32 * rnorm::fold_warps(wide), 0, s>>>(f.by_group, groups, p.hidden, dpost_gamma,
+                                                                                    dpost_beta);
             g_launches++;
             CHELIS_LAUNCH_CHECK("rnorm::fold_groups_kernel");
         }

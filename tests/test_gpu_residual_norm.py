@@ -110,6 +110,42 @@ def test_second_norm_alone(cuda, rows, hidden):
             S.check(getattr(got, name), *want[name], dtype if name == "dx" else "f32")
 
 
+# rows, hidden, gate: one norm's gradients with more rows than there are teams of few values a thread; every width of
+# a team, rows that end inside packs and teams, gates whose rows end inside a team's
+MANY = [(2500, 264, 1), (1300, 512, 0), (1299, 504, 3), (700, 1000, 7), (640, 1024, 1), (330, 2048, 1), (322, 2056, 161),
+        (170, 4096, 1), (163, 4104, 0), (100, 8192, 1), (102, 8184, 2)]
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,hidden,gate", MANY)
+def test_one_norm_of_many_rows(cuda, rows, hidden, gate, kind):
+    rng = np.random.default_rng(rows * 3 + hidden)
+    for dtype in ("f32", "bf16", "f16"):
+        y, fy = _rows(rng, (rows, hidden), dtype)
+        b, fb = _rows(rng, (rows, hidden), dtype, 0.5)
+        dy, fdy = _rows(rng, (rows, hidden), dtype)
+        dh, fdh = _rows(rng, (rows, hidden), dtype)
+
+        def compare(got, want):
+            for name, g in got._asdict().items():
+                assert (g is None) == (name not in want), name
+                if g is not None:
+                    S.check(g, *want[name], dtype if name in ("dx", "dbranch") else "f32")
+
+        betas = kind == "layer"
+        dev, ref = _params(rng, hidden, kind, False, 0, True, betas=betas)  # the second alone
+        dev["scale"] = ref["scale"] = 1.0
+        for d, fd in ((dy, fdy), (None, None)):
+            want = S.join_bwd(fd, fdh, fy, None, ref)
+            want.pop("dbranch", None)  # no branch
+            compare(cuda.residual_norm_bwd(d, dh, y, None, **dev), want)
+        dev, ref = _params(rng, hidden, kind, True, gate, False, betas=betas)  # the first alone
+        compare(cuda.residual_norm_bwd(dy, None, y, b, **dev), S.join_bwd(fdy, None, fy, fb, dict(ref, has_branch=True)))
+        if gate:  # a gate alone
+            dev, ref = _params(rng, hidden, kind, False, gate, False)
+            compare(cuda.residual_norm_bwd(dy, None, y, b, **dev), S.join_bwd(fdy, None, fy, fb, dict(ref, has_branch=True)))
+
+
 @pytest.mark.parametrize("hidden", [40, 1024, 5000])
 def test_mean_far_from_zero(cuda, hidden):
     """A mean of 1000 standard deviations costs the digits that the input's own
