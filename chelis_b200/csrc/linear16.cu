@@ -317,71 +317,122 @@ __device__ __forceinline__ void act_piece(const GeluConstants<HOLD> &k, f32x2 (&
         for (int c = 0; c < PIECE / 2; ++c) v[c] = add2(v[c], x[c]);
 }
 
-// One warp's 32 rows and a quarter of the columns of a tile, from tensor memory to the
-// results, a piece at a time, the next one's sums loading meanwhile.  `used` counts
-// the boxes that TMA has stored.
+// ---- long contractions ------------------------------------------------------
+// The tensor core's sum loses what lies below its last place at every 16 of k, so it
+// drifts towards 0: by 1e-6 of it at k = 1024, 4.4e-6 at 4096, 1.9e-5 at 16384, 7.6e-5 at
+// 65536 (normal numbers; 8e-5 at 16384 where all products have one sign).  In an f32
+// result, such as a weight gradient over many tokens, that is far more than f32's own
+// roundings.  So the kernel of f32 results without an activation, which also makes the
+// parts, cuts a tile's contraction into chunks of 1024 at most, which take the two
+// accumulators in turn, and its finishing warps add them up in registers, rounding as
+// f32 does: 1e-6 at any k.  1024 x 4096 x 16384 takes 108 us for 105, 4096 x 4096 x 65536
+// 1640 for 1630 (chunks of 4096, 4.4e-6: 106 and 1600).  Half a step of a 16-bit result
+// is 20 times and more what it would gain, at 130 us for 109 (16384 x 1024 x 4096, chunks
+// of 2048); with an activation there are no 64 registers to spare.
+constexpr int CHUNK = 16;  // blocks of the contraction
+constexpr bool adds_chunks(bool f32, int32_t act) { return f32 && act == CHELIS_ACT_NONE; }
+constexpr int MOST_PIECES = TN / (4 * PIECE);
+struct Chunks {
+    int count, blocks;  // of a tile, of a chunk (the last one may have fewer)
+};
+template <bool LONG>
+__device__ __forceinline__ Chunks chunks_of(int kbs) {
+    if constexpr (!LONG) return {1, kbs};
+    const int count = (kbs + CHUNK - 1) / CHUNK;
+    return {count, (kbs + count - 1) / count};
+}
+__device__ __forceinline__ int pieces_of(const Params &p, int col0) {
+    return min((static_cast<int>(p.n) - col0 + PIECE - 1) / PIECE, p.tn / (4 * PIECE));
+}
+// A warp's sums of one chunk on top of those before.
+__device__ __forceinline__ void add_chunk(uint32_t acc, int pieces, f32x2 (&sum)[MOST_PIECES][PIECE / 2]) {
+#pragma unroll
+    for (int i = 0; i < MOST_PIECES; ++i)
+        if (i < pieces) {
+            uint32_t r[PIECE];
+            tmem_ld_32x32b_x16(acc + i * PIECE, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < PIECE / 2; ++c)
+                sum[i][c] = add2(sum[i][c], gemm8::pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])));
+        }
+}
+
+// One warp's piece i of its 32 rows and a quarter of the columns of a tile, from the
+// sums, which sums(v) gives, to the results.  `used` counts the boxes that TMA has
+// stored.
+template <bool F32, bool BF, int32_t ACT, bool HOLD, typename Sums>
+__device__ __forceinline__ void finish_piece(const Params &p, const CUtensorMap *map_out, unsigned char *boxes, unsigned char *&box,
+                                             int &used, int lane, int row, int rows, int col0, int part, bool aux_here,
+                                             const GeluConstants<HOLD> &constants, int i, int pieces, Sums sums) {
+    constexpr int PER_BOX = F32 ? 1 : 2, WORDS = F32 ? 16 : 8;
+    const int n = static_cast<int>(p.n), col = col0 + i * PIECE, odd = F32 ? 0 : i & 1;
+    f32x2 v[PIECE / 2], x[PIECE / 2];
+    if (p.vec && odd == 0) {
+        if (aux_here) {
+            box = boxes + i / 2 * BOX;
+        } else {
+            box = boxes + (used & 1) * BOX;
+            if (lane == 0) wait_reads_but_last();
+            __syncwarp();
+        }
+        ++used;
+    }
+    if (aux_here) {
+        if constexpr (!F32) {
+            uint32_t w[8];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint4 u = *box_at(box, lane, odd * 2 + c);
+                w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
+            }
+            to_values<F32, BF>(w, x);
+        }
+    } else if (p.f.aux_kind != AUX_NONE) {
+        get_piece<F32, BF>(p, boxes, lane, row, rows, col, x);
+    }
+    sums(v);
+    if (p.f.bias) add_bias<BF>(p.f, col, n, v);
+    if (p.f.pre) put_piece<F32, BF>(p, p.f.pre, boxes, lane, v, row, rows, col, 0);
+    act_piece(constants, v, x, p.f.aux_kind, ACT == ANY_ACT ? p.f.act : ACT);
+    if (!p.vec) {
+        put_piece<F32, BF>(p, p.f.out, boxes, lane, v, row, rows, col, part);
+        return;
+    }
+    uint32_t w[WORDS];
+    to_words<F32, BF>(v, w);
+#pragma unroll
+    for (int c = 0; c < WORDS; c += 4)
+        *box_at(box, lane, odd * 2 + c / 4) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
+    if (odd == PER_BOX - 1 || i + 1 == pieces) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            scaled8::tma_store_3d(map_out, smem_u32(box), col - odd * PIECE, row, part);
+            scaled8::store_commit();
+        }
+    }
+}
+// All of its pieces from tensor memory, the next one's sums loading meanwhile.
 template <bool F32, bool BF, int32_t ACT, bool HOLD, typename Release>
 __device__ __forceinline__ void finish_tile(const Params &p, const CUtensorMap *map_out, unsigned char *boxes, int &used, int lane,
                                             uint32_t acc, int row, int rows, int col0, int part, bool aux_here,
                                             const GeluConstants<HOLD> &constants, Release release) {
-    constexpr int PER_BOX = F32 ? 1 : 2, WORDS = F32 ? 16 : 8;
-    const int n = static_cast<int>(p.n), pieces = min((n - col0 + PIECE - 1) / PIECE, p.tn / (4 * PIECE));
+    const int pieces = pieces_of(p, col0);
     uint32_t r[PIECE];
     unsigned char *box = boxes;
     tmem_ld_32x32b_x16(acc, r);
 #pragma unroll 2
-    for (int i = 0; i < pieces; ++i) {
-        const int col = col0 + i * PIECE, odd = F32 ? 0 : i & 1;
-        f32x2 v[PIECE / 2], x[PIECE / 2];
-        if (p.vec && odd == 0) {
-            if (aux_here) {
-                box = boxes + i / 2 * BOX;
-            } else {
-                box = boxes + (used & 1) * BOX;
-                if (lane == 0) wait_reads_but_last();
-                __syncwarp();
-            }
-            ++used;
-        }
-        if (aux_here) {
-            if constexpr (!F32) {
-                uint32_t w[8];
+    for (int i = 0; i < pieces; ++i)
+        finish_piece<F32, BF, ACT>(p, map_out, boxes, box, used, lane, row, rows, col0, part, aux_here, constants, i, pieces,
+                                   [&](f32x2 (&v)[PIECE / 2]) {
+            tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint4 u = *box_at(box, lane, odd * 2 + c);
-                    w[4 * c] = u.x, w[4 * c + 1] = u.y, w[4 * c + 2] = u.z, w[4 * c + 3] = u.w;
-                }
-                to_values<F32, BF>(w, x);
-            }
-        } else if (p.f.aux_kind != AUX_NONE) {
-            get_piece<F32, BF>(p, boxes, lane, row, rows, col, x);
-        }
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < PIECE / 2; ++c) v[c] = gemm8::pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-        if (i + 1 < pieces) tmem_ld_32x32b_x16(acc + (i + 1) * PIECE, r);
-        else release();  // all of the sums have been read: the next tile but one may have them
-        if (p.f.bias) add_bias<BF>(p.f, col, n, v);
-        if (p.f.pre) put_piece<F32, BF>(p, p.f.pre, boxes, lane, v, row, rows, col, 0);
-        act_piece(constants, v, x, p.f.aux_kind, ACT == ANY_ACT ? p.f.act : ACT);
-        if (!p.vec) {
-            put_piece<F32, BF>(p, p.f.out, boxes, lane, v, row, rows, col, part);
-            continue;
-        }
-        uint32_t w[WORDS];
-        to_words<F32, BF>(v, w);
-#pragma unroll
-        for (int c = 0; c < WORDS; c += 4)
-            *box_at(box, lane, odd * 2 + c / 4) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
-        if (odd == PER_BOX - 1 || i + 1 == pieces) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                scaled8::tma_store_3d(map_out, smem_u32(box), col - odd * PIECE, row, part);
-                scaled8::store_commit();
-            }
-        }
-    }
+            for (int c = 0; c < PIECE / 2; ++c)
+                v[c] = gemm8::pack2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+            if (i + 1 < pieces) tmem_ld_32x32b_x16(acc + (i + 1) * PIECE, r);
+            else release();  // all of the sums have been read: the next tile but one may have them
+        });
 }
 
 // BF: bf16 operands, else f16.  F32: f32 results, else the operands' type; ACT is
@@ -436,6 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int mt = static_cast<int>((p.m + TM - 1) / TM), nt = static_cast<int>((p.n + p.tn - 1) / p.tn);
     const int tiles = uniform(mt * nt * p.parts);
+    constexpr bool LONG = adds_chunks(F32, ACT);
     int32_t issued = 0;
 
     if (warp < 4) {
@@ -485,20 +537,21 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t tb = uniform(static_cast<int>(tmem_base));
             const uint64_t desc_a = operand_desc(p.amn), desc_b = operand_desc(p.bmn);
             const uint32_t step_a = p.amn ? 16 * 128 : 32, step_b = p.bmn ? 16 * 128 : 32;
-            int32_t it = 0, tile = 0;
+            int32_t it = 0, use = 0;  // stages, accumulators taken
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true, ready = false;
-            for (int L = worker; ok && L < tiles; L += workers, ++tile) {
-                const int kbs = p.parts > 1 ? uniform(tile_at(p, mt, nt, L).kbs) : p.kblocks;
-                const int cur = tile & 1;
+            // `blocks` stages into the next accumulator
+            const auto chunk = [&](int blocks) {
+                const int cur = use & 1;
                 const uint32_t d = tb + (cur ? static_cast<uint32_t>(TN) : 0u);
-                // this accumulator's last tile but one has been read
-                if (tile >= 2) ok = all(wait<true>(&acc_empty[cur], ((tile >> 1) - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_MMA));
-                if (!ok) break;
-                for (int i = 0; i < kbs; ++i, ++it) {
+                // what it held before has been read
+                if (use >= 2) ok = all(wait<true>(&acc_empty[cur], ((use >> 1) - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_MMA));
+                if (!ok) return;
+                ++use;
+                for (int i = 0; i < blocks; ++i, ++it) {
                     if (!ready) ok = all(wait(&full[stage], phase, tries, abort_flag, DEVERR_TIMEOUT_MMA));
-                    if (!ok) break;
+                    if (!ok) return;
                     tc_fence_after();
                     // ask for the next stage now, read the answer after this one's instructions
                     const int next = stage + 1 == STAGES ? 0 : stage + 1;
@@ -511,12 +564,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                             mma_f16_pair(d, at_address(desc_a, a + kk * step_a), at_address(desc_b, b + kk * step_b), p.idesc,
                                          !(i == 0 && kk == 0));
                         mma_commit_pair(&empty[stage], 0x3);
-                        if (i == kbs - 1) mma_commit_pair(&acc_full[cur], 0x3);
+                        if (i == blocks - 1) mma_commit_pair(&acc_full[cur], 0x3);
                     }
                     __syncwarp();
                     ready = all(peek);
                     stage = next;
                     phase = next_phase;
+                }
+            };
+            for (int L = worker; ok && L < tiles; L += workers) {
+                const int kbs = p.parts > 1 ? uniform(tile_at(p, mt, nt, L).kbs) : p.kblocks;
+                if constexpr (LONG) {
+                    const int most = uniform(chunks_of<LONG>(kbs).blocks);
+                    for (int left = kbs; ok && left > 0; left -= most) chunk(min(left, most));
+                } else {
+                    chunk(kbs);
                 }
             }
             if (lane == 0) *consumed = it;
@@ -530,9 +592,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint64_t *aux_bar = &aux_full[warp - 4];
         const bool aux_tma = !F32 && p.aux_tma;
         const GeluConstants<!F32 && ACT == CHELIS_ACT_GELU> constants;
-        int32_t tile = 0, aux_count = 0, used = 0;
+        int32_t use = 0, aux_count = 0, used = 0;  // use: accumulators read
         bool ok = true;
-        for (int L = worker; ok && L < tiles; L += workers, ++tile) {
+        auto sums_at = [&] { return tmem_base + lanes + (use & 1 ? static_cast<uint32_t>(TN) : 0u) + side * span; };
+        auto landed_sums = [&] {
+            return all(wait(&acc_full[use & 1], (use >> 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE));
+        };
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_relaxed(mapa_shared(smem_u32(&acc_empty[use & 1]), 0));
+        };
+        for (int L = worker; ok && L < tiles; L += workers, ++use) {
             const Tile t = tile_at(p, mt, nt, L);
             const int row0 = t.m0 + static_cast<int>(rank) * BM + quad * 32, col0 = t.n0 + side * span;
             const bool live = row0 < p.m && col0 < p.n;  // else nothing to read or store
@@ -548,8 +619,34 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 ++aux_count;
             }
-            const int b = tile & 1;
-            ok = all(wait(&acc_full[b], (tile >> 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE));
+            if constexpr (LONG) {
+                const int chunks = chunks_of<LONG>(t.kbs).count;
+                if (chunks > 1) {
+                    f32x2 sum[MOST_PIECES][PIECE / 2] = {};
+                    const int pieces = pieces_of(p, col0);
+                    for (int c = 0; c < chunks; ++c) {
+                        if (c) ++use;
+                        ok = landed_sums();
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (live) add_chunk(sums_at(), pieces, sum);
+                        release();
+                    }
+                    if (!ok) break;
+                    unsigned char *box = boxes;
+                    if (live)
+#pragma unroll
+                        for (int i = 0; i < MOST_PIECES; ++i)
+                            if (i < pieces)
+                                finish_piece<F32, BF, ACT>(p, &map_out, boxes, box, used, lane, row0, rows, col0, t.part, false,
+                                                           constants, i, pieces, [&](f32x2 (&v)[PIECE / 2]) {
+#pragma unroll
+                                    for (int c = 0; c < PIECE / 2; ++c) v[c] = sum[i][c];
+                                });
+                    continue;
+                }
+            }
+            ok = landed_sums();
             if (aux_tma && live) {
                 // taken on an abort too: the copies land before the block leaves
                 if (ok) ok = all(wait(aux_bar, (aux_count - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE));
@@ -557,14 +654,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             if (!ok) break;
             tc_fence_after();
-            const uint32_t acc = tmem_base + lanes + (b ? static_cast<uint32_t>(TN) : 0u) + side * span;
-            auto release = [&] {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive_relaxed(mapa_shared(smem_u32(&acc_empty[b]), 0));
-            };
             if (live)
-                finish_tile<F32, BF, ACT>(p, &map_out, boxes, used, lane, acc, row0, rows, col0, t.part, aux_tma, constants,
+                finish_tile<F32, BF, ACT>(p, &map_out, boxes, used, lane, sums_at(), row0, rows, col0, t.part, aux_tma, constants,
                                           release);
             else release();
         }

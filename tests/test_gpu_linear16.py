@@ -383,3 +383,41 @@ def test_refusals(cuda):
                 lambda: cuda.column_sums16(a.float())):
         with pytest.raises(ValueError):
             bad()
+
+
+# f32 results by chunks of the contraction (k > 1024): tiles of 256 and 128 columns, and parts of more than a chunk
+@pytest.mark.parametrize("m,n,k,ta,tb", [(300, 5000, 2200, False, False), (300, 2600, 2049, False, True), (513, 5001, 1100, True, False),
+                                         (300, 5000, 1024, False, False), (300, 5000, 1025, True, True), (130, 1000, 20000, True, False),
+                                         (1024, 4096, 16384, True, False)])
+def test_long_contractions_are_added_up(cuda, m, n, k, ta, tb):
+    """Whole numbers, whose sums f32 holds, with everything that may follow the sums."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+
+    def whole(shape, dtype):
+        return torch.randint(-4, 5, shape, generator=gen, device="cuda").to(dtype)
+
+    for dtype in DT:
+        a, b = whole((k, m) if ta else (m, k), _t(dtype)), whole((n, k) if tb else (k, n), _t(dtype))
+        bias, res = whole((n,), torch.float32), whole((m, n), torch.float32)
+        z = (a.double().t() if ta else a.double()) @ (b.double().t() if tb else b.double())
+        assert torch.equal(cuda.matmul16(a, b, ta, tb, dtype=torch.float32).double(), z)
+        y, pre = cuda.matmul16(a, b, ta, tb, bias=bias, residual=res, keep_pre=True, dtype=torch.float32)
+        z += bias.double()
+        assert torch.equal(pre.double(), z) and torch.equal(y.double(), z + res.double())
+
+
+@pytest.mark.parametrize("m,n,k", [(512, 5000, 16384), (512, 5000, 65536), (512, 256, 65536)])
+def test_long_sums_do_not_drift(cuda, m, n, k):
+    """Sums of k positive products in f32 against float64.  An MMA adds 16 products to
+    the sum and loses at most 2 units of its last place, 2^-22 of it; a chunk of 1024
+    is 64 of them on a sum that grows evenly, 64 / 2 * 2^-22 = 2^-17 of the chunk, twice
+    that for the unevenness; adding up k / 1024 chunks rounds by 2^-24 each."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    for dtype in DT:
+        a = torch.randn((k, m), generator=gen, device="cuda").abs().to(_t(dtype))
+        b = torch.randn((k, n), generator=gen, device="cuda").abs().to(_t(dtype))
+        got = cuda.matmul16(a, b, trans_a=True, dtype=torch.float32)
+        ref = a.double().t() @ b.double()
+        assert float(((got.double() - ref).abs() / ref).max()) <= 2.0 ** -16 + k / 1024 * 2.0 ** -24
