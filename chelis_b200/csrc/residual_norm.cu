@@ -12,8 +12,8 @@
 //   dgate = g1 s1 + b1 s0,  dg1 = sum gate s1,  db1 = sum gate s0
 //
 // (the rms norm without the means of q and w; without a first norm dgate = sum
-// dt branch, kept as s1).  A row's variance is taken about its warps' own means,
-// put together exactly, so a mean far from 0 costs no digits.
+// dt branch, kept as s1).  A row's values are taken about its warps' own means, which
+// are put together exactly, so a mean far from 0 costs no digits but those of its sum.
 //
 // 16384 x 1024 bf16, both norms, gate and residual: 34 us (134 MB, 3.9 TB/s; the
 // floor is 20): bound by a row's chain of sums at 16 warps a multiprocessor.  With 8
@@ -81,7 +81,7 @@ __device__ __forceinline__ void multiply_add(float (&v)[N], const float (&a)[N],
         for (int c = 0; c < N; ++c) v[c] = fmaf(v[c], a[c], s[c]);
     }
 }
-// Sum of v, and of the squares about `centre`.
+// Sum of v; v less `centre`, in place, and the sum of its squares.
 template <int N>
 __device__ __forceinline__ float values_sum(const float *v) {
     if constexpr (N % 2 == 0) {
@@ -98,13 +98,15 @@ __device__ __forceinline__ float values_sum(const float *v) {
     }
 }
 template <int N>
-__device__ __forceinline__ float squares_about(const float *v, float centre) {
+__device__ __forceinline__ float centre_squares(float *v, float centre) {
     if constexpr (N % 2 == 0) {
         const f32x2 m = pack2(-centre, -centre);
         f32x2 q = 0ull;
 #pragma unroll
         for (int c = 0; c < N; c += 2) {
             const f32x2 d = gemm8::add2(pack2(v[c], v[c + 1]), m);
+            const float2 r = unpack2(d);
+            v[c] = r.x, v[c + 1] = r.y;
             q = gemm8::fma2(d, d, q);
         }
         const float2 r = unpack2(q);
@@ -113,11 +115,16 @@ __device__ __forceinline__ float squares_about(const float *v, float centre) {
         float q = 0.0f;
 #pragma unroll
         for (int c = 0; c < N; ++c) {
-            const float d = v[c] - centre;
-            q = fmaf(d, d, q);
+            v[c] -= centre;
+            q = fmaf(v[c], v[c], q);
         }
         return q;
     }
+}
+// sum / n by the reciprocal of n, rounded once.
+__device__ __forceinline__ float quotient(float sum, float n, float inv) {
+    const float m = sum * inv;
+    return fmaf(fmaf(-m, n, sum), inv, m);
 }
 
 // to = a b, sum += a b, sum += a, of N of them; the sum of a b; a =
@@ -269,7 +276,7 @@ struct Team {
     const int t, id, warp, lane, hidden;
     const bool second;        // the half of the warp that looks after the second of two sums
     const uint32_t tries;
-    float inv, own_inv;       // 1 / hidden, 1 / values of this warp's (0 for none)
+    float inv, own, own_inv;  // 1 / hidden; values of this warp's, 1 / them (0 for none)
     float slot_own, slot_inv;  // of the warp whose slot this lane reads
     int turn = 0;
     bool in[PACKS];
@@ -283,9 +290,10 @@ struct Team {
         : shared(sh), t(threadIdx.x % SPAN), id(threadIdx.x / SPAN), warp(threadIdx.x / 32 % W), lane(threadIdx.x & 31),
           hidden(h), second((threadIdx.x & 16) != 0), tries(*static_cast<volatile uint32_t *>(&g_wait_tries)),
           stage_bytes(rows.arrays * rows.row_bytes) {
-        const int own = values_of(warp), other = values_of(lane % W);
+        const int mine = values_of(warp), other = values_of(lane % W);
         inv = 1.0f / static_cast<float>(h);
-        own_inv = own ? 1.0f / static_cast<float>(own) : 0.0f;
+        own = static_cast<float>(mine);
+        own_inv = mine ? 1.0f / own : 0.0f;
         slot_own = static_cast<float>(other);
         slot_inv = other ? 1.0f / static_cast<float>(other) : 0.0f;
 #pragma unroll
@@ -420,36 +428,45 @@ struct Team {
         const float r = rsqrtf(v);
         return v < INFINITY ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
     }
-    // Mean and reciprocal root of what a row is divided by, of two rows at once (or
-    // one twice): each warp's sum, its squares about its own mean, then the team's.
-    __device__ __forceinline__ void stats2(const float (&u)[E], const float (&v)[E], bool two, bool rms, float eps,
-                                           float *mean_u, float *r_u, float *mean_v, float *r_v) {
-        float su = 0.0f, sv = 0.0f, sum = 0.0f, cu = 0.0f, cv = 0.0f;
+    // Rows u and v at once (or one: two false): their values less the warp's own mean,
+    // in place, and what takes them to the normalised row, n = u r + shift: the
+    // reciprocal root of the variance and the rest of the mean.  Each warp's sum, its
+    // squares about its mean, then the team's.  The difference comes before the product:
+    // as u r - mean r the rounding of mean r is left, 1e-3 of a constant row of 100s.
+    // The mean is carried in two parts, so a row whose sum f32 holds is off by no more
+    // than its products' roundings.
+    __device__ __forceinline__ void stats2(float (&u)[E], float (&v)[E], bool two, bool rms, float eps, float *shift_u,
+                                           float *r_u, float *shift_v, float *r_v) {
+        float su = 0.0f, sv = 0.0f, sum = 0.0f, centre = 0.0f, cu = 0.0f, cv = 0.0f;
         if (!rms) {
             su = values_sum<E>(u);
             if (two) sv = values_sum<E>(v);
             sum = halves_sum(su, sv);
-            both(sum * own_inv, cu, cv);
+            centre = quotient(sum, own, own_inv);
+            both(centre, cu, cv);
         }
         float qu = 0.0f, qv = 0.0f;
 #pragma unroll
         for (int i = 0; i < PACKS; ++i)
             if (in[i]) {
-                qu += squares_about<N>(u + i * N, cu);
-                if (two) qv += squares_about<N>(v + i * N, cv);
+                qu += centre_squares<N>(u + i * N, cu);
+                if (two) qv += centre_squares<N>(v + i * N, cv);
             }
-        float q = halves_sum(qu, qv), mean = sum * own_inv;
+        float q = halves_sum(qu, qv), rest;
         if constexpr (W > 1) {
             float2(*s)[W] = slot();
             if ((lane & 15) == 0) s[second][warp] = make_float2(sum, q);
             barrier();
             const float2 o = s[second][lane % W];
-            mean = slots_sum(o.x) * inv;
-            const float d = rms ? 0.0f : fmaf(o.x, slot_inv, -mean);
+            const float all = static_cast<float>(hidden), total = slots_sum(o.x), mean = quotient(total, all, inv);
+            const float d = rms ? 0.0f : quotient(o.x, slot_own, slot_inv) - mean;
             q = slots_sum(fmaf(slot_own * d, d, o.y));
+            rest = (mean - centre) + fmaf(-mean, all, total) * inv;
+        } else {
+            rest = fmaf(-centre, own, sum) * own_inv;
         }
         const float r = root(fmaf(q, inv, eps));
-        both(mean, *mean_u, *mean_v);
+        both(-rest * r, *shift_u, *shift_v);
         both(r, *r_u, *r_v);
     }
     // Copies that a wait gave up on get another 200 us to land before the block
@@ -508,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             gate_end = (group + 1) * p.per_gate;
         }
         team.wait();
-        float v[E], mean = 0.0f, r = 1.0f, none;
+        float v[E], shift = 0.0f, r = 1.0f, none;
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
             float u[N] = {};
@@ -517,8 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int c = 0; c < N; ++c) v[i * N + c] = u[c];
         }
         if (branch) {
-            if (post) team.stats2(v, v, false, rms, p.eps, &mean, &r, &none, &none);
-            const float shift = -mean * r;
+            if (post) team.stats2(v, v, false, rms, p.eps, &shift, &r, &none, &none);
 #pragma unroll
             for (int i = 0; i < PACKS; ++i)
                 if (team.in[i]) {
@@ -556,8 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
         }
         if (pre) {
-            team.stats2(v, v, false, rms, p.eps, &mean, &r, &none, &none);
-            const float shift = -mean * r;
+            team.stats2(v, v, false, rms, p.eps, &shift, &r, &none, &none);
 #pragma unroll
             for (int i = 0; i < PACKS; ++i)
                 if (team.in[i]) {
@@ -670,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         int64_t row, last;
         for (unit_rows(unit, &row, &last); row < last; ++row) {
             team.wait();
-            float v[E], b[E], dt[E], mean2, r2, mean1 = 0.0f, r1 = 1.0f;
+            float v[E], b[E], dt[E], shift2, r2, shift1 = 0.0f, r1 = 1.0f;
 #pragma unroll
             for (int i = 0; i < PACKS; ++i) {
                 float u[N] = {}, w[N] = {};
@@ -680,8 +695,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int c = 0; c < N; ++c) v[i * N + c] = u[c], b[i * N + c] = w[c];
             }
             if (pre) {
-                team.stats2(v, b, post, rms, p.eps, &mean2, &r2, &mean1, &r1);
-                const float shift2 = -mean2 * r2;
+                team.stats2(v, b, post, rms, p.eps, &shift2, &r2, &shift1, &r1);
                 float sq = 0.0f, sqn = 0.0f;
 #pragma unroll
                 for (int i = 0; i < PACKS; ++i)
@@ -706,12 +720,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < PACKS; ++i) combine<N>(dt + i * N, v + i * N, -sqn, -sq, r2);
             } else {
-                if (post) team.stats2(b, b, false, rms, p.eps, &mean1, &r1, &mean2, &r2);
+                if (post) team.stats2(b, b, false, rms, p.eps, &shift1, &r1, &shift2, &r2);
 #pragma unroll
                 for (int e = 0; e < E; ++e) dt[e] = 0.0f;
             }
-            if (!post) mean1 = 0.0f, r1 = 1.0f;
-            const float shift1 = -mean1 * r1;
+            if (!post) shift1 = 0.0f, r1 = 1.0f;
 #pragma unroll
             for (int i = 0; i < PACKS; ++i)
                 if (team.in[i]) {

@@ -318,3 +318,65 @@ def test_refusals(cuda):
     wide = torch.zeros(1, 8200, device="cuda")
     with pytest.raises(Exception, match="8192"):
         cuda.residual_norm(wide, wide)
+
+
+# values of at most 11 bits: f32 holds every sum of 8192 of them, so a row's mean is exact or its nearest f32
+CONSTANT = {"f32": [7.5, 100.0, 1000.5, -30000.0], "bf16": [7.5, 100.0, 0.1015625], "f16": [7.5, 1000.5, 0.0999755859375]}
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("hidden", [1, 37, 40, 100, 264, 1000, 1024, 4104, 8192])
+def test_constant_rows_give_beta(cuda, rows, hidden):
+    """Whatever the constant: y is gate * beta and h beta, to the bit, and the
+    gammas' gradients are 0; by parameters in shared memory, in registers and for
+    each group's gate.  dbranch is r (w - mean w), a row's sum rounding by ROW."""
+    import torch
+    rng = np.random.default_rng(hidden)
+    for dtype, values in CONSTANT.items():
+        for i, c in enumerate(values):
+            b = torch.full((rows, hidden), c, dtype=_t(dtype), device="cuda")
+            assert float(b[0, 0]) == c
+            ones = torch.ones(hidden, device="cuda")
+            gate = torch.full((rows, hidden) if i % 2 else (hidden,), 1.5, device="cuda")
+            p = dict(post_gamma=ones * 3, post_beta=ones * 0.25, gate=gate, pre_gamma=ones * 5)
+            y, h = cuda.residual_norm(torch.zeros_like(b), b, pre_beta=ones * 0.125, **p)
+            assert (y == 0.375).all() and (h == 0.125).all()
+            _, h = cuda.residual_norm(b, None, pre_gamma=ones * 5, pre_beta=ones * 0.125)
+            assert (h == 0.125).all()
+            dy, fdy = _rows(rng, (rows, hidden), dtype)
+            g = cuda.residual_norm_bwd(dy, dy, y, b, **p)
+            assert not g.dpost_gamma.any() and not g.dpre_gamma.any()
+            assert not cuda.residual_norm_bwd(dy, dy, b, None, pre_gamma=ones).dpre_gamma.any()
+            g = cuda.residual_norm_bwd(dy, None, y, b, post_gamma=ones * 3, gate=gate)
+            assert not g.dpost_gamma.any()
+            w, r = fdy * 4.5, 1 / np.sqrt(1e-5)
+            S.check(g.dbranch, r * (w - w.mean(-1, keepdims=True)),
+                    2 * S.ROW * r * (np.abs(w) + np.abs(w).mean(-1, keepdims=True)), dtype)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("hidden", [37, 40, 100, 1000, 1024, 4104, 8192])
+def test_nearly_constant_rows(cuda, rows, hidden):
+    """Rows of 1000.5 with a step of 0.5 here and there, whose sums f32 holds: the
+    deviations are exact and the mean has twice f32's digits, so n is off by the
+    root's ROW and eight roundings of its own, not by those of 1000.5 r."""
+    import torch
+    rng = np.random.default_rng(hidden + rows)
+    fb = 1000.5 + 0.5 * rng.integers(0, 3, (rows, hidden)) * (rng.random((rows, hidden)) < 0.1)
+    fb[:, 0] += 0.5
+    b = torch.from_numpy(fb.astype(np.float32)).cuda()
+    ones = torch.ones(hidden, device="cuda")
+    n, r = S.stats(fb, "layer", 1e-5)
+    en = (S.ROW + 8 * S.U) * np.abs(n)
+    S.check(cuda.residual_norm(torch.zeros_like(b), b, post_gamma=ones)[0], n, en, "f32")
+    S.check(cuda.residual_norm(b, None, pre_gamma=ones)[1], n, en, "f32")
+    dy, fdy = _rows(rng, (rows, hidden), "f32")
+    want, bound = S._through_norm(fdy, np.zeros_like(fdy), n, en, r, "layer")
+    terms = np.abs(fdy) * en
+    sums = (fdy * n).sum(0), terms.sum(0) + (rows + 64) * S.U * np.abs(fdy * n).sum(0)
+    g = cuda.residual_norm_bwd(dy, None, b, b, post_gamma=ones)
+    S.check(g.dbranch, want, bound, "f32")
+    S.check(g.dpost_gamma, *sums, "f32")
+    g = cuda.residual_norm_bwd(None, dy, b, None, pre_gamma=ones)
+    S.check(g.dx, want, bound, "f32")
+    S.check(g.dpre_gamma, *sums, "f32")
