@@ -912,6 +912,12 @@ __global__ void __launch_bounds__(32 * MANY_WARPS)
     }
 }
 
+// The shared memory that a launch may have.  The attribute that admits it belongs to the
+// kernel, which serves rows of many lengths on many host threads, so it is set to one
+// value for all of them: with each launch's own, two threads' calls could set it and
+// launch by turns, and the longer rows' launch was refused.
+constexpr int MOST_SHARED = 208 * 1024;
+
 // The ring's shape and the grid for f(T, VEC, W, PACKS, grid, shared memory): MOST
 // values a thread (8 where one warp can take the row so), the fewest warps a team.
 // `params`: bytes of parameters that would lie beside the ring; *staged, whether they do.
@@ -924,7 +930,7 @@ void launch(int32_t dtype, bool vec, int64_t hidden, Rows &in, int64_t rows, int
     in.row_bytes = static_cast<int32_t>((hidden * experts::width(dtype) + 15) / 16 * 16);
     const int64_t stage = static_cast<int64_t>(in.arrays) * in.row_bytes * teams;
     // the parameters, where that leaves two stages, or the one that there is
-    const int64_t room = 208 * 1024, beside = vec ? (room - params) / stage : 0;
+    const int64_t room = MOST_SHARED, beside = vec ? (room - params) / stage : 0;
     *staged = params > 0 && (beside >= 2 || (beside == 1 && room / stage == 1));
     const int64_t stages = vec ? (*staged ? beside : room / stage) : 0;
     in.stages = static_cast<int32_t>(stages > MAX_STAGES ? MAX_STAGES : stages);
@@ -990,7 +996,7 @@ extern "C" int chelis_cuda_residual_norm(int32_t dtype, int32_t kind, int64_t ro
     int rc = CHELIS_CUDA_OK;
     const auto run = [&](auto t, auto v, auto w, auto packs, unsigned grid, size_t smem) {
         auto kernel = rnorm::fwd_kernel<decltype(t), decltype(v)::value, decltype(w)::value, decltype(packs)::value>;
-        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, rnorm::MOST_SHARED),
                         "cudaFuncSetAttribute");
         if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, current_stream()>>>(p, in);
     };
@@ -1071,7 +1077,7 @@ extern "C" int chelis_cuda_residual_norm_bwd(int32_t dtype, int32_t kind, int64_
             p.unit_sums = unit_sums ? sums : nullptr;
             p.pre_sums = pre_sums ? sums + unit_n : nullptr;
             auto kernel = rnorm::bwd_kernel<decltype(t), decltype(v)::value, W, decltype(packs)::value, decltype(parts)::value>;
-            rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+            rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, rnorm::MOST_SHARED),
                             "cudaFuncSetAttribute");
             if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, s>>>(p, in);
         };

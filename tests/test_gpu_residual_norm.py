@@ -380,3 +380,41 @@ def test_nearly_constant_rows(cuda, rows, hidden):
     g = cuda.residual_norm_bwd(None, dy, b, None, pre_gamma=ones)
     S.check(g.dx, want, bound, "f32")
     S.check(g.dpre_gamma, *sums, "f32")
+
+
+def test_two_threads_with_rows_of_different_lengths(cuda):
+    """Calls of one kernel with different needs of shared memory, from two host
+    threads that do little else, all launch and give their bits."""
+    import threading
+
+    import torch
+    from chelis_b200 import lib as L
+    lib = L.load()
+    jobs = []
+    for hidden in (1024, 264):
+        rng = np.random.default_rng(hidden)
+        x, b = (_rows(rng, (300, hidden), "bf16")[0] for _ in range(2))
+        gamma = torch.ones(hidden, device="cuda")
+        y, h, s = torch.empty_like(x), torch.empty_like(x), torch.cuda.Stream()
+        args = cuda._residual_norm.pack(s.cuda_stream, L.DTYPE_BF16, L.NORM_LAYER, 300, hidden, x.data_ptr(), b.data_ptr(),
+                                        gamma.data_ptr(), 0, 0, 1, 1.0, gamma.data_ptr(), 0, 1e-5, y.data_ptr(), h.data_ptr())
+        jobs.append((args, s, y, h, cuda.residual_norm(x, b, post_gamma=gamma, pre_gamma=gamma), (x, b, gamma)))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(args):
+        for _ in range(30000):
+            if lib.chelis_cuda_call_packed(L.PACKED_RESIDUAL_NORM, args):
+                failed.append(L.last_error())
+                return
+
+    threads = [threading.Thread(target=work, args=(job[0],)) for job in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for _, _, y, h, want, _ in jobs:
+        assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    cuda.device_status()
