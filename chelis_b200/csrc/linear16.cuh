@@ -6,9 +6,10 @@
 //
 // Q(a) = 1 - Phi(a) = e^(-a^2/2) R(a) with R(a) = erfcx(a / sqrt 2) / 2 smooth:
 // a polynomial of degree 7 in t = 1 / (1 + 0.35 a), fitted to least relative
-// error over 0 <= a <= 14.5 (3e-7; 6e-7 in f32), past which Q is below f32.  So
-// the tail keeps its relative accuracy, as erfc would, at about 17 instructions
-// a value: an epilogue that calls erfcf and expf leaves the tensor core idle.
+// error over 0 <= a <= 14.5 (3e-7; 6e-7 in f32).  So the tail keeps its relative
+// accuracy, as erfc would, at about 17 instructions a value: an epilogue that calls
+// erfcf and expf leaves the tensor core idle.  From a = 13.2 on e^(-a^2/2) is below
+// 2^-126 and taken for 0, which is 5e-39 of gelu and 6e-38 of its slope.
 // Against 16-bit results, half a step of which is 2^-9 or 2^-12, this is exact.
 #pragma once
 
@@ -104,7 +105,9 @@ __device__ __forceinline__ f32x2 gelu_slope(const GeluConstants<HOLD> &k, f32x2 
     const float2 h = gemm8::unpack2(mul2(e, fma2(na, k.density, r)));
     return gemm8::pack2(z.x < 0.0f ? h.x : 1.0f - h.x, z.y < 0.0f ? h.y : 1.0f - h.y);
 }
-__device__ __forceinline__ float sigmoid(float z) { return rcp(1.0f + ex2(z * -1.44269504089f)); }
+// A quarter of 1 + e^-z, so that the reciprocal of one between 2^126 and 2^128 (z below
+// -87.33) is no number that the hardware's takes for 0; s itself may be one.
+__device__ __forceinline__ float sigmoid(float z) { return 0.25f * rcp(fmaf(ex2(z * -1.44269504089f), 0.25f, 0.25f)); }
 __device__ __forceinline__ float silu_value(float z) {
     return max_nan(z, -128.0f) * sigmoid(z);  // s(-128) is 0 in f32
 }

@@ -421,3 +421,21 @@ def test_long_sums_do_not_drift(cuda, m, n, k):
         got = cuda.matmul16(a, b, trans_a=True, dtype=torch.float32)
         ref = a.double().t() @ b.double()
         assert float(((got.double() - ref).abs() / ref).max()) <= 2.0 ** -16 + k / 1024 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("m", [4, 64])
+@pytest.mark.parametrize("dtype", DT)
+def test_activations_of_far_negative_numbers(cuda, dtype, m):
+    """Where e^-z and e^(-z^2/2) come to the ends of f32's range: silu keeps its
+    digits down to -88.7, results of both widths as close as the bounds say."""
+    import torch
+    v = torch.tensor([-86.0, -87.3, -87.35, -87.4, -87.6, -88.0, -88.3, -88.5, -88.7, -89.0, -12.9, -13.1, -13.2, -13.3, -13.5, -14.4],
+                     device="cuda")
+    a = torch.zeros(m, 16, dtype=_t(dtype), device="cuda")
+    b = torch.zeros(16, v.numel(), dtype=_t(dtype), device="cuda")
+    z = v.double().cpu().numpy()
+    for activation in ("silu", "gelu"):
+        ref = S.act(z, activation)[0]
+        bound = S.act_error(z, activation) + 2 * S.U * np.abs(ref)
+        for out in ("f32", dtype):
+            S.check(cuda.matmul16(a, b, bias=v, activation=activation, dtype=_t(out))[m - 1], ref, bound, out)
