@@ -902,14 +902,17 @@ __global__ void __launch_bounds__(32 * FEW_WARPS)
 }
 
 // ---- activation's gradient, column sums -----------------------------------
+// dz may be dy: plain loads of it, each before its own store.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    act_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ z, int64_t count, int32_t act, T *__restrict__ dz) {
+    act_bwd_kernel(const T *dy, const T *__restrict__ z, int64_t count, int32_t act, T *dz) {
     using P = experts::Pack<T, VEC>;
     const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * P::N;
     for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * P::N; i < count; i += step) {
-        const P g = experts::load_pack<T, VEC>(dy + i), x = experts::load_pack<T, VEC>(z + i);
-        P o;
+        const P x = experts::load_pack<T, VEC>(z + i);
+        P g, o;
+        if constexpr (VEC) *reinterpret_cast<uint4 *>(&g) = *reinterpret_cast<const uint4 *>(dy + i);
+        else g.v[0] = dy[i];
 #pragma unroll
         for (int c = 0; c < P::N; ++c)
             o.v[c] = experts::from_f32<T>(slope_times(experts::to_f32(g.v[c]), experts::to_f32(x.v[c]), act));

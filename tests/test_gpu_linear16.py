@@ -439,3 +439,34 @@ def test_activations_of_far_negative_numbers(cuda, dtype, m):
         bound = S.act_error(z, activation) + 2 * S.U * np.abs(ref)
         for out in ("f32", dtype):
             S.check(cuda.matmul16(a, b, bias=v, activation=activation, dtype=_t(out))[m - 1], ref, bound, out)
+
+
+@pytest.mark.parametrize("count", [1, 37, 4096, 8 * 300 * 3, 5000000])
+def test_activation_gradients_in_place(cuda, count):
+    """dz may be dy, by the C entry."""
+    import torch
+    from chelis_b200 import lib as L
+    for dtype, code in (("bf16", L.DTYPE_BF16), ("f16", L.DTYPE_F16)):
+        gen = torch.Generator(device="cuda").manual_seed(count)
+        dy, z = (torch.randn(count, generator=gen, device="cuda").to(_t(dtype)) for _ in range(2))
+        for activation, act in (("gelu", L.ACT_GELU), ("silu", L.ACT_SILU), ("relu", L.ACT_RELU)):
+            want, own = cuda.activation16_bwd(dy, z, activation), dy.clone()
+            L.call("chelis_cuda_activation16_bwd", code, act, own.data_ptr(), z.data_ptr(), count, own.data_ptr())
+            assert torch.equal(own, want)
+
+
+@pytest.mark.parametrize("m,n,k,out", [(8, 64, 136, "f32"), (300, 264, 136, "f32"), (300, 263, 136, "f32"), (90, 264, 4160, None),
+                                       (90, 263, 4160, "f32"), (300, 5000, 2200, "f32"), (300, 2604, 2200, "f32")])
+def test_residual_may_be_the_result_in_f32_and_in_parts(cuda, m, n, k, out):
+    import torch
+    from chelis_b200 import lib as L
+    rng = np.random.default_rng(m + n + k)
+    for activation, act in ((None, L.ACT_NONE), ("silu", L.ACT_SILU)):
+        a, _ = _make(rng, (m, k), "f16")
+        b, _ = _make(rng, (k, n), "f16", 0.1)
+        r, _ = _make(rng, (m, n), out or "f16")
+        want = cuda.matmul16(a, b, activation=activation, residual=r, dtype=r.dtype)
+        code = L.DTYPE_F32 if out else L.DTYPE_F16
+        L.call("chelis_cuda_matmul16", L.DTYPE_F16, 0, 0, m, n, k, a.data_ptr(), b.data_ptr(), None, 0, act, r.data_ptr(), None,
+               None, code, r.data_ptr())
+        assert torch.equal(want, r)

@@ -218,3 +218,18 @@ def test_reference_norm_gradients_against_differences(kind):
         d = rng.standard_normal(at[name].shape)
         numeric = (loss(dict(at, **{name: at[name] + 1e-6 * d})) - loss(dict(at, **{name: at[name] - 1e-6 * d}))) / 2e-6
         assert abs(numeric - (grads["d" + name][0] * d).sum()) < 1e-6
+
+
+def _kernel(file, name):
+    """The source of a kernel, from its name to the brace that ends it."""
+    import os
+    from chelis_b200 import build
+    text = open(os.path.join(build.CSRC, file)).read()
+    return text[text.index(f"    {name}("):].split("\n}\n")[0]
+
+
+def test_gradients_that_may_be_results_are_no_read_only_data():
+    """activation16_bwd's dz may be dy: neither may be promised to the compiler as
+    read alone, by __restrict__ or by __ldg."""
+    text = _kernel("linear16.cu", "act_bwd_kernel")
+    assert "const T *dy" in text and "T *dz" in text and "__ldg" not in text and "load_pack<T, VEC>(dy" not in text
