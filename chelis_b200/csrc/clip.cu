@@ -70,8 +70,13 @@ __device__ __forceinline__ double squares(const float (&v)[N]) {
 }
 
 // `count` numbers by THREADS threads: single ones up to 16 bytes' alignment, packs,
-// single ones.
-template <int THREADS, typename T>
+// single ones.  READ_ONLY: no one writes them in this launch.
+template <bool READ_ONLY>
+__device__ __forceinline__ uint4 load_packed(const uint4 *p) {
+    if constexpr (READ_ONLY) return __ldg(p);
+    else return *p;
+}
+template <int THREADS, bool READ_ONLY, typename T>
 __device__ __forceinline__ double chunk_squares(const T *p, int64_t count, int thread) {
     constexpr int N = 16 / sizeof(T), DEEP = 8;
     double sum = 0.0;
@@ -82,7 +87,7 @@ __device__ __forceinline__ double chunk_squares(const T *p, int64_t count, int t
     for (; i + (DEEP - 1) * THREADS < packs; i += DEEP * THREADS) {
         uint4 u[DEEP];
 #pragma unroll
-        for (int d = 0; d < DEEP; ++d) u[d] = __ldg(q + i + d * THREADS);
+        for (int d = 0; d < DEEP; ++d) u[d] = load_packed<READ_ONLY>(q + i + d * THREADS);
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
             float v[N];
@@ -92,7 +97,7 @@ __device__ __forceinline__ double chunk_squares(const T *p, int64_t count, int t
     }
     for (; i < packs; i += THREADS) {
         float v[N];
-        wide<T>(__ldg(q + i), v);
+        wide<T>(load_packed<READ_ONLY>(q + i), v);
         sum += squares(v);
     }
     const int64_t tail = head + packs * N;
@@ -107,11 +112,12 @@ __device__ __forceinline__ double chunk_squares(const T *p, int64_t count, int t
     return sum;
 }
 
-template <int THREADS>
+template <int THREADS, bool READ_ONLY>
 __device__ __forceinline__ double squares_part(const Entry &e, int64_t at, int64_t count, int thread) {
-    if (e.in == CHELIS_DTYPE_F32) return chunk_squares<THREADS>(static_cast<const float *>(e.src) + at, count, thread);
-    if (e.in == CHELIS_DTYPE_BF16) return chunk_squares<THREADS>(static_cast<const __nv_bfloat16 *>(e.src) + at, count, thread);
-    return chunk_squares<THREADS>(static_cast<const __half *>(e.src) + at, count, thread);
+    if (e.in == CHELIS_DTYPE_F32) return chunk_squares<THREADS, READ_ONLY>(static_cast<const float *>(e.src) + at, count, thread);
+    if (e.in == CHELIS_DTYPE_BF16)
+        return chunk_squares<THREADS, READ_ONLY>(static_cast<const __nv_bfloat16 *>(e.src) + at, count, thread);
+    return chunk_squares<THREADS, READ_ONLY>(static_cast<const __half *>(e.src) + at, count, thread);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         const Entry &e = table.t[tensor];
         const int64_t at = static_cast<int64_t>(c - e.first) * CHUNK;
         const int64_t count = e.count - at < CHUNK ? e.count - at : CHUNK;
-        sum += squares_part<THREADS>(e, at, count, threadIdx.x);
+        sum += squares_part<THREADS, true>(e, at, count, threadIdx.x);
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(THREADS)
     for (int c = warp; c < table.chunks; c += THREADS / 32) {
         const Entry &e = table.t[tensor_of(table, c)];
         const int64_t at = static_cast<int64_t>(c - e.first) * FEW_CHUNK;
-        sum += squares_part<32>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, lane);
+        sum += squares_part<32, !SCALE>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, lane);
     }
     const double v = sqrt(block_sum(sum));
     if (threadIdx.x == 0) *norm = static_cast<float>(v);

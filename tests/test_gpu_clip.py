@@ -196,3 +196,14 @@ def test_refusals(cuda):
         with pytest.raises(L.ChelisCudaError):
             bad()
     assert (a == 1).all() and (b == 1).all()
+
+
+@pytest.mark.parametrize("sizes", [[1], [7, 0, 33], [1000, 24000, 1], [2000] * 32, [65536]])
+def test_few_numbers_in_place_are_those_out_of_place(cuda, sizes):
+    """One block reads the numbers for the norm and scales them in the same launch."""
+    import torch
+    for dtype in ("f32", "bf16", "f16"):
+        g = _make(sizes, [dtype] * len(sizes))
+        out = [torch.empty_like(t) for t in g]
+        norm = cuda.clip_grads(g, 0.25, out=out)
+        assert torch.equal(cuda.clip_grads(g, 0.25), norm) and all(torch.equal(a, b) for a, b in zip(g, out))

@@ -233,3 +233,9 @@ def test_gradients_that_may_be_results_are_no_read_only_data():
     read alone, by __restrict__ or by __ldg."""
     text = _kernel("linear16.cu", "act_bwd_kernel")
     assert "const T *dy" in text and "T *dz" in text and "__ldg" not in text and "load_pack<T, VEC>(dy" not in text
+
+
+def test_numbers_that_are_clipped_in_place_are_no_read_only_data():
+    """One launch reads few numbers for their norm and scales them: by plain loads."""
+    text = _kernel("clip.cu", "small_kernel")
+    assert "squares_part<32, !SCALE>" in text and "__restrict__" not in text and "__ldg" not in text
