@@ -180,9 +180,21 @@ __global__ void __launch_bounds__(THREADS)
     if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
+// What the numbers are multiplied by.
+struct Factor {
+    float f;
+    double tiny;  // f itself where it is below 2^-126, of which f32 lacks digits; else 0
+};
+
 template <int THREADS, typename T, typename U>
-__device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, float c, int thread) {
+__device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, Factor factor, int thread) {
     constexpr int N = 16 / sizeof(T), DEEP = 8;
+    if (factor.tiny != 0.0) {
+        for (int64_t i = thread; i < count; i += THREADS)
+            o[i] = experts::from_f32<U>(static_cast<float>(static_cast<double>(experts::to_f32(p[i])) * factor.tiny));
+        return;
+    }
+    const float c = factor.f;
     const int64_t skew = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T);
     int64_t head = skew < count ? skew : count;
     // packs want the result aligned as well as the source
@@ -220,7 +232,7 @@ __device__ __forceinline__ void scale_chunk(const T *p, U *o, int64_t count, flo
         o[tail + thread] = experts::from_f32<U>(experts::to_f32(p[tail + thread]) * c);
 }
 template <int THREADS, typename T>
-__device__ __forceinline__ void scale_as(const Entry &e, int64_t at, int64_t count, float c, int thread) {
+__device__ __forceinline__ void scale_as(const Entry &e, int64_t at, int64_t count, Factor c, int thread) {
     const T *p = static_cast<const T *>(e.src) + at;
     if (e.out == CHELIS_DTYPE_F32) scale_chunk<THREADS>(p, static_cast<float *>(e.dst) + at, count, c, thread);
     else if (e.out == CHELIS_DTYPE_BF16) scale_chunk<THREADS>(p, static_cast<__nv_bfloat16 *>(e.dst) + at, count, c, thread);
@@ -228,15 +240,17 @@ __device__ __forceinline__ void scale_as(const Entry &e, int64_t at, int64_t cou
 }
 
 template <int THREADS>
-__device__ __forceinline__ void scale_part(const Entry &e, int64_t at, int64_t count, float c, int thread) {
+__device__ __forceinline__ void scale_part(const Entry &e, int64_t at, int64_t count, Factor c, int thread) {
     if (e.in == CHELIS_DTYPE_F32) scale_as<THREADS, float>(e, at, count, c, thread);
     else if (e.in == CHELIS_DTYPE_BF16) scale_as<THREADS, __nv_bfloat16>(e, at, count, c, thread);
     else scale_as<THREADS, __half>(e, at, count, c, thread);
 }
 
 // A norm that is reported as infinite or NaN changes nothing.
-__device__ __forceinline__ float factor(double norm, float max_norm) {
-    return norm > max_norm && static_cast<float>(norm) < INFINITY ? static_cast<float>(max_norm / norm) : 1.0f;
+__device__ __forceinline__ Factor factor(double norm, float max_norm) {
+    if (!(norm > max_norm && static_cast<float>(norm) < INFINITY)) return {1.0f, 0.0};
+    const double c = max_norm / norm;
+    return {static_cast<float>(c), c < 0x1p-126 ? c : 0.0};
 }
 
 template <int N>
@@ -245,13 +259,13 @@ __global__ void __launch_bounds__(THREADS, 2)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const double v = total_norm(sums, n);
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = static_cast<float>(v);
-    const float c = factor(v, max_norm);
+    const Factor c = factor(v, max_norm);
     const int first = block_first(table.chunks, blockIdx.x), last = block_first(table.chunks, blockIdx.x + 1);
     int tensor = first < last ? tensor_of(table, last - 1) : 0;
     for (int chunk = last - 1; chunk >= first; --chunk) {
         while (table.t[tensor].first > chunk) --tensor;
         const Entry &e = table.t[tensor];
-        if (c == 1.0f && e.src == e.dst) continue;  // as they are
+        if (c.f == 1.0f && e.src == e.dst) continue;  // as they are
         const int64_t at = static_cast<int64_t>(chunk - e.first) * CHUNK;
         const int64_t count = e.count - at < CHUNK ? e.count - at : CHUNK;
         scale_part<THREADS>(e, at, count, c, threadIdx.x);
@@ -276,12 +290,12 @@ __global__ void __launch_bounds__(THREADS)
     const double v = sqrt(block_sum(sum));
     if (threadIdx.x == 0) *norm = static_cast<float>(v);
     if (!SCALE) return;
-    const float f = factor(v, max_norm);
-    for (int c = warp; c < table.chunks; c += THREADS / 32) {
-        const Entry &e = table.t[tensor_of(table, c)];
-        if (f == 1.0f && e.src == e.dst) continue;
-        const int64_t at = static_cast<int64_t>(c - e.first) * FEW_CHUNK;
-        scale_part<32>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, f, lane);
+    const Factor c = factor(v, max_norm);
+    for (int chunk = warp; chunk < table.chunks; chunk += THREADS / 32) {
+        const Entry &e = table.t[tensor_of(table, chunk)];
+        if (c.f == 1.0f && e.src == e.dst) continue;
+        const int64_t at = static_cast<int64_t>(chunk - e.first) * FEW_CHUNK;
+        scale_part<32>(e, at, e.count - at < FEW_CHUNK ? e.count - at : FEW_CHUNK, c, lane);
     }
 }
 

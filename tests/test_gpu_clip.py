@@ -207,3 +207,26 @@ def test_few_numbers_in_place_are_those_out_of_place(cuda, sizes):
         out = [torch.empty_like(t) for t in g]
         norm = cuda.clip_grads(g, 0.25, out=out)
         assert torch.equal(cuda.clip_grads(g, 0.25), norm) and all(torch.equal(a, b) for a, b in zip(g, out))
+
+
+@pytest.mark.parametrize("sizes", [[1000, 33], [1000, 70001, 5]])
+@pytest.mark.parametrize("scale,bound", [(1e25, 1.0), (1e25, 1e-3), (1e35, 1e-3), (1e35, 1e-8), (1e35, 1e-30), (1e35, 1e-44), (1e35, 0.0),
+                                         (1.0, 1e-36), (1e-3, 1e-42)])
+def test_clipping_by_a_factor_outside_f32(cuda, sizes, scale, bound):
+    """A factor below 2^-126 keeps its digits: numbers of a finite norm come out
+    as the formula says, with half a step of what they are where they vanish."""
+    import torch
+    bound = float(np.float32(bound))
+    for out in ("f32", "bf16"):
+        g = _make(sizes, ["f32", "bf16" if scale > 1e3 else "f32", "f32"][:len(sizes)], scale)
+        ref = _norm(g)
+        assert bound < ref < 3e38
+        dst = [torch.full_like(t, 9.0, dtype=_t(out)) for t in g]
+        norm = cuda.clip_grads(g, bound, out=dst)
+        assert abs(float(norm) - ref) <= 8 * U * ref
+        for a, b in zip(dst, g):
+            _check(a, b, bound / ref)
+        own = [t.clone() for t in g]
+        cuda.clip_grads(own, bound)
+        for a, b in zip(own, g):
+            _check(a, b, bound / ref)
