@@ -479,13 +479,17 @@ struct Team {
 };
 
 // By the whole block: parameters as Team::staged takes them, times `factor`'s if
-// that is given, `absent` where there are none.
+// that is given, `absent` where there are none.  Whether all that this thread put
+// there is finite.
 template <int N>
-__device__ __forceinline__ void stage_params(float *to, const float *p, const float *factor, float absent, int hidden) {
+__device__ __forceinline__ bool stage_params(float *to, const float *p, const float *factor, float absent, int hidden) {
+    bool finite = true;
     for (int c = threadIdx.x; c < hidden; c += THREADS) {
         const int at = N == 8 ? (c / 8 * 4 + c % 4) + (c & 4 ? hidden / 2 : 0) : c;
         to[at] = (p ? __ldg(p + c) : absent) * (factor ? __ldg(factor + c) : 1.0f);
+        finite &= fabsf(to[at]) < INFINITY;
     }
+    return finite;
 }
 
 // y = scale x + N1(branch) c1 + c0 with c1 = gate g1, c0 = gate b1, h = N2(y) g2 + b2.
@@ -503,18 +507,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (VEC && team.t == 0)
         for (int s = 0; s < in.stages && first + s < last; ++s) team.fetch(in, first + s, s);
     const bool rms = p.rms != 0, post = p.post_gamma != nullptr, pre = p.pre_gamma != nullptr, branch = p.branch != nullptr;
-    // one gate at most: it goes into c1 and c0
-    const bool staged = VEC && p.staged, one_gate = p.per_gate >= p.rows;
+    // one gate at most: it goes into c1 and c0, unless that leaves f32: gate (n g1 +
+    // b1) is an infinity where gate g1 n + gate b1 may be the difference of two
+    bool staged = VEC && p.staged;
+    const bool one_gate = p.per_gate >= p.rows;
     float *const c1 =
         reinterpret_cast<float *>(rows_smem + static_cast<size_t>(G::TEAMS) * in.stages * in.arrays * in.row_bytes);
     float *const c0 = c1 + p.hidden, *const g2 = c0 + p.hidden, *const b2 = g2 + p.hidden;
     if (staged) {
         const float *g = one_gate ? p.gate : nullptr;
-        stage_params<N>(c1, p.post_gamma, g, 1.0f, p.hidden);
-        stage_params<N>(c0, p.post_beta, g, 0.0f, p.hidden);
+        bool finite = stage_params<N>(c1, p.post_gamma, g, 1.0f, p.hidden);
+        finite &= stage_params<N>(c0, p.post_beta, g, 0.0f, p.hidden);
         stage_params<N>(g2, p.pre_gamma, nullptr, 1.0f, p.hidden);
         stage_params<N>(b2, p.pre_beta, nullptr, 0.0f, p.hidden);
-        __syncthreads();
+        staged = __syncthreads_and(finite);
     }
     const float *gate = nullptr;
     int64_t gate_end = first;

@@ -418,3 +418,37 @@ def test_two_threads_with_rows_of_different_lengths(cuda):
     for _, _, y, h, want, _ in jobs:
         assert torch.equal(y, want[0]) and torch.equal(h, want[1])
     cuda.device_status()
+
+
+@pytest.mark.parametrize("betas", [False, True])
+@pytest.mark.parametrize("hidden", [64, 100, 1024])
+def test_infinite_gates(cuda, hidden, betas):
+    """gate (n gamma + beta) with a gate of inf, -inf, NaN or one whose product with
+    gamma leaves f32: the formula's infinities and NaN, and finite numbers elsewhere,
+    by every way the parameters take."""
+    import torch
+    rng = np.random.default_rng(hidden)
+    for kind in ("layer", "rms"):
+        for post in (True, False):
+            dev, ref = _params(rng, hidden, kind, post, 1, False, betas=betas and post)
+            for p in (dev["gate"], ref["gate"]):
+                p[3], p[5], p[7], p[9] = float("inf"), -float("inf"), float("nan"), 3e38
+            if post:
+                for p in (dev["post_gamma"], ref["post_gamma"]):
+                    p[9] = 2.0 ** -20
+                    p[11] = 3e38
+                for p in (dev["gate"], ref["gate"]):
+                    p[11] = 2.0 ** 20  # gate gamma leaves f32, (n gamma) gate does so too for |n| > 2^-20
+            for rows in (9, 300):
+                x, fx = _rows(rng, (rows, hidden), "f32")
+                b, fb = _rows(rng, (rows, hidden), "f32")
+                y, _ = cuda.residual_norm(x, b, **dev)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    want, bound, _, _ = S.join(fx, fb, ref)
+                    want[np.abs(want) > 3.5e38] *= np.inf
+                y = y.double().cpu().numpy()
+                assert (np.isnan(y) == np.isnan(want)).all()
+                sure = ~np.isnan(want) & ~((np.abs(want) > 3.3e38) & np.isfinite(want))
+                with np.errstate(invalid="ignore"):
+                    same = (y == want) | (np.isfinite(want) & (np.abs(y - want) <= bound))
+                assert same[sure].all()
