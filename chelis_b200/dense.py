@@ -7,8 +7,10 @@ and vector-Jacobian product.
 
 x and the matrices are bf16 or f16, W1 [d, ff] and W2 [ff, d]; norms, gate and
 their gradients are f32, and so are the matrices' gradients.  The second norm,
-the betas, the gate and the biases may be None.  Clip the gradients of a whole
-step with ops.clip_grads, after dp.allreduce_sum where there are several GPUs.
+the betas, the gate and the biases may be None.  Clip the parameters' gradients
+of a whole step (all of feed_forward_bwd's but dx, which is the gradient of what
+comes before) with ops.clip_grads, after dp.allreduce_sum where there are several
+GPUs.
 """
 from __future__ import annotations
 

@@ -70,7 +70,7 @@ def run(case: str) -> None:
         x, dy = randn(16384, d).bfloat16(), randn(16384, d).bfloat16()
         _, saved = dense.feed_forward(x, p)
         grads = dense.feed_forward_bwd(dy, saved, p)
-        ops.clip_grads(grads.values(), 1.0)
+        ops.clip_grads([g for name, g in grads.items() if name != "dx"], 1.0)  # the parameters'
         wide = randn(16384, 4096)
         ops.residual_norm_bwd(wide, wide, wide, wide, post_gamma=randn(4096), gate=randn(8, 4096), pre_gamma=randn(4096))
         logits = randn(16384, 64)

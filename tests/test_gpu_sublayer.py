@@ -155,3 +155,18 @@ def test_routed_layer_with_the_balance_loss(cuda, masked):
         assert float((diff - extra).abs().max()) <= 2e-6 * float(g0[name].abs().max()) + 1e-5 * float(extra.abs().max())
     norm = cuda.clip_grads([g1["dx"], g1["drouter"], g1["dw1"], g1["dw2"]], 1.0)
     assert float(norm) > 1 and abs(float(cuda.grad_norm([g1[n] for n in ("dx", "drouter", "dw1", "dw2")])) - 1) < 1e-5
+
+
+def test_the_profiled_step_clips_the_parameters_alone(cuda, monkeypatch):
+    """dx belongs to what comes before: neither in the norm nor scaled."""
+    from chelis_b200 import profile_cases
+    shapes, clip = [], cuda.clip_grads
+
+    def recorded(grads, *args, **kw):
+        grads = list(grads)
+        shapes.extend(tuple(g.shape) for g in grads)
+        return clip(grads, *args, **kw)
+
+    monkeypatch.setattr(cuda, "clip_grads", recorded)
+    profile_cases.run("sublayer")
+    assert sorted(shapes) == sorted([(1024, 4096), (4096, 1024), (4096,)] + [(1024,)] * 6)
