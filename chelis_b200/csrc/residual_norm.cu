@@ -15,16 +15,19 @@
 // dt branch, kept as s1).  A row's values are taken about its warps' own means, which
 // are put together exactly, so a mean far from 0 costs no digits but those of its sum.
 //
-// 16384 x 1024 bf16, both norms, gate and residual: 34 us (134 MB, 3.9 TB/s; the
+// 16384 x 1024 bf16, both norms, gate and residual: 35 us (134 MB, 3.9 TB/s; the
 // floor is 20): bound by a row's chain of sums at 16 warps a multiprocessor.  With 8
 // values a thread it took 62 (84 instructions a value, most of them a row's fixed
 // ones), with 32 and IEEE divisions away 44, with the parameters in shared memory 34.
-// Gradients of 16384 x 4096 f32 with 8 gates: 291 us (1.61 GB, 5.5 TB/s; the floor is
+// 16384 x 1024 f32 54 us (268 MB, 5.0 TB/s), 16384 x 4096 f32 183 (5.9 TB/s), though of
+// f32 rows of 1024, 2048, 4096 and 8192 shared memory holds no more than those at work.
+// Gradients of 16384 x 4096 f32 with 8 gates: 298 us (1.61 GB, 5.4 TB/s; the floor is
 // 246), 643 with rows loaded as they were wanted, 461 through the ring of bulk copies,
-// and the rest by reciprocals, sums of two at once, pointers carried along and packed
-// instructions.  16384 x 1024 bf16, one norm 39 us (134 MB, 3.5 TB/s), both 72 (2.8
-// TB/s): instructions and a row's chains of sums at 16 warps a multiprocessor; 64 to 86
-// and 107 with every team's sums written out and folded by few warps.
+// 291 by reciprocals, sums of two at once, pointers carried along and packed
+// instructions, the last 7 for the mean's second part.  16384 x 1024 bf16, one norm 42 us
+// (134 MB, 3.2 TB/s), both 76 (2.6 TB/s): instructions and a row's chains of sums at 16
+// warps a multiprocessor; 64 to 86 and 107 with every team's sums written out and folded
+// by few warps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -1006,7 +1009,13 @@ extern "C" int chelis_cuda_residual_norm(int32_t dtype, int32_t kind, int64_t ro
                         "cudaFuncSetAttribute");
         if (rc == CHELIS_CUDA_OK) kernel<<<grid, rnorm::THREADS, smem, current_stream()>>>(p, in);
     };
-    // few rows: eight values a thread, a row over as many warps as there are
+    // Few rows: eight values a thread, a row over as many warps as there are; more: 32,
+    // which have fewer instructions a number and a longer chain of sums.  us with 8 and
+    // with 32, bf16: 148 x 1024 5.4, 8.2, 600 x 1024 6.7, 8.2, 1200 x 1024 9.1, 8.5, 16384 x 1024
+    // 60, 35; 200 x 4096 8.2, 9.3, 300 x 4096 10.4, 9.3; 148 x 8192 7.2, 9.5, 149 x 8192 11.0, 9.7;
+    // f32 200 x 4096 8.7, 9.5, 300 x 4096 11.0, 9.7.  So the rows of 8192 are parted where the
+    // two meet; shorter ones meet at a million numbers, and from 149 rows to there take up
+    // to 3 us more than they would with 8.
     if (rows <= sm_count()) rnorm::launch<8>(dtype, vec, hidden, in, rows, 0, &p.staged, run);
     else rnorm::launch<32>(dtype, vec, hidden, in, rows, 16 * hidden, &p.staged, run);
     CHELIS_TRY(rc);
@@ -1092,7 +1101,8 @@ extern "C" int chelis_cuda_residual_norm_bwd(int32_t dtype, int32_t kind, int64_
         using Post = std::integral_constant<int, rnorm::POST>;
         // Where there are more rows than teams of 8 values a thread, one norm's gradients
         // in 16, which its sums leave registers for: 4800 x 1024 bf16 18.7 us for 22.5 with
-        // 8, 300 x 1024 9.7 for 8.6.  Both norms' in 8.
+        // 8, 300 x 1024 9.7 for 8.6 (both some 4 % less, before means had two parts).  Both
+        // norms' in 8.
         const bool many = vec && hidden > 256 && rows * hidden > sm_count() * 4096ll;
         if (many && dh && !needs_branch && !dbranch)
             rnorm::launch<16>(dtype, vec, hidden, in, rows, 4 * hidden, &p.staged, [&](auto t, auto v, auto... rest) {
