@@ -322,23 +322,26 @@ __device__ __forceinline__ void act_piece(const GeluConstants<HOLD> &k, f32x2 (&
 // drifts towards 0: by 1e-6 of it at k = 1024, 4.4e-6 at 4096, 1.9e-5 at 16384, 7.6e-5 at
 // 65536 (normal numbers; 8e-5 at 16384 where all products have one sign).  In an f32
 // result, such as a weight gradient over many tokens, that is far more than f32's own
-// roundings.  So the kernel of f32 results without an activation, which also makes the
-// parts, cuts a tile's contraction into chunks of 1024 at most, which take the two
-// accumulators in turn, and its finishing warps add them up in registers, rounding as
-// f32 does: 1e-6 at any k.  1024 x 4096 x 16384 takes 108 us for 105, 4096 x 4096 x 65536
-// 1640 for 1630 (chunks of 4096, 4.4e-6: 106 and 1600).  Half a step of a 16-bit result
-// is 20 times and more what it would gain, at 130 us for 109 (16384 x 1024 x 4096, chunks
-// of 2048); with an activation there are no 64 registers to spare.
-constexpr int CHUNK = 16;  // blocks of the contraction
-constexpr bool adds_chunks(bool f32, int32_t act) { return f32 && act == CHELIS_ACT_NONE; }
+// roundings.  So the kernels without an activation, whose contraction may be the long
+// one (the f32 kernel also makes the parts), cut a tile's contraction into chunks, which
+// take the two accumulators in turn, and their finishing warps add them up in registers,
+// rounding as f32 does.  f32 results by chunks of 1024 at most: 1e-6 at any k, 1024 x 4096 x
+// 16384 108 us for 105, 4096 x 4096 x 65536 1640 for 1630 (chunks of 4096, 4.4e-6: 106 and
+// 1600).  16-bit results by chunks of 16384, whose drift is below half a step of f16 by a
+// factor of 3 even where all products have one sign; smaller ones would not show, at 130
+// us for 109 (16384 x 1024 x 4096, chunks of 2048).  With an activation there are no 64
+// registers to spare.
+constexpr int CHUNK_F32 = 16, CHUNK_16 = 256;  // blocks of the contraction
+constexpr bool adds_chunks(int32_t act) { return act == CHELIS_ACT_NONE; }
 constexpr int MOST_PIECES = TN / (4 * PIECE);
 struct Chunks {
     int count, blocks;  // of a tile, of a chunk (the last one may have fewer)
 };
-template <bool LONG>
+template <bool LONG, bool F32>
 __device__ __forceinline__ Chunks chunks_of(int kbs) {
     if constexpr (!LONG) return {1, kbs};
-    const int count = (kbs + CHUNK - 1) / CHUNK;
+    constexpr int MOST = F32 ? CHUNK_F32 : CHUNK_16;
+    const int count = (kbs + MOST - 1) / MOST;
     return {count, (kbs + count - 1) / count};
 }
 __device__ __forceinline__ int pieces_of(const Params &p, int col0) {
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int mt = static_cast<int>((p.m + TM - 1) / TM), nt = static_cast<int>((p.n + p.tn - 1) / p.tn);
     const int tiles = uniform(mt * nt * p.parts);
-    constexpr bool LONG = adds_chunks(F32, ACT);
+    constexpr bool LONG = adds_chunks(ACT);
     int32_t issued = 0;
 
     if (warp < 4) {
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int L = worker; ok && L < tiles; L += workers) {
                 const int kbs = p.parts > 1 ? uniform(tile_at(p, mt, nt, L).kbs) : p.kblocks;
                 if constexpr (LONG) {
-                    const int most = uniform(chunks_of<LONG>(kbs).blocks);
+                    const int most = uniform(chunks_of<LONG, F32>(kbs).blocks);
                     for (int left = kbs; ok && left > 0; left -= most) chunk(min(left, most));
                 } else {
                     chunk(kbs);
@@ -603,6 +606,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
             if (lane == 0) arrive_relaxed(mapa_shared(smem_u32(&acc_empty[use & 1]), 0));
         };
+        // taken on an abort too: the copies land before the block leaves
+        auto aux_landed = [&] {
+            if (ok) ok = all(wait(aux_bar, (aux_count - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE));
+            else landed(aux_bar, (aux_count - 1) & 1, tries);
+        };
         for (int L = worker; ok && L < tiles; L += workers, ++use) {
             const Tile t = tile_at(p, mt, nt, L);
             const int row0 = t.m0 + static_cast<int>(rank) * BM + quad * 32, col0 = t.n0 + side * span;
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 ++aux_count;
             }
             if constexpr (LONG) {
-                const int chunks = chunks_of<LONG>(t.kbs).count;
+                const int chunks = chunks_of<LONG, F32>(t.kbs).count;
                 if (chunks > 1) {
                     f32x2 sum[MOST_PIECES][PIECE / 2] = {};
                     const int pieces = pieces_of(p, col0);
@@ -632,13 +640,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (live) add_chunk(sums_at(), pieces, sum);
                         release();
                     }
+                    if (aux_tma && live) aux_landed();
                     if (!ok) break;
                     unsigned char *box = boxes;
                     if (live)
 #pragma unroll
                         for (int i = 0; i < MOST_PIECES; ++i)
                             if (i < pieces)
-                                finish_piece<F32, BF, ACT>(p, &map_out, boxes, box, used, lane, row0, rows, col0, t.part, false,
+                                finish_piece<F32, BF, ACT>(p, &map_out, boxes, box, used, lane, row0, rows, col0, t.part, aux_tma,
                                                            constants, i, pieces, [&](f32x2 (&v)[PIECE / 2]) {
 #pragma unroll
                                     for (int c = 0; c < PIECE / 2; ++c) v[c] = sum[i][c];
@@ -647,11 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             ok = landed_sums();
-            if (aux_tma && live) {
-                // taken on an abort too: the copies land before the block leaves
-                if (ok) ok = all(wait(aux_bar, (aux_count - 1) & 1, tries, abort_flag, DEVERR_TIMEOUT_EPILOGUE));
-                else landed(aux_bar, (aux_count - 1) & 1, tries);
-            }
+            if (aux_tma && live) aux_landed();
             if (!ok) break;
             tc_fence_after();
             if (live)

@@ -694,8 +694,8 @@ int chelis_cuda_matmul8_wgrad(int32_t format_a, int32_t format_b, int64_t n, int
 enum { CHELIS_ACT_NONE = 0, CHELIS_ACT_RELU = 1, CHELIS_ACT_GELU = 2, CHELIS_ACT_SILU = 3 };
 /* z = op(a) . op(b) + bias and out = act(z) + residual, [m][n] of out_dtype, from
  * bf16 or f16 matrices a [m][k] ([k][m] when trans_a) and b [k][n] ([n][k] when
- * trans_b); sums f32 (those of f32 results without an activation added up from chunks of
- * 1024 of k), act taken of them, each result rounded once.  gelu is
+ * trans_b); sums f32 (without an activation added up from chunks of k, 1024 for f32 results,
+ * 16384 for others), act taken of them, each result rounded once.  gelu is
  * z Phi(z), silu z / (1 + e^-z).  bias [n] (f32 or dtype), residual, pre (where z
  * is stored) and through [m][n] may be NULL; residual, pre and through have
  * out_dtype, which is f32 or dtype.  With through, out is instead the gradient

@@ -470,3 +470,40 @@ def test_residual_may_be_the_result_in_f32_and_in_parts(cuda, m, n, k, out):
         L.call("chelis_cuda_matmul16", L.DTYPE_F16, 0, 0, m, n, k, a.data_ptr(), b.data_ptr(), None, 0, act, r.data_ptr(), None,
                None, code, r.data_ptr())
         assert torch.equal(want, r)
+
+
+@pytest.mark.parametrize("m,n,k,residual", [(512, 5000, 131072, False), (512, 5000, 131072, True), (300, 2600, 100001, True),
+                                            (257, 5003, 40000, True)])
+def test_long_sums_of_16_bits_do_not_drift(cuda, m, n, k, residual):
+    """As above in chunks of 16384: 1024 MMAs on a sum that grows evenly, 1024 / 2 *
+    2^-22 = 2^-13 of it, twice that for the unevenness, and half a step."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    for dtype in DT:
+        a = torch.randn((k, m), generator=gen, device="cuda").abs().to(_t(dtype))
+        b = (torch.randn((k, n), generator=gen, device="cuda").abs() * 0.25).to(_t(dtype))
+        res = torch.randn((m, n), generator=gen, device="cuda").to(_t(dtype)) if residual else None
+        got = cuda.matmul16(a, b, trans_a=True, residual=res)
+        ref = a.double().t() @ b.double()
+        bound = (2.0 ** -12 * ref).cpu().numpy()
+        if residual:
+            ref += res.double()
+        S.check(got, ref.cpu().numpy(), bound, dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 5000, 17000), (300, 5003, 33000), (513, 2600, 16385)])
+def test_long_contractions_of_16_bits_are_added_up(cuda, m, n, k):
+    """Whole numbers with everything that may follow the sums; two numbers in a
+    hundred are not 0, so that the results are whole in 16 bits nearly all."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k)
+
+    def whole(shape, dtype):
+        x = torch.randint(-2, 3, shape, generator=gen, device="cuda")
+        return (x * (torch.rand(shape, generator=gen, device="cuda") < 0.02)).to(_t(dtype))
+
+    for dtype in DT:
+        a, b, bias, res = whole((m, k), dtype), whole((k, n), dtype), whole((n,), dtype), whole((m, n), dtype)
+        y, pre = cuda.matmul16(a, b, bias=bias, residual=res, keep_pre=True)
+        z = a.double() @ b.double() + bias.double()
+        assert torch.equal(pre, z.to(_t(dtype))) and torch.equal(y, (z + res.double()).to(_t(dtype)))
