@@ -910,9 +910,9 @@ def matmul16(a: torch.Tensor, b: torch.Tensor, trans_a: bool = False, trans_b: b
     """act(op(a).op(b) + bias) + residual of two bf16 or two f16 matrices: f32
     sums on the tensor cores, what follows them in the same kernel, one
     rounding to dtype (f32 or the operands' own, the default).  The tensor
-    core's sums are 4e-6 off at k = 4096 and 2e-5 at 16384; results without an
-    activation are added up from chunks, and so f32 ones 1e-6 off and others no
-    more than that 2e-5 at any k.  activation is
+    core's sums of normal numbers are 4e-6 off at k = 4096 and 2e-5 at 16384;
+    without an activation they are added up from chunks, so that f32 results are
+    1e-6 off and 16-bit ones no more than those 2e-5 at any k.  activation is
     relu, gelu (exact) or silu; bias [n] is f32 or of the operands' type, and
     residual [m, n] of dtype.  keep_pre: (y, z) with z = op(a).op(b) + bias, what
     the activation's gradient needs.
